@@ -14,6 +14,8 @@ from .kernel import (Acc, Dot, NumericPolicy, Order, Quant, Scaling, Window, ama
                      per_tensor_scale_dev, probe_fp32, probe_fp64, gemm_dev, gemm_launches,
                      gemm_route, quantize_dev, set_thin_tiles, ROUTE_DOUBLE, ROUTE_FP32,
                      ROUTE_SCANNED, ROUTE_STAGED, ROUTE_PROVEN)
+from .native import (AdamW, Mx4, linear_xent_dev, linear_xent_grad_dev, linear_xent_mean_dev,
+                     mx4_dequantize_dev, mx4_gemm_dev, mx4_quantize_dev)
 from . import policies
 
 _lib.load()
@@ -22,4 +24,6 @@ __all__ = ["Context", "DriftError", "Formats", "MiniFloat", "Rng", "Rounding", "
            "Dot", "NumericPolicy", "Order", "Quant", "Scaling", "Window", "contraction", "contract",
            "contract_dev", "gemm", "gemm_dev", "gemm_launches", "gemm_route", "quantize_dev",
            "ROUTE_DOUBLE", "ROUTE_FP32", "ROUTE_SCANNED", "ROUTE_STAGED", "ROUTE_PROVEN", "set_thin_tiles",
-           "amax_dev", "check_dev", "policies"]
+           "amax_dev", "check_dev", "policies", "AdamW", "Mx4", "linear_xent_dev",
+           "linear_xent_grad_dev", "linear_xent_mean_dev", "mx4_dequantize_dev", "mx4_gemm_dev",
+           "mx4_quantize_dev"]

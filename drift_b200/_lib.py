@@ -51,6 +51,38 @@ class DriftContraction(ctypes.Structure):
         ("accumulate", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class DriftMx4(ctypes.Structure):
+    """struct drift_mx4 (include/drift_b200.h)."""
+
+    _fields_ = [("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("codes", ctypes.c_void_p),
+                ("scales", ctypes.c_void_p)]
+
+
+class DriftXent(ctypes.Structure):
+    """struct drift_xent (include/drift_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("tokens", "depth", "vocab", "x_stride", "w_stride")] \
+        + [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "targets")] \
+        + [("ignore_index", ctypes.c_int64), ("target_bits", ctypes.c_int32),
+           ("type", ctypes.c_int32)]
+
+
+class DriftAdamW(ctypes.Structure):
+    """struct drift_adamw (include/drift_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] \
+        + [("state_bits", ctypes.c_int32), ("rounding", ctypes.c_int32)]
+
+
+class DriftAdamWTensor(ctypes.Structure):
+    """struct drift_adamw_tensor (include/drift_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "m", "v", "m_scale", "v_scale",
+                                               "copy")] \
+        + [("n", ctypes.c_int64)] \
+        + [(n, ctypes.c_int32) for n in ("param_type", "grad_type", "copy_type", "reserved")]
+
+
 # Every exported symbol with its ctypes signature, in header order.
 _P = ctypes.POINTER
 _vp, _i32, _i64, _d = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_double
@@ -106,6 +138,19 @@ SIGNATURES = {
     "drift_tanh_backward_dev": (_int, [_vp, _vp, _vp, _i64, _vp]),
     "drift_scale_for_dev": (_int, [_vp, _int, _vp, _vp, _i32, _vp, _vp, _vp]),
     "drift_adam_dev": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _d, _i32, _vp]),
+    "drift_mx4_sizes": (_int, [_i64, _i64, _P(_i64), _P(_i64)]),
+    "drift_mx4_quantize_dev": (_int, [_vp, _P(DriftPolicy), _int, _int, _vp, _i64, _i64, _i64, _vp,
+                                      _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "drift_mx4_dequantize_dev": (_int, [_vp, _P(DriftMx4), _int, _vp, _i64, _vp]),
+    "drift_mx4_gemm_workspace": (_int, [_i64, _i64, _i64, _P(_i64)]),
+    "drift_mx4_gemm_dev": (_int, [_vp, _P(DriftMx4), _P(DriftMx4), _vp, _int, _vp, _i64, _vp, _i64,
+                                  _vp]),
+    "drift_linear_xent_workspace": (_int, [_P(DriftXent), _int, _P(_i64)]),
+    "drift_linear_xent_dev": (_int, [_vp, _P(DriftXent), _vp, _vp, _vp, _vp, _i64, _vp]),
+    "drift_linear_xent_grad_dev": (_int, [_vp, _P(DriftXent), _vp, _vp, _i64, _vp, _i64, _vp, _i64,
+                                          _vp, _vp, _i64, _vp]),
+    "drift_adamw_dev": (_int, [_vp, _P(DriftAdamW), _P(DriftAdamWTensor), _i64, _vp, _vp, _vp, _vp,
+                               _vp, _vp]),
     "drift_probe_fp64": (_int, [_vp, _P(_d)]),
     "drift_probe_fp32": (_int, [_vp, _P(_d)]),
     "drift_check_dev": (_int, [_vp, _vp]),

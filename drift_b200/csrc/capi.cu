@@ -184,7 +184,7 @@ static int take_device_error(drift_ctx *ctx, cudaStream_t st) {
     if (flags & DEV_ERR_NAN_FINITE) return fail(DRIFT_ENAN_FINITE, "NaN cast into a format without NaN");
     if (flags & DEV_ERR_NO_RNG) return fail(DRIFT_EINVAL, "stochastic rounding needs an Rng");
     if (flags & DEV_ERR_TIMEOUT) return fail(DRIFT_ETIMEOUT, "device wait gave up");
-    if (flags & DEV_ERR_INDEX) return fail(DRIFT_EINVAL, "token outside the embedding table");
+    if (flags & DEV_ERR_INDEX) return fail(DRIFT_EINVAL, "token outside the embedding table or vocabulary");
     return DRIFT_OK;
 }
 
@@ -1157,6 +1157,219 @@ int drift_adam_dev(drift_ctx *ctx, double *d_param, const double *d_grad, double
     rc = launch_adam(d_param, d_grad, d_m, d_v, n, c1, c2, lr, fp32_master ? 1 : 0,
                      pick(ctx, stream));
     return rc ? fail(rc, "adam") : DRIFT_OK;
+}
+
+// ------------------------------------------------------------------ native operators
+
+// Makes the context's device current for one call.
+namespace {
+struct DeviceScope {
+    int before = -1, status = DRIFT_OK;
+    explicit DeviceScope(drift_ctx *ctx) {
+        if (!ctx) {
+            status = fail(DRIFT_EINVAL, "null context");
+            return;
+        }
+        cudaError_t e = cudaGetDevice(&before);
+        if (e == cudaSuccess && before == ctx->device) before = -1;
+        else if (e == cudaSuccess) e = cudaSetDevice(ctx->device);
+        if (e != cudaSuccess) status = cuda_fail(e, "cudaSetDevice");
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+}  // namespace
+
+static bool misaligned(const void *p, unsigned to) {
+    return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0;
+}
+
+// Rows and columns that the packed form's 32-bit indices reach.
+static bool mx4_shape_ok(int64_t rows, int64_t cols) {
+    return rows >= 0 && cols >= 0 && rows < (1LL << 31) && cols < (1LL << 31) &&
+           ((rows + 127) / 128 * 128) * ((cols + 255) / 256) < (1LL << 32);
+}
+
+int drift_mx4_sizes(int64_t rows, int64_t cols, int64_t *code_bytes, int64_t *scale_bytes) {
+    if (!mx4_shape_ok(rows, cols)) return fail(DRIFT_EINVAL, "bad shape");
+    if (code_bytes) *code_bytes = rows * ((cols + 31) / 32 * 16);
+    if (scale_bytes) *scale_bytes = (rows + 127) / 128 * ((cols + 255) / 256 * 2) * 512;
+    return DRIFT_OK;
+}
+
+int drift_mx4_quantize_dev(drift_ctx *ctx, const drift_policy *p, int rounding, int type,
+                           const void *d_src, int64_t rows, int64_t cols, int64_t row_stride,
+                           uint8_t *d_codes, uint8_t *d_scales, uint8_t *d_codes_t,
+                           uint8_t *d_scales_t, uint64_t *d_rng_state, int64_t *d_clamped,
+                           int64_t *d_clamped_t, void *stream) {
+    DeviceScope scope(ctx);
+    if (scope.status) return scope.status;
+    if (!p || type < 0 || type > 3 || !mx4_shape_ok(rows, cols) || !mx4_shape_ok(cols, rows) ||
+        (rows > 1 && row_stride < cols) || rounding < 0 || rounding > 2)
+        return fail(DRIFT_EINVAL, "bad arguments");
+    if (p->scaling != DRIFT_MX_BLOCK || p->scale_block != 32 ||
+        (p->input_format != DRIFT_E2M1 && p->grad_format != DRIFT_E2M1))
+        return fail(DRIFT_EINVAL, "the packed cast needs e2m1 elements and MX blocks of 32");
+    if (p->mx_headroom < -1024 || p->mx_headroom > 1024) return fail(DRIFT_EINVAL, "bad headroom");
+    if (rounding == DRIFT_STOCHASTIC && !d_rng_state)
+        return fail(DRIFT_EINVAL, "stochastic rounding needs an Rng");
+    if (rows == 0 || cols == 0) return DRIFT_OK;
+    if (!d_src || !d_codes != !d_scales || !d_codes_t != !d_scales_t || (!d_codes && !d_codes_t))
+        return fail(DRIFT_EINVAL, "null pointer");
+    if (misaligned(d_codes, 16) || misaligned(d_scales, 16) || misaligned(d_codes_t, 16) ||
+        misaligned(d_scales_t, 16))
+        return fail(DRIFT_EINVAL, "codes and scales must be 16-byte aligned");
+    const int rc = launch_mx4_quantize(
+        p->mx_headroom, rounding, type, d_src, rows, cols, rows > 1 ? row_stride : cols, d_codes,
+        d_scales, d_codes_t, d_scales_t, d_rng_state, (unsigned long long *)d_clamped,
+        (unsigned long long *)d_clamped_t, ctx->d_err(), pick(ctx, stream));
+    return rc ? fail(rc, "mx4 quantize launch") : DRIFT_OK;
+}
+
+static int check_mx4(const drift_mx4 *q) {
+    if (!q || !mx4_shape_ok(q->rows, q->cols)) return fail(DRIFT_EINVAL, "bad packed matrix");
+    if (q->rows && q->cols && (!q->codes || !q->scales))
+        return fail(DRIFT_EINVAL, "null pointer");
+    if (misaligned(q->codes, 16) || misaligned(q->scales, 16))
+        return fail(DRIFT_EINVAL, "codes and scales must be 16-byte aligned");
+    return DRIFT_OK;
+}
+
+int drift_mx4_dequantize_dev(drift_ctx *ctx, const drift_mx4 *q, int type, void *d_dst,
+                             int64_t row_stride, void *stream) {
+    DeviceScope scope(ctx);
+    if (scope.status) return scope.status;
+    int rc = check_mx4(q);
+    if (rc) return rc;
+    if (type < 0 || type > 3 || (q->rows > 1 && row_stride < q->cols))
+        return fail(DRIFT_EINVAL, "bad arguments");
+    if (q->rows == 0 || q->cols == 0) return DRIFT_OK;
+    if (!d_dst) return fail(DRIFT_EINVAL, "null pointer");
+    rc = launch_mx4_dequantize(q, type, d_dst, q->rows > 1 ? row_stride : q->cols,
+                               pick(ctx, stream));
+    return rc ? fail(rc, "mx4 dequantize launch") : DRIFT_OK;
+}
+
+int drift_mx4_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes) {
+    if (!bytes || !mx4_shape_ok(M, K) || !mx4_shape_ok(N, K))
+        return fail(DRIFT_EINVAL, "bad shape");
+    *bytes = mx4_gemm_workspace(M, N, K);
+    return DRIFT_OK;
+}
+
+int drift_mx4_gemm_dev(drift_ctx *ctx, const drift_mx4 *A, const drift_mx4 *B,
+                       const float *d_bias, int type, void *d_C, int64_t c_stride, void *d_ws,
+                       int64_t ws_bytes, void *stream) {
+    DeviceScope scope(ctx);
+    if (scope.status) return scope.status;
+    int rc = check_mx4(A);
+    if (!rc) rc = check_mx4(B);
+    if (rc) return rc;
+    if (A->cols != B->cols || type < 0 || type > 3 || (A->rows > 1 && c_stride < B->rows))
+        return fail(DRIFT_EINVAL, "bad arguments");
+    if (A->rows == 0 || B->rows == 0) return DRIFT_OK;
+    if (!d_C) return fail(DRIFT_EINVAL, "null pointer");
+    const int64_t need = mx4_gemm_workspace(A->rows, B->rows, A->cols);
+    if (need && (!d_ws || ws_bytes < need || misaligned(d_ws, 256)))
+        return fail(DRIFT_EINVAL, "workspace too small or misaligned");
+    rc = launch_mx4_gemm(A, B, d_bias, type, d_C, A->rows > 1 ? c_stride : B->rows, d_ws,
+                         ctx->d_err(), pick(ctx, stream));
+    return rc ? fail(rc, "mx4 gemm launch") : DRIFT_OK;
+}
+
+static int check_xent(const drift_xent *op) {
+    if (!op || op->tokens < 0 || op->depth < 1 || op->vocab < 1 || op->tokens >= (1LL << 31) ||
+        op->depth >= (1LL << 31) || op->vocab >= (1LL << 31))
+        return fail(DRIFT_EINVAL, "bad shape");
+    if ((op->type != DRIFT_T_BF16 && op->type != DRIFT_T_FP16) ||
+        (op->target_bits != 32 && op->target_bits != 64))
+        return fail(DRIFT_EINVAL, "bad type");
+    if (op->x_stride < op->depth || op->w_stride < op->depth || op->x_stride % 8 ||
+        op->w_stride % 8 || op->x_stride >= (1LL << 38) || op->w_stride >= (1LL << 38) ||
+        misaligned(op->x, 16) || misaligned(op->w, 16))
+        return fail(DRIFT_EINVAL, "rows of x and w must be 16-byte aligned");
+    if (op->tokens && (!op->x || !op->w || !op->targets)) return fail(DRIFT_EINVAL, "null pointer");
+    return DRIFT_OK;
+}
+
+int drift_linear_xent_workspace(const drift_xent *op, int grad, int64_t *bytes) {
+    if (!op || !bytes || op->tokens < 0 || op->depth < 1 || op->vocab < 1)
+        return fail(DRIFT_EINVAL, "bad shape");
+    *bytes = xent_workspace(op, grad != 0);
+    return DRIFT_OK;
+}
+
+int drift_linear_xent_dev(drift_ctx *ctx, const drift_xent *op, float *d_loss, float *d_lse,
+                          float *d_mean, void *d_ws, int64_t ws_bytes, void *stream) {
+    DeviceScope scope(ctx);
+    if (scope.status) return scope.status;
+    int rc = check_xent(op);
+    if (rc) return rc;
+    if (op->tokens && !d_lse) return fail(DRIFT_EINVAL, "null pointer");
+    if (!d_ws || ws_bytes < xent_workspace(op, false) || misaligned(d_ws, 256))
+        return fail(DRIFT_EINVAL, "workspace too small or misaligned");
+    rc = launch_xent(op, d_loss, d_lse, d_mean, d_ws, ctx->d_err(), pick(ctx, stream));
+    return rc ? fail(rc, "linear cross entropy launch") : DRIFT_OK;
+}
+
+int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, const float *d_lse,
+                               const float *d_dloss, int64_t dloss_stride, void *d_dx,
+                               int64_t dx_stride, void *d_dw, int64_t dw_stride, float *d_db,
+                               void *d_ws, int64_t ws_bytes, void *stream) {
+    DeviceScope scope(ctx);
+    if (scope.status) return scope.status;
+    int rc = check_xent(op);
+    if (rc) return rc;
+    if ((op->tokens && (!d_lse || !d_dloss)) || dloss_stride < 0)
+        return fail(DRIFT_EINVAL, "bad arguments");
+    if ((d_dx && dx_stride < op->depth) || (d_dw && dw_stride < op->depth))
+        return fail(DRIFT_EINVAL, "bad stride");
+    if (!d_ws || ws_bytes < xent_workspace(op, true) || misaligned(d_ws, 256))
+        return fail(DRIFT_EINVAL, "workspace too small or misaligned");
+    rc = launch_xent_grad(op, d_lse, d_dloss, dloss_stride, d_dx, dx_stride, d_dw, dw_stride,
+                          d_db, d_ws, ctx->d_err(), pick(ctx, stream));
+    return rc ? fail(rc, "linear cross entropy gradient launch") : DRIFT_OK;
+}
+
+int drift_adamw_dev(drift_ctx *ctx, const drift_adamw *h, const drift_adamw_tensor *tensors,
+                    int64_t count, int64_t *d_step, float *d_scalars, const float *d_lr,
+                    const float *d_grad_scale, uint64_t *d_rng_state, void *stream) {
+    DeviceScope scope(ctx);
+    if (scope.status) return scope.status;
+    if (!h || count < 0 || (count && !tensors) || !d_step || !d_scalars ||
+        misaligned(d_scalars, 8))
+        return fail(DRIFT_EINVAL, "bad arguments");
+    if ((h->state_bits != 32 && h->state_bits != 8) ||
+        !(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1 && h->eps >= 0))
+        return fail(DRIFT_EINVAL, "bad hyperparameters");
+    if (h->rounding != DRIFT_NEAREST_EVEN &&
+        (h->rounding != DRIFT_STOCHASTIC || h->state_bits != 8))
+        return fail(DRIFT_EINVAL, "bad rounding");
+    if (h->rounding == DRIFT_STOCHASTIC && !d_rng_state)
+        return fail(DRIFT_EINVAL, "stochastic rounding needs an Rng");
+    for (int64_t i = 0; i < count; i++) {
+        const drift_adamw_tensor &t = tensors[i];
+        const auto bad_type = [](int32_t y) { return y < DRIFT_T_F32 || y > DRIFT_T_FP16; };
+        if (t.n < 0 || t.n >= (1LL << 40) || t.reserved) return fail(DRIFT_EINVAL, "bad tensor");
+        if (t.n == 0) continue;
+        if (bad_type(t.param_type) || bad_type(t.grad_type) || (t.copy && bad_type(t.copy_type)))
+            return fail(DRIFT_EINVAL, "bad tensor type");
+        if ((!t.param || !t.grad || !t.m || !t.v ||
+                    (h->state_bits == 8 && (!t.m_scale || !t.v_scale))))
+            return fail(DRIFT_EINVAL, "null pointer");
+        const unsigned pa = t.param_type == DRIFT_T_F32 ? 4 : 2;
+        const unsigned ga = t.grad_type == DRIFT_T_F32 ? 4 : 2;
+        const unsigned ca = t.copy && t.copy_type == DRIFT_T_F32 ? 4 : 2;
+        const unsigned sa = h->state_bits == 32 ? 4 : 1;
+        if (misaligned(t.param, pa) || misaligned(t.grad, ga) || misaligned(t.copy, ca) ||
+            misaligned(t.m, sa) || misaligned(t.v, sa) || misaligned(t.m_scale, 4) ||
+            misaligned(t.v_scale, 4))
+            return fail(DRIFT_EINVAL, "misaligned tensor");
+    }
+    const int rc = launch_adamw(h, tensors, count, d_step, d_scalars, d_lr, d_grad_scale,
+                                d_rng_state, pick(ctx, stream));
+    return rc ? fail(rc, "adamw launch") : DRIFT_OK;
 }
 
 int drift_check_dev(drift_ctx *ctx, void *stream) {

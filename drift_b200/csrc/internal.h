@@ -148,6 +148,30 @@ int launch_scale_for(int fmt, const double *amax_now, double *hist, int32_t len,
 int launch_adam(double *p, const double *g, double *m, double *v, int64_t n, double c1, double c2,
                 double lr, int fp32, cudaStream_t st);
 
+// mx4.cu
+int launch_mx4_quantize(int headroom, int rm, int type, const void *src, int64_t rows,
+                        int64_t cols, int64_t row_stride, uint8_t *codes, uint8_t *scales,
+                        uint8_t *codes_t, uint8_t *scales_t, uint64_t *d_state,
+                        unsigned long long *clamped, unsigned long long *clamped_t, int *d_err,
+                        cudaStream_t st);
+int launch_mx4_dequantize(const drift_mx4 *q, int type, void *dst, int64_t stride,
+                          cudaStream_t st);
+// mx4_gemm.cu
+int64_t mx4_gemm_workspace(int64_t M, int64_t N, int64_t K);
+int launch_mx4_gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, int type, void *C,
+                    int64_t c_stride, void *ws, int *d_err, cudaStream_t st);
+// xent.cu
+int64_t xent_workspace(const drift_xent *op, bool grad);
+int launch_xent(const drift_xent *op, float *loss, float *lse, float *mean, void *ws, int *err,
+                cudaStream_t st);
+int launch_xent_grad(const drift_xent *op, const float *lse, const float *g, int64_t g_stride,
+                     void *dx, int64_t dx_stride, void *dw, int64_t dw_stride, float *db, void *ws,
+                     int *err, cudaStream_t st);
+// adamw.cu
+int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_t count,
+                 int64_t *d_step, float *d_scalars, const float *d_lr, const float *d_grad_scale,
+                 uint64_t *d_rng, cudaStream_t st);
+
 // Streaming multiprocessors of the current device (148 on B200), used to size
 // grid-stride launches; 148 if the query fails.
 inline int sm_count() {

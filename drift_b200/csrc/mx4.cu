@@ -1,0 +1,490 @@
+// mx4.cu — microscaled 4-bit floating point as the hardware holds it: the cast
+// into packed e2m1 codes and power-of-two scales, and back to values.
+//
+// The numbers are those of Quant.quantize's MX cast with e2m1 elements and
+// blocks of 32 (java/src/main/java/io/drift/kernel/Quant.java:95-123): block
+// exponent floor(log2 amax) - 2 + headroom within [-127, 127], NaN ignored in
+// amax, blocks whose amax is 0 or Inf held as zeros, elements rounded and
+// saturated at 6, values above 6 before rounding counted as clamped. Blocks
+// start afresh in every row, since a product contracts rows.
+//
+// Bound: HBM bytes (the source once, 17/32 byte an element out, for each
+// direction of blocks). Along rows a lane takes eight elements, so four lanes
+// share a block and its amax is two shuffles. Down columns a CTA stages a tile
+// of 128 x 64 in shared memory; where both directions are wanted they read the
+// same tile, so the source is read once.
+#include <algorithm>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "codec.cuh"
+#include "internal.h"
+#include "mx4.cuh"
+
+namespace drift {
+
+// ------------------------------------------------------------------ one block's arithmetic
+
+template <int TYPE> struct MxSrc;
+template <> struct MxSrc<DRIFT_T_F64> {
+    using T = double;
+    using V = double;
+    __device__ static V get(T x) { return x; }
+};
+template <> struct MxSrc<DRIFT_T_F32> {
+    using T = float;
+    using V = float;
+    __device__ static V get(T x) { return x; }
+};
+template <> struct MxSrc<DRIFT_T_BF16> {
+    using T = __nv_bfloat16;
+    using V = float;
+    __device__ static V get(T x) { return __bfloat162float(x); }
+};
+template <> struct MxSrc<DRIFT_T_FP16> {
+    using T = __half;
+    using V = float;
+    __device__ static V get(T x) { return __half2float(x); }
+};
+
+// Magnitude for amax: NaN counts as nothing (Quant.java:25-34).
+__device__ __forceinline__ float mx_mag(float x) { return x == x ? fabsf(x) : 0.0f; }
+__device__ __forceinline__ double mx_mag(double x) { return x == x ? fabs(x) : 0.0; }
+
+// Math.getExponent of the value as a double, so a float subnormal has its own
+// exponent.
+__device__ __forceinline__ int mx_exponent(float a) {
+    const int e = (int)(__float_as_uint(a) >> 23);
+    return e ? e - 127 : -118 - __clz(__float_as_uint(a));  // 31 - clz - 149
+}
+__device__ __forceinline__ int mx_exponent(double a) { return java_get_exponent(a); }
+
+struct MxScale {
+    int shared;  // exponent of the block's scale
+    bool zero;   // amax 0 or Inf: the block is held as zeros
+};
+
+template <class V>
+__device__ __forceinline__ MxScale mx_scale(V amax, int headroom) {
+    MxScale s;
+    s.zero = !(amax > (V)0) || isinf(amax);
+    const int e = mx_exponent(amax) - 2 + headroom;
+    s.shared = s.zero ? 0 : max(-127, min(127, e));
+    return s;
+}
+
+// x * 2^-shared: exact, except far below the smallest code.
+__device__ __forceinline__ float mx_scaled(float x, int shared) {
+    const unsigned up = (unsigned)(127 - shared) << 23;
+    return x * (shared < 127 ? __uint_as_float(up) : 0x1p-127f);
+}
+__device__ __forceinline__ double mx_scaled(double x, int shared) {
+    return __dmul_rn(x, pow2(-shared));
+}
+
+// A double narrowed to float with its lost bits kept as a sticky lowest bit, so
+// that the rounding to e2m1 sees on which side of a midpoint the double was.
+__device__ __forceinline__ float mx_narrow(float x) { return x; }
+__device__ __forceinline__ float mx_narrow(double x) {
+    const float f = __double2float_rz(x);
+    return (double)f == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+
+// Codes of two values to nearest, ties to the even code, saturating at 6: lo in
+// bits 0-3, hi in bits 4-7.
+__device__ __forceinline__ unsigned mx_rn2(float lo, float hi) {
+    unsigned out;
+    asm("{\n .reg .b8 t, z;\n cvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 z, %3, %3;\n mov.b32 %0, {t, z, z, z};\n}"
+        : "=r"(out)
+        : "f"(hi), "f"(lo), "f"(0.0f));
+    return out;
+}
+
+// The code toward zero of |x| <= 6, and its value.
+__device__ __forceinline__ unsigned mx_floor(float a, float &base) {
+    if (a < 1.0f) {
+        base = a >= 0.5f ? 0.5f : 0.0f;
+        return a >= 0.5f;
+    }
+    const unsigned b = __float_as_uint(a);
+    base = __uint_as_float(b & 0xffc00000u);
+    return (b >> 22) - (127u * 2 - 2);  // 1 -> 2, 1.5 -> 3, 2 -> 4, ... 6 -> 7
+}
+
+// Code of one scaled value under truncation or stochastic rounding (u53: its
+// draw). The fraction of the step that truncation drops is exact in V; Java
+// rounds up where nextDouble() is below it (MiniFloat.java:264-273).
+template <class V>
+__device__ __forceinline__ unsigned mx_code(V x, int rm, uint64_t u53) {
+    const V a = fmin(fabs(x), (V)6);
+    float base;
+    unsigned code = mx_floor(sizeof(V) == 8 ? __double2float_rz((double)a) : (float)a, base);
+    if (rm == DRIFT_STOCHASTIC) {
+        const V frac = (a - (V)base) * (base < 2.0f ? (V)2 : base < 4.0f ? (V)1 : (V)0.5);
+        if (u53_to_double(u53) * 0x1p-53 < (double)frac) code++;
+    }
+    return code | (signbit(x) ? 8u : 0u);
+}
+
+// Eight values of one block (or zeros past the end) to 32 bits of codes.
+// `draw` is the index of element 0's draw, `step` the distance to the next
+// element's.
+template <class V>
+__device__ __forceinline__ unsigned mx_pack8(const V (&x)[8], const MxScale &s, int rm,
+                                             uint64_t state, uint64_t draw, uint64_t step,
+                                             int valid, unsigned &clamps, int &err) {
+    V y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        V v = j < valid ? x[j] : (V)0;
+        if (v != v) {  // the format has no NaN: flagged, held as +0
+            if (!s.zero) err |= DEV_ERR_NAN_FINITE;
+            v = (V)0;
+        }
+        y[j] = s.zero ? (V)0 : mx_scaled(v, s.shared);
+        clamps += fabs(y[j]) > (V)6;
+    }
+    unsigned w = 0;
+    if (rm == DRIFT_NEAREST_EVEN) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) w |= (mx_rn2(mx_narrow(y[2 * j]), mx_narrow(y[2 * j + 1])) & 0xffu) << (8 * j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint64_t u = rm == DRIFT_STOCHASTIC ? draw_u53(state, draw + j * step) : 0;
+            w |= mx_code(y[j], rm, u) << (4 * j);
+        }
+    }
+    return w;
+}
+
+// ------------------------------------------------------------------ the cast
+
+struct MxCast {
+    const void *src;
+    int64_t rows, cols, row_stride;
+    int headroom, rm;
+    bool vec;                          // rows start 16-byte aligned
+    uint8_t *codes, *scales;           // blocks along rows
+    uint8_t *codes_t, *scales_t;       // blocks down columns: the transpose, packed
+    uint64_t draw_t;                   // first draw of the transposed cast
+    const uint64_t *state;
+    unsigned long long *clamped, *clamped_t;
+    int *err;
+};
+
+template <int TYPE>
+__device__ __forceinline__ void mx_load8(const MxCast &a, int64_t row, int64_t col, int valid,
+                                         typename MxSrc<TYPE>::V (&x)[8]) {
+    using S = MxSrc<TYPE>;
+    const typename S::T *p =
+        static_cast<const typename S::T *>(a.src) + row * a.row_stride + col;
+    if (a.vec && valid == 8) {
+        constexpr int kVec = sizeof(typename S::T) * 8 / 16;
+        uint4 w[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; j++) w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
+        const typename S::T *q = reinterpret_cast<const typename S::T *>(w);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = S::get(q[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = j < valid ? S::get(p[j]) : (typename S::V)0;
+    }
+}
+
+__device__ __forceinline__ void mx_finish(unsigned clamps, int err, unsigned long long *clamped,
+                                          int *d_err) {
+    clamps = __reduce_add_sync(0xffffffffu, clamps);
+    err = (int)__reduce_or_sync(0xffffffffu, (unsigned)err);
+    if ((threadIdx.x & 31) == 0) {
+        if (clamped && clamps) atomicAdd(clamped, (unsigned long long)clamps);
+        if (err) atomicOr(d_err, err);
+    }
+}
+
+// Blocks along rows: a warp takes 256 elements of one row (eight blocks, two
+// tiles of scales) at a time. Rows past the end up to the tile's 128, and
+// blocks past the row's end, get their padding bytes.
+template <int TYPE>
+__global__ void __launch_bounds__(256) mx4_rows_kernel(const MxCast a, uint32_t per_row,
+                                                       uint32_t items) {
+    using V = typename MxSrc<TYPE>::V;
+    const int lane = threadIdx.x & 31;
+    const int64_t blocks = mx4_blocks(a.cols), row_bytes = blocks * 16;
+    const uint64_t state = a.rm == DRIFT_STOCHASTIC ? *a.state : 0;
+    unsigned clamps = 0;
+    int err = 0;
+    const uint32_t stride = gridDim.x * 8;
+    for (uint32_t it = blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += stride) {
+        const uint32_t row = it / per_row, chunk = it - row * per_row;
+        const int64_t col = (int64_t)chunk * 256 + lane * 8;
+        const int64_t block = col >> 5;
+        const int valid =
+            row < a.rows ? (int)max((int64_t)0, min((int64_t)8, a.cols - col)) : 0;
+        V x[8];
+        mx_load8<TYPE>(a, row, col, valid, x);
+        V amax = (V)0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) amax = fmax(amax, mx_mag(x[j]));
+        amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const MxScale s = mx_scale(amax, a.headroom);
+        const unsigned w = mx_pack8(x, s, a.rm, state, (uint64_t)row * a.cols + col, 1, valid,
+                                    clamps, err);
+        if (row < a.rows && block < blocks)
+            *reinterpret_cast<unsigned *>(a.codes + row * row_bytes + col / 2) = w;
+        // Lanes 0 and 16 gather the four scale bytes of their tile.
+        const unsigned byte = row < a.rows && block < blocks ? (unsigned)(s.shared + 127) : 127u;
+        unsigned four = byte;
+        four |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
+        four |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
+        four |= __shfl_down_sync(0xffffffffu, byte, 12) << 24;
+        if ((lane & 15) == 0)
+            *reinterpret_cast<unsigned *>(a.scales + mx4_scale_offset(row, block, per_row * 2)) =
+                four;
+    }
+    mx_finish(clamps, err, a.clamped, a.err);
+}
+
+// Blocks down columns (and along rows too, where a.codes is given): a CTA
+// stages 128 rows x 64 columns of the source.
+constexpr int kMxTr = 128, kMxTc = 64;
+
+template <int TYPE>
+__global__ void __launch_bounds__(256) mx4_cols_kernel(const MxCast a, uint32_t row_tiles,
+                                                       uint32_t col_tiles) {
+    using S = MxSrc<TYPE>;
+    using T = typename S::T;
+    using V = typename S::V;
+    // 8 elements of padding a row: column reads by a warp's 32 lanes then touch
+    // consecutive words of one row.
+    constexpr int kLd = kMxTc + 16 / (int)sizeof(T);
+    extern __shared__ __align__(16) unsigned char mx_smem[];
+    T *tile = reinterpret_cast<T *>(mx_smem);
+    const uint32_t tile_r = blockIdx.x / col_tiles, tile_c = blockIdx.x - tile_r * col_tiles;
+    const int64_t r0 = (int64_t)tile_r * kMxTr, c0 = (int64_t)tile_c * kMxTc;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const uint64_t state = a.rm == DRIFT_STOCHASTIC ? *a.state : 0;
+    constexpr int kPer = 16 / sizeof(T), kVecs = kMxTc / kPer;
+    for (int i = tid; i < kMxTr * kVecs; i += 256) {
+        const int r = i / kVecs, c = i % kVecs * kPer;
+        const T *p = static_cast<const T *>(a.src) + (r0 + r) * a.row_stride + c0 + c;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (r0 + r < a.rows) {
+            if (a.vec && c0 + c + kPer <= a.cols) {
+                w = __ldg(reinterpret_cast<const uint4 *>(p));
+            } else {
+                T *q = reinterpret_cast<T *>(&w);
+#pragma unroll
+                for (int j = 0; j < kPer; j++)
+                    if (c0 + c + j < a.cols) q[j] = p[j];
+            }
+        }
+        *reinterpret_cast<uint4 *>(tile + r * kLd + c) = w;
+    }
+    __syncthreads();
+
+    // Down columns: thread = (column, block of 32 rows).
+    {
+        unsigned clamps = 0;
+        int err = 0;
+        const int c = tid & 63, b = tid >> 6;
+        const int64_t col = c0 + c, row = r0 + b * 32;
+        const int64_t k_tiles = mx4_k_tiles(a.rows), blocks = mx4_blocks(a.rows);
+        V amax = (V)0;
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            amax = fmax(amax, mx_mag(S::get(tile[(b * 32 + j) * kLd + c])));
+        const MxScale s = mx_scale(amax, a.headroom);
+        uint4 w;
+        unsigned *wp = reinterpret_cast<unsigned *>(&w);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            V x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = S::get(tile[(b * 32 + q * 8 + j) * kLd + c]);
+            wp[q] = mx_pack8(x, s, a.rm, state,
+                             a.draw_t + (uint64_t)(row + q * 8) * a.cols + col, a.cols, 8, clamps,
+                             err);
+        }
+        if (col < a.cols && row < a.rows)
+            *reinterpret_cast<uint4 *>(a.codes_t + col * blocks * 16 + (row >> 5) * 16) = w;
+        // Scale bytes, with the padding of the last tiles: this CTA's columns up
+        // to the tile's 128 rows, and blocks up to a whole pair of tiles.
+        const int64_t last = mx4_row_tiles(a.cols) * 128;
+        if (col < last) {
+            a.scales_t[mx4_scale_offset(col, row >> 5, k_tiles)] =
+                col < a.cols && row < a.rows ? (uint8_t)(s.shared + 127) : (uint8_t)127;
+            if (tile_r + 1 == row_tiles && tile_r % 2 == 0)
+                a.scales_t[mx4_scale_offset(col, (row >> 5) + 4, k_tiles)] = 127;
+        }
+        mx_finish(clamps, err, a.clamped_t, a.err);
+    }
+    if (!a.codes) return;
+
+    // Along rows: eight elements a thread, four threads a block of 32.
+    {
+        unsigned clamps = 0;
+        int err = 0;
+        const int64_t blocks = mx4_blocks(a.cols), k_tiles = mx4_k_tiles(a.cols);
+#pragma unroll
+        for (int i = 0; i < kMxTr * kMxTc / 8 / 256; i++) {
+            const int at = i * 256 + tid, r = at >> 3, c = (at & 7) * 8;
+            V x[8];
+            V amax = (V)0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[j] = S::get(tile[r * kLd + c + j]);
+                amax = fmax(amax, mx_mag(x[j]));
+            }
+            amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const MxScale s = mx_scale(amax, a.headroom);
+            const int64_t row = r0 + r, col = c0 + c, block = col >> 5;
+            const unsigned w =
+                mx_pack8(x, s, a.rm, state, (uint64_t)row * a.cols + col, 1, 8, clamps, err);
+            const bool in = row < a.rows && block < blocks;
+            if (in) *reinterpret_cast<unsigned *>(a.codes + row * blocks * 16 + col / 2) = w;
+            if ((lane & 3) == 0 && block < k_tiles * 4) {
+                a.scales[mx4_scale_offset(row, block, k_tiles)] =
+                    in ? (uint8_t)(s.shared + 127) : (uint8_t)127;
+                // The last columns' CTA also writes the pair's remaining blocks.
+                if (tile_c + 1 == col_tiles)
+                    for (int64_t b = block + 2; b < k_tiles * 4; b += 2)
+                        a.scales[mx4_scale_offset(row, b, k_tiles)] = 127;
+            }
+        }
+        mx_finish(clamps, err, a.clamped, a.err);
+    }
+}
+
+__global__ void mx4_advance_kernel(uint64_t *state, uint64_t draws) { *state += draws * kGolden; }
+
+template <int TYPE>
+static int launch_cast(const MxCast &a, cudaStream_t st) {
+    using T = typename MxSrc<TYPE>::T;
+    if (!a.codes_t) {
+        const uint32_t per_row = (uint32_t)(mx4_k_tiles(a.cols) / 2);
+        const uint32_t items = (uint32_t)(mx4_row_tiles(a.rows) * 128) * per_row;
+        const uint32_t grid = std::min<uint32_t>((items + 7) / 8, (uint32_t)sm_count() * 8);
+        mx4_rows_kernel<TYPE><<<grid, 256, 0, st>>>(a, per_row, items);
+    } else {
+        constexpr int smem = kMxTr * (kMxTc * (int)sizeof(T) + 16);
+        if (smem > 48 * 1024 &&
+            cudaFuncSetAttribute(mx4_cols_kernel<TYPE>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 smem) != cudaSuccess)
+            return DRIFT_ECUDA;
+        // Columns up to the tile's 128, so that every padding byte is written.
+        const uint32_t row_tiles = (uint32_t)mx4_row_tiles(a.rows);
+        const uint32_t col_tiles = (uint32_t)mx4_row_tiles(a.cols) * 2;
+        mx4_cols_kernel<TYPE><<<row_tiles * col_tiles, 256, smem, st>>>(a, row_tiles, col_tiles);
+    }
+    return DRIFT_OK;
+}
+
+int launch_mx4_quantize(int headroom, int rm, int type, const void *src, int64_t rows,
+                        int64_t cols, int64_t row_stride, uint8_t *codes, uint8_t *scales,
+                        uint8_t *codes_t, uint8_t *scales_t, uint64_t *d_state,
+                        unsigned long long *clamped, unsigned long long *clamped_t, int *d_err,
+                        cudaStream_t st) {
+    static const int size[4] = {8, 4, 2, 2};
+    MxCast a;
+    a.src = src;
+    a.rows = rows, a.cols = cols, a.row_stride = row_stride;
+    a.headroom = headroom, a.rm = rm;
+    a.vec = reinterpret_cast<uintptr_t>(src) % 16 == 0 && row_stride * size[type] % 16 == 0;
+    a.codes = codes, a.scales = scales, a.codes_t = codes_t, a.scales_t = scales_t;
+    a.draw_t = codes ? (uint64_t)rows * cols : 0;
+    a.state = d_state;
+    a.clamped = clamped, a.clamped_t = clamped_t;
+    a.err = d_err;
+    int rc;
+    switch (type) {
+        case DRIFT_T_F64: rc = launch_cast<DRIFT_T_F64>(a, st); break;
+        case DRIFT_T_F32: rc = launch_cast<DRIFT_T_F32>(a, st); break;
+        case DRIFT_T_BF16: rc = launch_cast<DRIFT_T_BF16>(a, st); break;
+        default: rc = launch_cast<DRIFT_T_FP16>(a, st); break;
+    }
+    if (rc) return rc;
+    if (rm == DRIFT_STOCHASTIC)
+        mx4_advance_kernel<<<1, 1, 0, st>>>(
+            d_state, (uint64_t)rows * cols * ((codes != nullptr) + (codes_t != nullptr)));
+    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+}
+
+// ------------------------------------------------------------------ back to values
+
+__device__ __forceinline__ double mx_value(unsigned code, int shared) {
+    const unsigned m = code & 7;
+    const double v = m < 2 ? 0.5 * m : (double)(2 + (m & 1)) * (double)(1 << (m >> 1)) * 0.25;
+    return (code & 8 ? -v : v) * pow2(shared);  // exact
+}
+
+// Eight values a thread. A double, float or bf16 holds every value exactly,
+// except that 2^127 times 2 or more overflows float and bf16; fp16 rounds.
+template <class T>
+__global__ void __launch_bounds__(256) mx4_values_kernel(const uint8_t *codes,
+                                                         const uint8_t *scales, int64_t rows,
+                                                         int64_t cols, T *dst, int64_t stride,
+                                                         uint32_t groups, bool vec) {
+    const int64_t row_bytes = mx4_row_bytes(cols), k_tiles = mx4_k_tiles(cols);
+    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        for (uint32_t g = blockIdx.x * 256 + threadIdx.x; g < groups; g += gridDim.x * 256) {
+            const int64_t col = (int64_t)g * 8;
+            const unsigned w =
+                *reinterpret_cast<const unsigned *>(codes + row * row_bytes + col / 2);
+            const int shared = (int)scales[mx4_scale_offset(row, col >> 5, k_tiles)] - 127;
+            __align__(16) T v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const double d = mx_value(w >> (4 * j) & 15, shared);
+                if constexpr (sizeof(T) == 8) v[j] = d;
+                else if constexpr (sizeof(T) == 4) v[j] = (float)d;
+                else v[j] = T((float)d);
+            }
+            T *p = dst + row * stride + col;
+            if (vec && col + 8 <= cols) {
+#pragma unroll
+                for (int j = 0; j < (int)sizeof(T) / 2; j++)
+                    reinterpret_cast<uint4 *>(p)[j] = reinterpret_cast<const uint4 *>(v)[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (col + j < cols) p[j] = v[j];
+            }
+        }
+    }
+}
+
+int launch_mx4_dequantize(const drift_mx4 *q, int type, void *dst, int64_t stride,
+                          cudaStream_t st) {
+    static const int size[4] = {8, 4, 2, 2};
+    const uint32_t groups = (uint32_t)((q->cols + 7) / 8);
+    const bool vec =
+        reinterpret_cast<uintptr_t>(dst) % 16 == 0 && stride * size[type] % 16 == 0;
+    const dim3 grid((groups + 255) / 256, (unsigned)std::min<int64_t>(q->rows, 65535));
+    switch (type) {
+        case DRIFT_T_F64:
+            mx4_values_kernel<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols,
+                                                    (double *)dst, stride, groups, vec);
+            break;
+        case DRIFT_T_F32:
+            mx4_values_kernel<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols,
+                                                    (float *)dst, stride, groups, vec);
+            break;
+        case DRIFT_T_BF16:
+            mx4_values_kernel<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols,
+                                                    (__nv_bfloat16 *)dst, stride, groups, vec);
+            break;
+        default:
+            mx4_values_kernel<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols,
+                                                    (__half *)dst, stride, groups, vec);
+    }
+    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+}
+
+}  // namespace drift

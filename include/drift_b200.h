@@ -513,6 +513,149 @@ DRIFT_API int drift_adam_dev(drift_ctx *ctx, double *d_param, const double *d_gr
                    double *d_m, double *d_v, int64_t n, int32_t step, double lr,
                    int32_t fp32_master, void *stream);
 
+/* ------------------------------------------- native training-step operators */
+/*
+ * The links of a training step (cast, contraction, loss, update) in the
+ * hardware's own arithmetic, next to the emulated ones above. No counterpart
+ * in the reference, except where a comment cites one. They allocate nothing
+ * and keep nothing in the context but its error word: every scratch buffer is
+ * the caller's, so calls on different streams, threads or captured graphs are
+ * independent as long as they have different buffers. They leave the calling
+ * thread's current device as it was. Pointers are device pointers of the
+ * context's device.
+ */
+/* Element types of matrices that cross as void*. */
+#define DRIFT_T_F64   0
+#define DRIFT_T_F32   1
+#define DRIFT_T_BF16  2
+#define DRIFT_T_FP16  3
+
+/*
+ * A matrix in microscaled 4-bit floating point: e2m1 elements and one E8M0
+ * scale per 32 consecutive elements of a row, blocks starting afresh in each
+ * row. `codes`: two elements a byte, the even one in the low nibble, a row
+ * taking ceil(cols / 32) * 16 bytes (padding codes are 0); 16-byte aligned.
+ * `scales`: exponent + 127, in tiles of 128 rows x 4 blocks of 512 bytes where
+ * row r, block b is byte (r % 32) * 16 + (r / 32) * 4 + b; a row of tiles has
+ * ceil(cols / 256) * 2 of them; padding bytes are 127; 16-byte aligned. The
+ * scale byte 255 is not used.
+ */
+typedef struct drift_mx4 {
+    int64_t rows, cols;
+    const uint8_t *codes;
+    const uint8_t *scales;
+} drift_mx4;
+/* Bytes of the two arrays of a rows x cols matrix. Pure host arithmetic. */
+DRIFT_API int drift_mx4_sizes(int64_t rows, int64_t cols, int64_t *code_bytes,
+                              int64_t *scale_bytes);
+/*
+ * The MX cast (Quant.quantize under MX_BLOCK, java/.../kernel/Quant.java:95-123)
+ * of a rows x cols matrix of `type`, rows `row_stride` elements apart, into
+ * the packed form: blocks along rows into (d_codes, d_scales), and blocks down
+ * columns, that is the transpose packed, into (d_codes_t, d_scales_t); either
+ * pair may be NULL, and both read the source once. The values equal the
+ * emulated cast's of each row (column) on its own. `p` must have e2m1 inputs
+ * (or gradients), MX_BLOCK scaling and blocks of 32; `rounding` is the cast's.
+ * Values beyond 6 before rounding are ADDED to *d_clamped (rows) and
+ * *d_clamped_t (columns), which may be NULL. NaN is held as 0 and reported by
+ * drift_check_dev as DRIFT_ENAN_FINITE.
+ * Stochastic rounding: element (i, j) uses draw i * cols + j of the stream, inexact or
+ * not (the emulated cast draws for inexact elements only); with both
+ * directions the column cast's draws follow the row cast's rows * cols. The state
+ * *d_rng_state is advanced past all of them.
+ */
+DRIFT_API int drift_mx4_quantize_dev(drift_ctx *ctx, const drift_policy *p, int rounding, int type,
+                           const void *d_src, int64_t rows, int64_t cols, int64_t row_stride,
+                           uint8_t *d_codes, uint8_t *d_scales, uint8_t *d_codes_t,
+                           uint8_t *d_scales_t, uint64_t *d_rng_state, int64_t *d_clamped,
+                           int64_t *d_clamped_t, void *stream);
+/* The values of a packed matrix, rows `row_stride` elements apart. Exact in
+ * double; float and bf16 hold all but products above their range (Inf). */
+DRIFT_API int drift_mx4_dequantize_dev(drift_ctx *ctx, const drift_mx4 *q, int type, void *d_dst,
+                             int64_t row_stride, void *stream);
+/*
+ * C[i * c_stride + o] = sum over k of a(i, k) b(o, k) (+ d_bias[o]): A->rows x
+ * B->rows outputs of `type`, A->cols == B->cols. Products are exact, sums
+ * fp32 in the tensor cores' order (contrast drift_gemm_dev, where the order is
+ * the policy's). d_ws holds the bytes that drift_mx4_gemm_workspace gives
+ * (NULL when 0), 256-byte aligned, untouched by others until the call's work is done.
+ */
+DRIFT_API int drift_mx4_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes);
+DRIFT_API int drift_mx4_gemm_dev(drift_ctx *ctx, const drift_mx4 *A, const drift_mx4 *B,
+                       const float *d_bias, int type, void *d_C, int64_t c_stride, void *d_ws,
+                       int64_t ws_bytes, void *stream);
+
+/*
+ * A linear layer's softmax cross entropy (Pass.java:134-153) over a vocabulary,
+ * its logits x W^T + bias computed in pieces and not kept. x: tokens x depth,
+ * W: vocab x depth, both of `type` (DRIFT_T_BF16 or DRIFT_T_FP16), rows x_stride
+ * and w_stride elements apart; bases and rows 16-byte aligned. bias: vocab
+ * floats or NULL. targets: int32 or int64 (target_bits); rows whose target is
+ * ignore_index have loss 0 and no gradient; any other target outside the
+ * vocabulary is treated so too and reported by drift_check_dev as
+ * DRIFT_EINVAL.
+ */
+typedef struct drift_xent {
+    int64_t tokens, depth, vocab;
+    int64_t x_stride, w_stride;
+    const void *x, *w;
+    const float *bias;
+    const void *targets;
+    int64_t ignore_index;
+    int32_t target_bits;   /* 32 or 64 */
+    int32_t type;
+} drift_xent;
+/* Workspace bytes of drift_linear_xent_dev (grad 0) and
+ * drift_linear_xent_grad_dev (grad 1), which may share one buffer. */
+DRIFT_API int drift_linear_xent_workspace(const drift_xent *op, int grad, int64_t *bytes);
+/* Per row: d_loss (may be NULL) and d_lse, the log of the sum of exponentials.
+ * d_mean (may be NULL): two floats, the mean loss of the rows that are not
+ * ignored (0 if all are) and 1 / their number (1 if all are). */
+DRIFT_API int drift_linear_xent_dev(drift_ctx *ctx, const drift_xent *op, float *d_loss,
+                          float *d_lse, float *d_mean, void *d_ws, int64_t ws_bytes,
+                          void *stream);
+/* Gradients, from d_lse of the forward call and the gradient of each row's
+ * loss, d_dloss[i * dloss_stride] (stride 0: one value for all rows): d_dx
+ * (tokens x depth) and d_dw (vocab x depth) of `type`, d_db (vocab floats); each
+ * may be NULL. Overwritten, not added to. The logits are computed again. */
+DRIFT_API int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, const float *d_lse,
+                               const float *d_dloss, int64_t dloss_stride, void *d_dx,
+                               int64_t dx_stride, void *d_dw, int64_t dw_stride, float *d_db,
+                               void *d_ws, int64_t ws_bytes, void *stream);
+
+/*
+ * One AdamW step over `count` tensors (decoupled weight decay; drift_adam_dev's
+ * update with weight_decay 0, in 32 bits). Per element, each operation rounded
+ * to fp32 on its own:
+ *   m' = b1 m + (1-b1) g;  v' = b2 v + ((1-b2) g) g;  r = sqrt(v')
+ *   p' = (1 - lr wd) p - (lr / (1 - b1^t) m') / (r / sqrt(1 - b2^t) + eps)
+ * state_bits 32: m and v are floats. state_bits 8: m and r are held as e4m3
+ * codes with one float scale per 256 consecutive elements, code =
+ * e4m3(x * (448 / amax)), value = code * (amax / 448), rounded to nearest or, with
+ * `rounding` stochastic, by one draw an element in tensor order.
+ */
+typedef struct drift_adamw {
+    double lr, beta1, beta2, eps, weight_decay;
+    int32_t state_bits;   /* 32 or 8 */
+    int32_t rounding;     /* DRIFT_NEAREST_EVEN, or DRIFT_STOCHASTIC with 8 bits */
+} drift_adamw;
+typedef struct drift_adamw_tensor {
+    void *param;          /* updated in place, param_type: F32, BF16 or FP16 */
+    const void *grad;     /* grad_type: F32, BF16 or FP16 */
+    void *m, *v;          /* floats, or e4m3 codes of m and of r */
+    float *m_scale, *v_scale;  /* 8 bits: ceil(n / 256) floats each */
+    void *copy;           /* NULL, or a second output for the new parameter */
+    int64_t n;
+    int32_t param_type, grad_type, copy_type, reserved;  /* reserved 0 */
+} drift_adamw_tensor;
+/* Takes step *d_step + 1 and stores it back, so that a captured call replays as
+ * the next step. d_scalars: 8 floats of scratch, 8-byte aligned. d_lr (may be
+ * NULL) replaces h->lr; d_grad_scale (may be NULL) multiplies every gradient. */
+DRIFT_API int drift_adamw_dev(drift_ctx *ctx, const drift_adamw *h,
+                    const drift_adamw_tensor *tensors, int64_t count, int64_t *d_step,
+                    float *d_scalars, const float *d_lr, const float *d_grad_scale,
+                    uint64_t *d_rng_state, void *stream);
+
 /* No counterpart in the reference: measures the FP64 pipe's DMUL+DADD issue
  * rate on the context's device (operations per second), the denominator of
  * the contraction's roofline. Takes a few milliseconds. */
