@@ -2,80 +2,37 @@
 //
 //   C[i, o] = sum_k a[i, k] b[o, k]  (+ bias[o])
 //
-// with a and b the values that codes and scales stand for and the sum in fp32.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+// with a and b the values that codes and scales stand for. The tensor cores
+// multiply the codes and apply the scales (tcgen05 kind::mxf4, one scale per 32
+// elements); sums are fp32 in TMEM and round once on the way out.
+#include <algorithm>
 
+#include "epilogue.cuh"
 #include "internal.h"
 #include "mx4.cuh"
+#include "tc.cuh"
 
 namespace drift {
 
-__device__ __forceinline__ float mx_code_value(unsigned c) {
-    const unsigned m = c & 7;
-    const float v = m < 2 ? 0.5f * m : (float)((2 + (m & 1)) << (m >> 1)) * 0.25f;
-    return c & 8 ? -v : v;
+static bool encode_codes(CUtensorMap *map, const drift_mx4 *q) {
+    const uint64_t bytes = (uint64_t)mx4_row_bytes(q->cols);
+    return tc::encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q->codes, bytes, q->rows, bytes, 128,
+                         128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-__device__ __forceinline__ float mx_scale_value(unsigned s) {
-    return s ? __uint_as_float(s << 23) : 0x1p-127f;
+// Rows of scale tiles, 256 words (two tiles) a stage; `box` rows at a time.
+static bool encode_scales(CUtensorMap *map, const drift_mx4 *q, uint32_t box) {
+    const uint64_t words = (uint64_t)mx4_k_tiles(q->cols) * 128;
+    return tc::encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, q->scales, words,
+                         mx4_row_tiles(q->rows), words * 4, 256, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-struct MxOperand {
-    const uint8_t *codes, *scales;
-    int64_t rows;
-};
-
-// 64 x 64 outputs a CTA, 4 x 4 a thread, one block of 32 at a time through
-// shared memory.
+// K = 0: the sum of nothing.
 template <class T>
-__global__ void __launch_bounds__(256) mx4_gemm_simple_kernel(MxOperand A, MxOperand B, int64_t K,
-                                                              const float *bias, T *C,
-                                                              int64_t c_stride) {
-    __shared__ float sa[32][65], sb[32][65];
-    const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int64_t blocks = mx4_blocks(K), k_tiles = mx4_k_tiles(K);
-    float acc[4][4] = {};
-    for (int64_t kb = 0; kb < blocks; kb++) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const MxOperand &X = h ? B : A;
-            float(*s)[65] = h ? sb : sa;
-            const int r = tid >> 2, q = tid & 3;  // four threads a row, eight codes each
-            const int64_t row = (h ? n0 : m0) + r;
-            unsigned w = 0;
-            float scale = 0.0f;
-            if (row < X.rows) {
-                w = *reinterpret_cast<const unsigned *>(X.codes + row * blocks * 16 + kb * 16 +
-                                                        q * 4);
-                scale = mx_scale_value(X.scales[mx4_scale_offset(row, kb, k_tiles)]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) s[q * 8 + j][r] = mx_code_value(w >> (4 * j) & 15) * scale;
-        }
-        __syncthreads();
-#pragma unroll 8
-        for (int k = 0; k < 32; k++) {
-            float a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) a[i] = sa[k][ty + 16 * i], b[i] = sb[k][tx + 16 * i];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t row = m0 + ty + 16 * i, col = n0 + tx + 16 * j;
-            if (row < A.rows && col < B.rows)
-                C[row * c_stride + col] = T(acc[i][j] + (bias ? bias[col] : 0.0f));
-        }
-    }
+__global__ void __launch_bounds__(256) fill_bias_kernel(T *C, int64_t stride, int64_t rows,
+                                                        int64_t cols, const float *bias) {
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < rows * cols; i += 256LL * gridDim.x)
+        C[i / cols * stride + i % cols] = T(bias ? bias[i % cols] : 0.0f);
 }
 
 int64_t mx4_gemm_workspace(int64_t M, int64_t N, int64_t K) {
@@ -83,27 +40,36 @@ int64_t mx4_gemm_workspace(int64_t M, int64_t N, int64_t K) {
     return 0;
 }
 
+template <class T>
+static int gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C, int64_t c_stride,
+                int *d_err, cudaStream_t st) {
+    if (a->cols == 0) {
+        fill_bias_kernel<<<sm_count() * 2, 256, 0, st>>>(C, c_stride, a->rows, b->rows, bias);
+        return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+    }
+    tc::Args args;
+    if (!encode_codes(&args.a, a) || !encode_codes(&args.b, b) ||
+        !encode_scales(&args.sfa, a, 1) || !encode_scales(&args.sfb, b, 2))
+        return DRIFT_ECUDA;
+    args.m_tiles = (int)((a->rows + tc::kTile - 1) / tc::kTile);
+    args.n_tiles = (int)((b->rows + tc::kTile - 1) / tc::kTile);
+    args.k_stages = (int)((a->cols + 255) / 256);
+    args.splits = 1;
+    args.err = d_err;
+    const StoreEpi<T> epi{C, c_stride, a->rows, b->rows, bias, nullptr,
+                          rows_aligned(C, c_stride)};
+    return tc::launch<tc::KIND_MX4, false, false, false>(args, epi, sm_count(), st);
+}
+
 int launch_mx4_gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, int type, void *C,
                     int64_t c_stride, void *ws, int *d_err, cudaStream_t st) {
-    (void)ws, (void)d_err;
-    const MxOperand A{a->codes, a->scales, a->rows}, B{b->codes, b->scales, b->rows};
-    const dim3 grid((unsigned)((a->rows + 63) / 64), (unsigned)((b->rows + 63) / 64));
+    (void)ws;
     switch (type) {
-        case DRIFT_T_F64:
-            mx4_gemm_simple_kernel<<<grid, 256, 0, st>>>(A, B, a->cols, bias, (double *)C, c_stride);
-            break;
-        case DRIFT_T_F32:
-            mx4_gemm_simple_kernel<<<grid, 256, 0, st>>>(A, B, a->cols, bias, (float *)C, c_stride);
-            break;
-        case DRIFT_T_BF16:
-            mx4_gemm_simple_kernel<<<grid, 256, 0, st>>>(A, B, a->cols, bias, (__nv_bfloat16 *)C,
-                                                         c_stride);
-            break;
-        default:
-            mx4_gemm_simple_kernel<<<grid, 256, 0, st>>>(A, B, a->cols, bias, (__half *)C,
-                                                         c_stride);
+        case DRIFT_T_F64: return gemm(a, b, bias, (double *)C, c_stride, d_err, st);
+        case DRIFT_T_F32: return gemm(a, b, bias, (float *)C, c_stride, d_err, st);
+        case DRIFT_T_BF16: return gemm(a, b, bias, (__nv_bfloat16 *)C, c_stride, d_err, st);
+        default: return gemm(a, b, bias, (__half *)C, c_stride, d_err, st);
     }
-    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
 }
 
 }  // namespace drift

@@ -1,71 +1,50 @@
 // xent.cu — a linear layer with softmax cross entropy over its outputs, in
-// pieces of the vocabulary, and its gradients; no more logits are held than one
-// piece's.
+// pieces of the vocabulary, and its gradients; no logits are kept.
 //
 //   l = x W^T + b       lse_i = log sum_v exp l_iv       loss_i = lse_i - l_i,t(i)
 //   d_iv = (exp(l_iv - lse_i) - [v = t(i)]) g_i
 //   dx = d W            dW = d^T x            db_v = sum_i d_iv
 //
-// x and W are bf16 (or fp16), sums and statistics fp32.
+// x and W are bf16 or fp16; sums, statistics and log sums are fp32. All four
+// products run on the tensor cores (tc.cuh):
+//
+//   forward   the logits' tile stays in registers: each thread reduces its 128
+//             columns of a row to a maximum, a sum of exponentials and perhaps the
+//             target's logit; a second kernel joins the parts of a row.
+//   gradient  a piece of the vocabulary at a time: the logits again, whose
+//             epilogue writes d in the inputs' type (one rounding, which halves
+//             its bytes and feeds the tensor cores; an element's error is half a
+//             unit of that type, as the results' own), then dx += d W and
+//             dW = d^T x from it, reading d and W where they lie (MN-major).
+//
+// fp16 holds d times a power of two that brings the largest |g| near 2^15, so
+// that small probabilities keep their bits; the products undo it exactly. bf16
+// has fp32's range and needs none.
+//
+// Bound: the tensor cores for many tokens (8 T D V operations with the
+// gradient's second computation of the logits, against 6 T D V if they were
+// kept); the bytes of W for few.
 #include <algorithm>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "common.cuh"
+#include "epilogue.cuh"
 #include "internal.h"
+#include "tc.cuh"
 
 namespace drift {
 
-template <class T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f(float x) { return x; }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+constexpr float kLog2e = 1.4426950408889634f;
 
-// C (+)= A B^T: A(i, k) at A[i*a_r + k*a_k], B(o, k) at B[o*b_r + k*b_k], 64 x 64
-// outputs a CTA.
-template <class TA, class TB, class TC>
-__global__ void __launch_bounds__(256) simple_gemm_kernel(int64_t M, int64_t N, int64_t K,
-                                                          const TA *A, int64_t a_r, int64_t a_k,
-                                                          const TB *B, int64_t b_r, int64_t b_k,
-                                                          TC *C, int64_t c_r, bool add) {
-    __shared__ float sa[32][65], sb[32][65];
-    const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += 32) {
-        for (int i = tid; i < 64 * 32; i += 256) {
-            const int ra = a_k == 1 ? i >> 5 : i & 63, ka = a_k == 1 ? i & 31 : i >> 6;
-            const int rb = b_k == 1 ? i >> 5 : i & 63, kb = b_k == 1 ? i & 31 : i >> 6;
-            sa[ka][ra] = m0 + ra < M && k0 + ka < K
-                             ? to_f(A[(m0 + ra) * a_r + (k0 + ka) * a_k]) : 0.0f;
-            sb[kb][rb] = n0 + rb < N && k0 + kb < K
-                             ? to_f(B[(n0 + rb) * b_r + (k0 + kb) * b_k]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll 8
-        for (int k = 0; k < 32; k++) {
-            float a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) a[i] = sa[k][ty + 16 * i], b[i] = sb[k][tx + 16 * i];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t row = m0 + ty + 16 * i, col = n0 + tx + 16 * j;
-            if (row < M && col < N) {
-                TC *c = C + row * c_r + col;
-                *c = TC(add ? to_f(*c) + acc[i][j] : acc[i][j]);
-            }
-        }
-    }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Maximum that keeps a NaN, so that a row with one has a NaN log sum.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 struct XentRows {
@@ -74,7 +53,7 @@ struct XentRows {
     int64_t ignore, vocab;
     // The target of row i; negative for an ignored row. One outside the
     // vocabulary sets `bad` and counts as ignored.
-    __device__ int64_t at(int64_t i, bool &bad) const {
+    __device__ __forceinline__ int64_t at(int64_t i, bool &bad) const {
         const int64_t t = wide ? static_cast<const int64_t *>(targets)[i]
                                : (int64_t) static_cast<const int32_t *>(targets)[i];
         if (t == ignore) return -1;
@@ -86,76 +65,182 @@ struct XentRows {
     }
 };
 
-// Maximum that keeps a NaN, so that a row with one has a NaN log sum.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// A maximum and a sum of exponentials relative to it.
+struct Stat {
+    float m, s;
+};
+__device__ __forceinline__ Stat join(Stat a, Stat b) {
+    Stat r;
+    r.m = max_nan(a.m, b.m);
+    r.s = r.m > -INFINITY ? a.s * exp2_fast((a.m - r.m) * kLog2e) +
+                                b.s * exp2_fast((b.m - r.m) * kLog2e)
+                          : 0.0f;
     return r;
 }
 
-// Joins a piece's logits to the running maximum, sum and target logit of a row.
-__global__ void __launch_bounds__(256) xent_stats_kernel(const float *logits, int64_t n,
-                                                         int64_t v0, const float *bias,
-                                                         XentRows rows, float *run, int *err) {
-    __shared__ float sm[8], ss[8];
-    const int64_t i = blockIdx.x;
-    const float *l = logits + i * n;
-    float m = -INFINITY, s = 0.0f;
-    for (int64_t v = threadIdx.x; v < n; v += 256) {
-        const float x = l[v] + (bias ? bias[v0 + v] : 0.0f);
-        const float top = max_nan(m, x);
-        if (top > -INFINITY) s = s * expf(m - top) + expf(x - top);
-        m = top;
+// ------------------------------------------------------------------ epilogues
+
+// Adds the bias; columns past the piece become -inf.
+__device__ __forceinline__ void finish_logits(float (&v)[128], int64_t col, int64_t cols,
+                                              const float *bias) {
+    if (bias) {
+#pragma unroll
+        for (int j = 0; j < 128; j++)
+            if (col + j < cols) v[j] += __ldg(bias + col + j);
     }
-    for (int o = 16; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(~0u, m, o), s2 = __shfl_xor_sync(~0u, s, o);
-        const float top = max_nan(m, m2);
-        if (top > -INFINITY) s = s * expf(m - top) + s2 * expf(m2 - top);
-        m = top;
-    }
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m, ss[threadIdx.x >> 5] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float *r = run + 3 * i;
-        if (v0) m = r[0], s = r[1];
-        else m = -INFINITY, s = 0.0f;
-        for (int w = 0; w < 8; w++) {
-            const float top = max_nan(m, sm[w]);
-            if (top > -INFINITY) s = s * expf(m - top) + ss[w] * expf(sm[w] - top);
-            m = top;
-        }
-        r[0] = m, r[1] = s;
-        bool bad = false;
-        const int64_t t = rows.at(i, bad);
-        if (bad) atomicOr(err, DEV_ERR_INDEX);
-        if (t >= v0 && t < v0 + n) r[2] = l[t - v0] + (bias ? bias[t] : 0.0f);
+    if (col + 128 > cols) {
+#pragma unroll
+        for (int j = 0; j < 128; j++)
+            if (col + j >= cols) v[j] = -INFINITY;
     }
 }
 
-// Losses and log sums of the rows from their running statistics; one CTA, so
-// that the mean over the counted rows is summed in a fixed order.
-__global__ void __launch_bounds__(1024) xent_finish_kernel(const float *run, int64_t T,
-                                                           XentRows rows, float *loss, float *lse,
-                                                           float *mean) {
+// Statistics of 128 logits of a row.
+struct StatsEpi {
+    Stat *parts;   // [column group of 128][row]
+    float *target; // target's logit per row
+    const float *bias;  // of the piece's first column
+    int64_t rows, cols, v0;
+    XentRows x;
+    __device__ __forceinline__ void run(float (&v)[128], int64_t row, int64_t col, const tc::Work &,
+                                        int) const {
+        if (col >= cols) return;
+        finish_logits(v, col, cols, bias);
+        float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int j = 4; j < 128; j++) m[j & 3] = max_nan(m[j & 3], v[j]);
+        const float top = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+        float s[4] = {};
+        // The difference first: a masked entry may be the type's lowest value, whose
+        // product with log2 e overflows.
+#pragma unroll
+        for (int j = 0; j < 128; j++) s[j & 3] += exp2_fast((v[j] - top) * kLog2e);
+        if (row >= rows) return;
+        const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+        parts[(col >> 7) * rows + row] = Stat{top, top > -INFINITY ? sum : 0.0f};
+        bool bad = false;
+        const int64_t t = x.at(row, bad) - v0 - col;
+        if (t >= 0 && t < 128) {
+            float l = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 128; j++)
+                if (j == (int)t) l = v[j];
+            target[row] = l;
+        }
+    }
+};
+
+// d of 128 logits of a row, in the inputs' type; and, with DB, its column sums
+// over the warp's 32 rows.
+template <class T, bool DB> struct GradEpi {
+    T *d;
+    int64_t ld;       // row stride of d, a multiple of 8
+    const float *bias;
+    int64_t rows, cols, v0;
+    XentRows x;
+    const float *lse, *g;
+    int64_t g_stride;
+    const float *scale;  // fp16: the power of two that d is held times, or null
+    float *sums;         // DB: [row / 32][column]
+    __device__ __forceinline__ void run(float (&v)[128], int64_t row, int64_t col, const tc::Work &,
+                                        int lane) const {
+        if (col >= cols) return;
+        finish_logits(v, col, cols, bias);
+        bool bad = false;
+        const int64_t t = row < rows ? x.at(row, bad) : -1;
+        const float gi = t >= 0 ? g[row * g_stride] : 0.0f;
+        const float z = t >= 0 ? lse[row] : 0.0f;
+        const int64_t at = t - v0 - col;
+#pragma unroll
+        for (int j = 0; j < 128; j++) {
+            const float p = exp2_fast((v[j] - z) * kLog2e);
+            v[j] = t >= 0 ? ((int64_t)j == at ? p - 1.0f : p) * gi : 0.0f;
+        }
+        if (DB) {
+            // 32 columns over 32 lanes at a time: at each step a lane keeps half of
+            // its columns and gets its partner's sums of them, so lane l ends with
+            // column l's sum.
+#pragma unroll
+            for (int c = 0; c < 128; c += 32) {
+                float a[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) a[j] = v[c + j];
+#pragma unroll
+                for (int h = 16; h; h >>= 1) {
+                    const bool up = lane & h;
+#pragma unroll
+                    for (int j = 0; j < h; j++) {
+                        const float keep = up ? a[j + h] : a[j], give = up ? a[j] : a[j + h];
+                        a[j] = keep + __shfl_xor_sync(0xffffffffu, give, h);
+                    }
+                }
+                if (col + c + lane < cols) sums[(row >> 5) * cols + col + c + lane] = a[0];
+            }
+        }
+        if (row >= rows) return;
+        if (scale) {
+            const float f = *scale;
+#pragma unroll
+            for (int j = 0; j < 128; j++) v[j] *= f;
+        }
+        T *p = d + row * ld + col;
+#pragma unroll
+        for (int j = 0; j < 128; j += 8)
+            if (col + j < ld) store8(p + j, v + j, 8, true);  // padding columns get zeros
+    }
+};
+
+// ------------------------------------------------------------------ small kernels
+
+// Joins a row's parts, and the running statistics of the pieces before, with 32
+// threads a row; the last piece gives its log sum and loss.
+__global__ void __launch_bounds__(256) xent_join_kernel(const Stat *parts, int n_parts, int64_t T,
+                                                        Stat *run, bool first, bool last,
+                                                        const float *target, XentRows x,
+                                                        float *loss, float *lse, int *err) {
+    __shared__ Stat sh[8][33];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+    Stat r{-INFINITY, 0.0f};
+    if (row < T) {
+#pragma unroll 4
+        for (int i = slice; i < n_parts; i += 8) r = join(r, parts[(int64_t)i * T + row]);
+    }
+    sh[slice][lane] = r;
+    __syncthreads();
+    if (slice || row >= T) return;
+    for (int i = 1; i < 8; i++) r = join(r, sh[i][lane]);
+    if (!first) r = join(run[row], r);
+    if (!last) {
+        run[row] = r;
+        return;
+    }
+    const float z = r.m + logf(r.s);
+    bool bad = false;
+    const int64_t t = x.at(row, bad);
+    if (bad) atomicOr(err, DEV_ERR_INDEX);
+    lse[row] = z;
+    if (loss) loss[row] = t >= 0 ? z - target[row] : 0.0f;
+}
+
+// The mean loss over the rows that count, summed in a fixed order by one CTA.
+__global__ void __launch_bounds__(1024) xent_mean_kernel(const float *lse, const float *target,
+                                                         int64_t T, XentRows x, float *mean) {
     __shared__ float sl[1024];
     __shared__ int sc[1024];
     float sum = 0.0f;
     int count = 0;
     for (int64_t i = threadIdx.x; i < T; i += 1024) {
-        const float z = run[3 * i] + logf(run[3 * i + 1]);
         bool bad = false;
-        const bool on = rows.at(i, bad) >= 0;
-        const float l = on ? z - run[3 * i + 2] : 0.0f;
-        lse[i] = z;
-        if (loss) loss[i] = l;
-        sum += l;
-        count += on;
+        if (x.at(i, bad) >= 0) sum += lse[i] - target[i], count++;
     }
-    if (!mean) return;
     sl[threadIdx.x] = sum, sc[threadIdx.x] = count;
     __syncthreads();
     for (int o = 512; o; o >>= 1) {
-        if (threadIdx.x < o) sl[threadIdx.x] += sl[threadIdx.x + o], sc[threadIdx.x] += sc[threadIdx.x + o];
+        if (threadIdx.x < o) {
+            sl[threadIdx.x] += sl[threadIdx.x + o];
+            sc[threadIdx.x] += sc[threadIdx.x + o];
+        }
         __syncthreads();
     }
     if (threadIdx.x == 0) {
@@ -165,122 +250,259 @@ __global__ void __launch_bounds__(1024) xent_finish_kernel(const float *run, int
     }
 }
 
-// A piece's logits to its part of d, in place.
-__global__ void __launch_bounds__(256) xent_dlogits_kernel(float *logits, int64_t n, int64_t v0,
-                                                           const float *bias, XentRows rows,
-                                                           const float *lse, const float *g,
-                                                           int64_t g_stride) {
-    const int64_t i = blockIdx.x;
-    bool bad = false;
-    const int64_t t = rows.at(i, bad);
-    const float z = lse[i], gi = t >= 0 ? g[i * g_stride] : 0.0f;
-    for (int64_t v = threadIdx.x; v < n; v += 256) {
-        const float p = expf(logits[i * n + v] + (bias ? bias[v0 + v] : 0.0f) - z);
-        logits[i * n + v] = t >= 0 ? (p - (v0 + v == t ? 1.0f : 0.0f)) * gi : 0.0f;
+// fp16: the power of two that brings the largest |g| into (2^14, 2^15], and its
+// inverse; 1 where no finite one would help.
+__global__ void __launch_bounds__(1024) xent_scale_kernel(const float *g, int64_t n, float *scale) {
+    __shared__ unsigned sm[32];
+    unsigned m = 0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024)
+        m = max(m, __float_as_uint(g[i]) & 0x7fffffffu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        m = __reduce_max_sync(0xffffffffu, sm[threadIdx.x]);
+        const int e = (int)(m >> 23);  // biased exponent
+        const bool use = e > 30 && e < 255;
+        const int k = use ? 14 - (e - 127) : 0;
+        if (threadIdx.x == 0) {
+            scale[0] = exp2f((float)k);
+            scale[1] = exp2f((float)-k);
+        }
     }
 }
 
-__global__ void __launch_bounds__(256) xent_colsum_kernel(const float *d, int64_t T, int64_t n,
-                                                          float *db) {
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v >= n) return;
+// db of a piece from the sums of groups of 32 rows, in order.
+__global__ void __launch_bounds__(256) xent_colsum_kernel(const float *sums, int64_t groups,
+                                                          int64_t n, float *db) {
+    __shared__ float sh[8][33];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t v = (int64_t)blockIdx.x * 32 + lane;
     float s = 0.0f;
-    for (int64_t i = 0; i < T; i++) s += d[i * n + v];
+    if (v < n) {
+#pragma unroll 4
+        for (int64_t i = slice; i < groups; i += 8) s += sums[i * n + v];
+    }
+    sh[slice][lane] = s;
+    __syncthreads();
+    if (slice || v >= n) return;
+    for (int i = 1; i < 8; i++) s += sh[i][lane];
     db[v] = s;
 }
 
+// Sums the parts of dx and rounds to its type.
 template <class T>
-__global__ void __launch_bounds__(256) narrow_kernel(const float *x, T *y, int64_t rows,
-                                                     int64_t cols, int64_t stride) {
-    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < rows * cols; i += 256LL * gridDim.x)
-        y[i / cols * stride + i % cols] = T(x[i]);
+__global__ void __launch_bounds__(256) xent_dx_kernel(const float *acc, int splits, int64_t part,
+                                                      int64_t ld, T *dx, int64_t rows,
+                                                      int64_t cols, int64_t stride,
+                                                      const float *alpha) {
+    const float f = alpha ? *alpha : 1.0f;
+    const int64_t groups = (cols + 3) / 4;
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < rows * groups; i += 256LL * gridDim.x) {
+        const int64_t r = i / groups, c = (i - r * groups) * 4;
+        float4 s = *reinterpret_cast<const float4 *>(acc + r * ld + c);
+        for (int k = 1; k < splits; k++) {
+            const float4 y = *reinterpret_cast<const float4 *>(acc + k * part + r * ld + c);
+            s.x += y.x, s.y += y.y, s.z += y.z, s.w += y.w;
+        }
+        const float v[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
+        T *p = dx + r * stride + c;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (c + j < cols) p[j] = T(v[j]);
+    }
 }
 
-static int64_t xent_piece(const drift_xent *op) {
-    const int64_t fit = (256LL << 20) / 4 / std::max<int64_t>(op->tokens, 1);
-    return std::max<int64_t>(64, std::min(op->vocab, fit / 64 * 64));
+// ------------------------------------------------------------------ plans
+
+static int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+static int tiles(int64_t x) { return (int)((x + tc::kTile - 1) / tc::kTile); }
+static int stages(int64_t k) { return (int)((k + 63) / 64); }
+
+// The forward pass holds 16 bytes a row and 256 columns; pieces keep that near
+// 64 MB.
+struct ForwardPlan {
+    int64_t piece, parts, target, run, bytes;  // offsets in the workspace
+};
+static ForwardPlan forward_plan(const drift_xent *op) {
+    ForwardPlan p;
+    const int64_t t = std::max<int64_t>(op->tokens, 1);
+    p.piece = std::min(up(op->vocab, 256), std::max<int64_t>(1, (64LL << 20) / (t * 16)) * 256);
+    p.parts = 0;
+    p.target = up(t * (p.piece / 128) * 8, 256);
+    p.run = p.target + up(t * 4, 256);
+    p.bytes = p.run + up(t * 8, 256);
+    return p;
+}
+
+// A piece of d is near 256 MB: large enough that the pass over the fp32 sums of
+// dx that each piece costs (8 bytes an element of dx) is small beside the
+// piece's products, small enough to be no burden beside W.
+struct GradPlan {
+    int64_t piece, ld, d, sums, acc, part, acc_ld, scale, bytes;
+    int pieces, splits;
+    bool direct;  // dx in one product, rounded by its epilogue
+};
+static GradPlan grad_plan(const drift_xent *op) {
+    GradPlan p;
+    const int64_t t = std::max<int64_t>(op->tokens, 1);
+    p.piece = std::min(up(op->vocab, 256), std::max<int64_t>(256, (128LL << 20) / t / 256 * 256));
+    p.pieces = (int)((op->vocab + p.piece - 1) / p.piece);
+    p.ld = std::min(p.piece, up(op->vocab, 8));
+    // dx contracts the vocabulary: with few tokens its tiles are fewer than the
+    // pairs of SMs, and the contraction is cut so that they all have work, down
+    // to 16 stages (1024 entries) a part.
+    const int dx_tiles = tiles(t) * tiles(op->depth);
+    const int most = std::max(1, stages(p.ld) / 16);
+    p.splits = std::max(1, std::min(most, 74 / dx_tiles));
+    p.direct = p.pieces == 1 && p.splits == 1;
+    p.acc_ld = up(op->depth, 4);
+    p.part = t * p.acc_ld;
+    p.d = 0;
+    p.sums = up(t * p.ld * 2, 256);
+    p.acc = p.sums + (op->bias ? up(up(t, 256) / 32 * p.ld * 4, 256) : 0);
+    p.scale = p.acc + (p.direct ? 0 : up(p.splits * p.part * 4, 256));
+    p.bytes = p.scale + 256;
+    return p;
 }
 
 int64_t xent_workspace(const drift_xent *op, bool grad) {
-    const int64_t run = (op->tokens * 3 * 4 + 255) / 256 * 256;
-    return run + op->tokens * xent_piece(op) * 4 + (grad ? op->tokens * op->depth * 4 : 0) + 256;
-}
-
-static dim3 tiles(int64_t m, int64_t n) {
-    return dim3((unsigned)((m + 63) / 64), (unsigned)((n + 63) / 64));
+    const int64_t f = forward_plan(op).bytes;
+    return grad ? std::max(f, grad_plan(op).bytes) : f;
 }
 
 static XentRows rows_of(const drift_xent *op) {
     return XentRows{op->targets, op->target_bits == 64, op->ignore_index, op->vocab};
 }
 
-template <class T>
-static int xent_forward(const drift_xent *op, float *loss, float *lse, float *mean, char *ws,
-                        int *err, cudaStream_t st) {
-    const int64_t n_t = op->tokens, piece = xent_piece(op);
-    float *run = (float *)ws, *logits = (float *)(ws + (n_t * 12 + 255) / 256 * 256);
-    for (int64_t v0 = 0; n_t && v0 < op->vocab; v0 += piece) {
-        const int64_t n = std::min(piece, op->vocab - v0);
-        simple_gemm_kernel<<<tiles(n_t, n), 256, 0, st>>>(
-            n_t, n, op->depth, (const T *)op->x, op->x_stride, 1,
-            (const T *)op->w + v0 * op->w_stride, op->w_stride, 1, logits, n, false);
-        xent_stats_kernel<<<(unsigned)n_t, 256, 0, st>>>(logits, n, v0, op->bias, rows_of(op), run,
-                                                         err);
-    }
-    xent_finish_kernel<<<1, 1024, 0, st>>>(run, n_t, rows_of(op), loss, lse, mean);
-    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+static int done() { return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA; }
+
+// The maps and shape of a piece's logits: x (T x D) against rows v0 .. of W.
+static bool logit_args(tc::Args &a, const drift_xent *op, int64_t v0, int64_t n, bool bf16,
+                       int *err) {
+    const char *w = static_cast<const char *>(op->w) + v0 * op->w_stride * 2;
+    a.m_tiles = tiles(op->tokens);
+    a.n_tiles = tiles(n);
+    a.k_stages = stages(op->depth);
+    a.splits = 1;
+    a.err = err;
+    return tc::encode_16(&a.a, bf16, op->x, op->tokens, op->depth, op->x_stride, true) &&
+           tc::encode_16(&a.b, bf16, w, n, op->depth, op->w_stride, true);
 }
 
-template <class T>
-static int xent_backward(const drift_xent *op, const float *lse, const float *g, int64_t g_stride,
-                         void *dx, int64_t dx_stride, void *dw, int64_t dw_stride, float *db,
-                         char *ws, int *err, cudaStream_t st) {
-    (void)err;
-    const int64_t n_t = op->tokens, d = op->depth, piece = xent_piece(op);
+template <bool BF16>
+static int forward(const drift_xent *op, float *loss, float *lse, float *mean, char *ws, int *err,
+                   cudaStream_t st) {
+    const ForwardPlan p = forward_plan(op);
+    const int64_t n_t = op->tokens;
+    const XentRows rows = rows_of(op);
+    Stat *parts = reinterpret_cast<Stat *>(ws + p.parts);
+    Stat *run = reinterpret_cast<Stat *>(ws + p.run);
+    float *target = reinterpret_cast<float *>(ws + p.target);
+    for (int64_t v0 = 0; n_t && v0 < op->vocab; v0 += p.piece) {
+        const int64_t n = std::min(p.piece, op->vocab - v0);
+        tc::Args a;
+        if (!logit_args(a, op, v0, n, BF16, err)) return DRIFT_ECUDA;
+        const StatsEpi epi{parts, target, op->bias ? op->bias + v0 : nullptr, n_t, n, v0, rows};
+        const int rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
+        if (rc) return rc;
+        xent_join_kernel<<<(unsigned)((n_t + 31) / 32), 256, 0, st>>>(
+            parts, (int)((n + 127) / 128), n_t, run, v0 == 0, v0 + n == op->vocab, target, rows,
+            loss, lse, err);
+    }
+    if (mean) xent_mean_kernel<<<1, 1024, 0, st>>>(lse, target, n_t, rows, mean);
+    return done();
+}
+
+template <class T, bool BF16>
+static int backward(const drift_xent *op, const float *lse, const float *g, int64_t g_stride, T *dx,
+                    int64_t dx_stride, T *dw, int64_t dw_stride, float *db, char *ws, int *err,
+                    cudaStream_t st) {
+    const GradPlan p = grad_plan(op);
+    const int64_t n_t = op->tokens, dep = op->depth;
     if (n_t == 0) {
-        if (dw) cudaMemset2DAsync(dw, dw_stride * 2, 0, d * 2, op->vocab, st);
+        if (dw) cudaMemset2DAsync(dw, dw_stride * 2, 0, dep * 2, op->vocab, st);
         if (db) cudaMemsetAsync(db, 0, op->vocab * 4, st);
-        return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+        return done();
     }
-    float *acc = (float *)ws, *logits = (float *)(ws + (n_t * d * 4 + 255) / 256 * 256);
-    for (int64_t v0 = 0; v0 < op->vocab; v0 += piece) {
-        const int64_t n = std::min(piece, op->vocab - v0);
-        const T *w = (const T *)op->w + v0 * op->w_stride;
-        simple_gemm_kernel<<<tiles(n_t, n), 256, 0, st>>>(n_t, n, d, (const T *)op->x,
-                                                          op->x_stride, 1, w, op->w_stride, 1,
-                                                          logits, n, false);
-        xent_dlogits_kernel<<<(unsigned)n_t, 256, 0, st>>>(logits, n, v0, op->bias, rows_of(op),
-                                                           lse, g, g_stride);
-        if (dx)
-            simple_gemm_kernel<<<tiles(n_t, d), 256, 0, st>>>(n_t, d, n, logits, n, 1, w, 1,
-                                                              op->w_stride, acc, d, v0 > 0);
-        if (dw)
-            simple_gemm_kernel<<<tiles(n, d), 256, 0, st>>>(
-                n, d, n_t, logits, 1, n, (const T *)op->x, 1, op->x_stride,
-                (T *)dw + v0 * dw_stride, dw_stride, false);
-        if (db)
-            xent_colsum_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(logits, n_t, n,
-                                                                            db + v0);
+    const XentRows rows = rows_of(op);
+    T *d = reinterpret_cast<T *>(ws + p.d);
+    float *sums = reinterpret_cast<float *>(ws + p.sums);
+    float *acc = reinterpret_cast<float *>(ws + p.acc);
+    float *scale = BF16 ? nullptr : reinterpret_cast<float *>(ws + p.scale);
+    if (scale) xent_scale_kernel<<<1, 1024, 0, st>>>(g, g_stride ? n_t : 1, scale);
+    const float *undo = scale ? scale + 1 : nullptr;
+    for (int64_t v0 = 0; v0 < op->vocab; v0 += p.piece) {
+        const int64_t n = std::min(p.piece, op->vocab - v0);
+        tc::Args a;
+        if (!logit_args(a, op, v0, n, BF16, err)) return DRIFT_ECUDA;
+        const float *bias = op->bias ? op->bias + v0 : nullptr;
+        int rc;
+        if (db) {
+            const GradEpi<T, true> epi{d,   p.ld, bias, n_t,      n,     v0,  rows,
+                                       lse, g,    g_stride, scale, sums};
+            rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
+            if (!rc)
+                xent_colsum_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>(
+                    sums, (n_t + 31) / 32, n, db + v0);
+        } else {
+            const GradEpi<T, false> epi{d,   p.ld, bias, n_t,      n,     v0,  rows,
+                                        lse, g,    g_stride, scale, nullptr};
+            rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
+        }
+        if (rc) return rc;
+        const char *w = static_cast<const char *>(op->w) + v0 * op->w_stride * 2;
+        if (dx) {
+            // dx (T x D) contracts the piece: d K-major, W's rows are k.
+            if (!tc::encode_16(&a.a, BF16, d, n_t, n, p.ld, true) ||
+                !tc::encode_16(&a.b, BF16, w, dep, n, op->w_stride, false))
+                return DRIFT_ECUDA;
+            a.m_tiles = tiles(n_t), a.n_tiles = tiles(dep), a.k_stages = stages(n);
+            a.splits = std::min(p.splits, a.k_stages);
+            if (p.direct) {
+                const StoreEpi<T> epi{dx, dx_stride, n_t, dep, nullptr, undo,
+                                      rows_aligned(dx, dx_stride)};
+                rc = tc::launch<tc::KIND_16, BF16, false, true>(a, epi, sm_count(), st);
+            } else {
+                const PartEpi epi{acc, p.part, p.acc_ld, n_t, dep, v0 > 0};
+                rc = tc::launch<tc::KIND_16, BF16, false, true>(a, epi, sm_count(), st);
+            }
+            if (rc) return rc;
+        }
+        if (dw) {
+            // dW (piece x D) contracts the tokens: rows of d and of x are k.
+            if (!tc::encode_16(&a.a, BF16, d, n, n_t, p.ld, false) ||
+                !tc::encode_16(&a.b, BF16, op->x, dep, n_t, op->x_stride, false))
+                return DRIFT_ECUDA;
+            a.m_tiles = tiles(n), a.n_tiles = tiles(dep), a.k_stages = stages(n_t);
+            a.splits = 1;
+            T *to = dw + v0 * dw_stride;
+            const StoreEpi<T> epi{to, dw_stride, n, dep, nullptr, undo, rows_aligned(to, dw_stride)};
+            rc = tc::launch<tc::KIND_16, BF16, true, true>(a, epi, sm_count(), st);
+            if (rc) return rc;
+        }
     }
-    if (dx) narrow_kernel<<<sm_count() * 4, 256, 0, st>>>(acc, (T *)dx, n_t, d, dx_stride);
-    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+    if (dx && !p.direct)
+        xent_dx_kernel<<<sm_count() * 8, 256, 0, st>>>(acc, p.splits, p.part, p.acc_ld, dx, n_t, dep,
+                                                       dx_stride, undo);
+    return done();
 }
 
 int launch_xent(const drift_xent *op, float *loss, float *lse, float *mean, void *ws, int *err,
                 cudaStream_t st) {
-    return op->type == DRIFT_T_BF16
-               ? xent_forward<__nv_bfloat16>(op, loss, lse, mean, (char *)ws, err, st)
-               : xent_forward<__half>(op, loss, lse, mean, (char *)ws, err, st);
+    return op->type == DRIFT_T_BF16 ? forward<true>(op, loss, lse, mean, (char *)ws, err, st)
+                                    : forward<false>(op, loss, lse, mean, (char *)ws, err, st);
 }
 
 int launch_xent_grad(const drift_xent *op, const float *lse, const float *g, int64_t g_stride,
                      void *dx, int64_t dx_stride, void *dw, int64_t dw_stride, float *db, void *ws,
                      int *err, cudaStream_t st) {
-    return op->type == DRIFT_T_BF16
-               ? xent_backward<__nv_bfloat16>(op, lse, g, g_stride, dx, dx_stride, dw, dw_stride,
-                                              db, (char *)ws, err, st)
-               : xent_backward<__half>(op, lse, g, g_stride, dx, dx_stride, dw, dw_stride, db,
-                                       (char *)ws, err, st);
+    if (op->type == DRIFT_T_BF16)
+        return backward<__nv_bfloat16, true>(op, lse, g, g_stride, (__nv_bfloat16 *)dx, dx_stride,
+                                             (__nv_bfloat16 *)dw, dw_stride, db, (char *)ws, err,
+                                             st);
+    return backward<__half, false>(op, lse, g, g_stride, (__half *)dx, dx_stride, (__half *)dw,
+                                   dw_stride, db, (char *)ws, err, st);
 }
 
 }  // namespace drift

@@ -85,7 +85,7 @@ def check_grads(x, w, tg, b, g, got):
     soft = p * torch.expm1(e.clamp(max=10.0)) * on + 2.0 ** -22 * dl.abs()
     # f16 holds d scaled by a power of two near 2^15 / max |g|, so that its
     # smallest step, 2^-24, stands for 2^-38 of the largest gradient.
-    floor = 2.0 ** -38 * on if x.dtype == torch.float16 else 0.0
+    floor = 2.0 ** -38 * float(g.abs().max()) * (on > 0) if x.dtype == torch.float16 else 0.0
     el = soft + half * (dl.abs() + soft) + floor
     X, W = x.double().abs(), w.double().abs()
     tiny = 2.0 ** -25 if x.dtype == torch.float16 else 0.0  # half a step of f16's subnormals
