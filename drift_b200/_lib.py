@@ -142,9 +142,7 @@ SIGNATURES = {
     "drift_mx4_quantize_dev": (_int, [_vp, _P(DriftPolicy), _int, _int, _vp, _i64, _i64, _i64, _vp,
                                       _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "drift_mx4_dequantize_dev": (_int, [_vp, _P(DriftMx4), _int, _vp, _i64, _vp]),
-    "drift_mx4_gemm_workspace": (_int, [_i64, _i64, _i64, _P(_i64)]),
-    "drift_mx4_gemm_dev": (_int, [_vp, _P(DriftMx4), _P(DriftMx4), _vp, _int, _vp, _i64, _vp, _i64,
-                                  _vp]),
+    "drift_mx4_gemm_dev": (_int, [_vp, _P(DriftMx4), _P(DriftMx4), _vp, _int, _vp, _i64, _vp]),
     "drift_linear_xent_workspace": (_int, [_P(DriftXent), _int, _P(_i64)]),
     "drift_linear_xent_dev": (_int, [_vp, _P(DriftXent), _vp, _vp, _vp, _vp, _i64, _vp]),
     "drift_linear_xent_grad_dev": (_int, [_vp, _P(DriftXent), _vp, _vp, _i64, _vp, _i64, _vp, _i64,

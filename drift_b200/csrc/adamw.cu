@@ -1,12 +1,15 @@
 // adamw.cu — one AdamW step over a list of tensors in one launch, moments in
 // 32 bits or in 8 bits with one scale per 256 elements.
 //
-// Every element does, in 32 bits, each operation rounded on its own
-// (-fmad=false; the order is part of the definition, so a plain evaluation in
-// the same order gives the same bits):
+// Every element does, in 32 bits, with fma(a, b, c) one rounding and every other
+// operation its own (this is the definition, so the same operations elsewhere
+// give the moments' bits):
 //
-//   m' = b1 m + (1-b1) g          v' = b2 v + ((1-b2) g) g        r = sqrt(v')
-//   p' = (1 - lr wd) p - (lr/(1-b1^t) m') / (r / sqrt(1-b2^t) + eps)
+//   m' = fma(b1, m, (1-b1) g)     v' = fma(b2, v, ((1-b2) g) g)   r = sqrt(v')
+//   p' = fma(1 - lr wd, p, -(lr/(1-b1^t) m') / fma(r, 1/sqrt(1-b2^t), eps))
+//
+// The quotient is a product with a reciprocal, within two units in the last
+// place: an IEEE division would be a sixth of the instructions.
 //
 // In 8 bits the first moment is held as e4m3 codes of m * (448 / amax) and
 // the second as e4m3 codes of its root r, which spans half the binades that v
@@ -28,9 +31,8 @@ namespace drift {
 
 constexpr int kAdamThreads = 256;
 constexpr int kAdamBlock = 256;                     // elements that share a scale
-constexpr int kAdamBlocksPerWarp = 2;
-constexpr int kAdamChunk = kAdamBlock * (kAdamThreads / 32) * kAdamBlocksPerWarp;
-constexpr int kAdamTensors = 128;                   // tensors of one launch
+constexpr int kAdamMostBlocks = 4;                  // blocks that a warp takes in turn
+constexpr int kAdamTensors = 256;                   // tensors of one launch
 
 struct AdamTensor {
     void *p;
@@ -48,6 +50,7 @@ struct AdamArgs {
     AdamTensor t[kAdamTensors];
     uint32_t first[kAdamTensors + 1];  // first chunk of each tensor
     int count;
+    int per_warp;  // blocks a warp takes
     float b1, b2, c1, c2, eps;
     const float *scal;        // lr/(1-b1^t), 1/sqrt(1-b2^t), 1 - lr wd
     const uint64_t *rng;      // Rng state of this step's draws
@@ -71,54 +74,114 @@ __global__ void adamw_prepare_kernel(int64_t *step, double b1, double b2, double
     }
 }
 
-__device__ __forceinline__ float half_bits_to_float(uint16_t h, int type) {
-    return type == DRIFT_T_BF16 ? __uint_as_float((unsigned)h << 16)
-                                : __half2float(__ushort_as_half(h));
+// ------------------------------------------------------------------ pairs of floats
+//
+// Two elements an instruction (mul.rn.f32x2, fma.rn.f32x2): each half is rounded
+// as the scalar operation would. There is no f2_add: the assembler contracts a
+// product and an add.rn.f32x2 into one fused operation, against -fmad=false, so
+// the sums are written as the fused operations that they become.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 f2_pack(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
+__device__ __forceinline__ f2 f2_both(float a) { return f2_pack(a, a); }
+__device__ __forceinline__ void f2_split(f2 x, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {  // within one unit
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// The larger magnitude; NaN wins.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+
+// ------------------------------------------------------------------ eight elements
+
+// Eight elements as they lie in memory: 16-bit types use the first word.
+struct Raw8 {
+    uint4 w[2];
+};
 
 __device__ __forceinline__ uint16_t float_to_half_bits(float f, int type) {
     return type == DRIFT_T_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f))
                                 : __half_as_ushort(__float2half_rn(f));
 }
 
-// Eight consecutive elements at `i`; `vec` reads them 16 bytes at a time.
-__device__ __forceinline__ void load8(const void *p, int type, int64_t i, int valid, bool vec,
-                                      float (&x)[8]) {
+// `whole`: all eight exist and are aligned for 16-byte accesses.
+__device__ __forceinline__ Raw8 load_raw(const void *p, int type, int64_t i, int valid,
+                                         bool whole) {
+    Raw8 r;
     if (type == DRIFT_T_F32) {
         const float *f = static_cast<const float *>(p) + i;
-        if (vec && valid == 8) {
-            const float4 a = *reinterpret_cast<const float4 *>(f);
-            const float4 b = *reinterpret_cast<const float4 *>(f + 4);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-            x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        if (whole) {
+            r.w[0] = __ldcs(reinterpret_cast<const uint4 *>(f));
+            r.w[1] = __ldcs(reinterpret_cast<const uint4 *>(f) + 1);
         } else {
+            unsigned *u = reinterpret_cast<unsigned *>(r.w);
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = j < valid ? f[j] : 0.0f;
+            for (int j = 0; j < 8; j++) u[j] = j < valid ? __float_as_uint(f[j]) : 0u;
         }
     } else {
         const uint16_t *h = static_cast<const uint16_t *>(p) + i;
-        if (vec && valid == 8) {
-            const uint4 a = *reinterpret_cast<const uint4 *>(h);
-            const unsigned w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                x[2 * j] = half_bits_to_float((uint16_t)w[j], type);
-                x[2 * j + 1] = half_bits_to_float((uint16_t)(w[j] >> 16), type);
-            }
+        if (whole) {
+            r.w[0] = __ldcs(reinterpret_cast<const uint4 *>(h));
         } else {
+            unsigned *u = reinterpret_cast<unsigned *>(r.w);
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = j < valid ? half_bits_to_float(h[j], type) : 0.0f;
+            for (int j = 0; j < 4; j++)
+                u[j] = (2 * j < valid ? h[2 * j] : 0u) |
+                       (2 * j + 1 < valid ? (unsigned)h[2 * j + 1] << 16 : 0u);
+        }
+    }
+    return r;
+}
+
+__device__ __forceinline__ void unpack(const Raw8 &r, int type, f2 (&x)[4]) {
+    const unsigned *u = reinterpret_cast<const unsigned *>(r.w);
+    if (type == DRIFT_T_F32) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            x[j] = f2_pack(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+    } else if (type == DRIFT_T_BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            x[j] = f2_pack(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
+            x[j] = f2_pack(f.x, f.y);
         }
     }
 }
 
-__device__ __forceinline__ void store8(void *p, int type, int64_t i, int valid, bool vec,
-                                       const float (&x)[8]) {
+__device__ __forceinline__ void store8(void *p, int type, int64_t i, int valid, bool whole,
+                                       const f2 (&y)[4]) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) f2_split(y[j], x[2 * j], x[2 * j + 1]);
     if (type == DRIFT_T_F32) {
         float *f = static_cast<float *>(p) + i;
-        if (vec && valid == 8) {
-            *reinterpret_cast<float4 *>(f) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4 *>(f + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        if (whole) {
+            __stcs(reinterpret_cast<float4 *>(f), make_float4(x[0], x[1], x[2], x[3]));
+            __stcs(reinterpret_cast<float4 *>(f) + 1, make_float4(x[4], x[5], x[6], x[7]));
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -126,13 +189,20 @@ __device__ __forceinline__ void store8(void *p, int type, int64_t i, int valid, 
         }
     } else {
         uint16_t *h = static_cast<uint16_t *>(p) + i;
-        if (vec && valid == 8) {
-            unsigned w[4];
+        if (whole) {
+            uint4 w;
+            unsigned *u = reinterpret_cast<unsigned *>(&w);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                w[j] = float_to_half_bits(x[2 * j], type) |
-                       (unsigned)float_to_half_bits(x[2 * j + 1], type) << 16;
-            *reinterpret_cast<uint4 *>(h) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < 4; j++) {
+                if (type == DRIFT_T_BF16) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+                    u[j] = *reinterpret_cast<const unsigned *>(&b);
+                } else {
+                    const __half2 b = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+                    u[j] = *reinterpret_cast<const unsigned *>(&b);
+                }
+            }
+            __stcs(reinterpret_cast<uint4 *>(h), w);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -141,38 +211,44 @@ __device__ __forceinline__ void store8(void *p, int type, int64_t i, int valid, 
     }
 }
 
-// Eight e4m3 codes and their values times `scale`.
-__device__ __forceinline__ void load_codes(const void *p, int64_t i, int valid, bool vec,
-                                           float scale, float (&x)[8]) {
+__device__ __forceinline__ uint64_t load_codes(const void *p, int64_t i, int valid, bool whole) {
     const uint8_t *c = static_cast<const uint8_t *>(p) + i;
+    if (whole) return __ldcs(reinterpret_cast<const unsigned long long *>(c));
     uint64_t w = 0;
-    if (vec && valid == 8) {
-        w = *reinterpret_cast<const uint64_t *>(c);
-    } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < valid) w |= (uint64_t)c[j] << (8 * j);
-    }
+    for (int j = 0; j < 8; j++)
+        if (j < valid) w |= (uint64_t)c[j] << (8 * j);
+    return w;
+}
+
+// Eight e4m3 codes' values times `scale`.
+__device__ __forceinline__ void decode(uint64_t w, float scale, f2 (&x)[4]) {
+    const f2 s = f2_both(scale);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(
-            (__nv_fp8x2_storage_t)(w >> (16 * j)), __NV_E4M3));
-        x[2 * j] = __low2float(h) * scale;
-        x[2 * j + 1] = __high2float(h) * scale;
+        const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(
+            (__nv_fp8x2_storage_t)(w >> (16 * j)), __NV_E4M3)));
+        x[j] = f2_mul(f2_pack(f.x, f.y), s);
     }
 }
 
-__device__ __forceinline__ float warp_max_bits(const float (&x)[8]) {
-    unsigned a = 0;
+__device__ __forceinline__ float warp_amax(const f2 (&x)[4]) {
+    float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) a = max(a, __float_as_uint(x[j]) & 0x7fffffffu);
-    return __uint_as_float(__reduce_max_sync(0xffffffffu, a));  // NaN above Inf above all else
+    for (int j = 0; j < 4; j++) {
+        float a, b;
+        f2_split(x[j], a, b);
+        m = max_abs(m, max_abs(a, b));
+    }
+    // As bit patterns magnitudes order like integers, NaN above Inf above all else.
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu));
 }
 
 // Stochastic rounding to e4m3: the code below |y| or the one above, the upper
 // with the dropped fraction as its probability (20 random bits). Below 2^-6
 // the quantum is 2^-9 throughout, which adding 2^-6 gives.
 __device__ __forceinline__ float round_e4m3_sr(float y, unsigned u20) {
+    if (y != y) return y;
     float a = fminf(fabsf(y), 448.0f);
     const bool sub = a < 0x1p-6f;
     if (sub) a += 0x1p-6f;
@@ -181,41 +257,130 @@ __device__ __forceinline__ float round_e4m3_sr(float y, unsigned u20) {
     return copysignf(a, y);
 }
 
-// Writes a warp's block of 256 values as codes and its scale. A block whose
-// values are all below 2^-100 is held as zeros (448 / amax would overflow);
-// one with an Inf or NaN reads back as NaN, so that it is not mistaken for
-// a state.
+// Codes of a lane's eight values times `inv`.
 template <bool SR>
-__device__ __forceinline__ void store_codes(void *p, float *scale, int64_t i, int64_t block,
-                                            int valid, bool vec, int lane, const float (&x)[8],
-                                            const unsigned (&u)[8]) {
-    const float amax = warp_max_bits(x);
-    float inv = 0.0f, s = 1.0f;
-    if (!(amax <= 3.402823466e38f)) {
-        inv = s = __uint_as_float(0x7fffffffu);
-    } else if (amax >= 0x1p-100f) {
-        inv = 448.0f / amax;
-        s = amax / 448.0f;
-    }
-    if (lane == 0) scale[block] = s;
-    uint64_t w = 0;
+__device__ __forceinline__ void store_codes(void *p, int64_t i, int valid, bool whole, float inv,
+                                            const f2 (&x)[4], const unsigned (&u)[8]) {
+    const f2 k = f2_both(inv);
+    unsigned h[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        float a = x[2 * j] * inv, b = x[2 * j + 1] * inv;
-        if (SR) {
-            a = a == a ? round_e4m3_sr(a, u[2 * j]) : a;
-            b = b == b ? round_e4m3_sr(b, u[2 * j + 1]) : b;
-        }
-        w |= (uint64_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)
-             << (16 * j);
+        float a, b;
+        f2_split(f2_mul(x[j], k), a, b);
+        if (SR) a = round_e4m3_sr(a, u[2 * j]), b = round_e4m3_sr(b, u[2 * j + 1]);
+        h[j] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     }
+    const uint2 w = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
     uint8_t *c = static_cast<uint8_t *>(p) + i;
-    if (vec && valid == 8) {
-        *reinterpret_cast<uint64_t *>(c) = w;
+    if (whole) {
+        __stcs(reinterpret_cast<uint2 *>(c), w);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (j < valid) c[j] = (uint8_t)(w >> (8 * j));
+            if (j < valid) c[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+    }
+}
+
+// ------------------------------------------------------------------ the step
+
+// What a lane has loaded of one block.
+template <bool EIGHT> struct Loaded {
+    Raw8 p, g, m, v;  // m, v: 32-bit moments
+};
+template <> struct Loaded<true> {
+    Raw8 p, g;
+    uint64_t m, v;
+    float ms, vs;
+};
+
+template <bool EIGHT>
+__device__ __forceinline__ void load_block(const AdamTensor &t, int64_t block, int lane,
+                                           Loaded<EIGHT> &l) {
+    const int64_t i = block * kAdamBlock + lane * 8;
+    const int valid = (int)max((int64_t)0, min((int64_t)8, t.n - i));
+    const bool whole = t.vec && valid == 8;
+    l.g = load_raw(t.g, t.gt, i, valid, whole);
+    l.p = load_raw(t.p, t.pt, i, valid, whole);
+    if constexpr (EIGHT) {
+        l.m = load_codes(t.m, i, valid, whole);
+        l.v = load_codes(t.v, i, valid, whole);
+        l.ms = t.ms[block];
+        l.vs = t.vs[block];
+    } else {
+        l.m = load_raw(t.m, DRIFT_T_F32, i, valid, whole);
+        l.v = load_raw(t.v, DRIFT_T_F32, i, valid, whole);
+    }
+}
+
+struct Scalars {
+    f2 b1, b2, c1, c2, eps, neg_a1, rc2, keep, gs;
+    bool scaled;
+};
+
+template <bool EIGHT, bool SR>
+__device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block, int lane,
+                                             const Loaded<EIGHT> &l, const Scalars &k,
+                                             uint64_t state) {
+    const int64_t i = block * kAdamBlock + lane * 8;
+    const int valid = (int)max((int64_t)0, min((int64_t)8, t.n - i));
+    const bool whole = t.vec && valid == 8;
+    f2 p[4], g[4], m[4], v[4], r[4];
+    unpack(l.g, t.gt, g);
+    unpack(l.p, t.pt, p);
+    if constexpr (EIGHT) {
+        decode(l.m, l.ms, m);
+        decode(l.v, l.vs, r);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = f2_mul(r[j], r[j]);
+    } else {
+        unpack(l.m, DRIFT_T_F32, m);
+        unpack(l.v, DRIFT_T_F32, v);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const f2 gj = k.scaled ? f2_mul(g[j], k.gs) : g[j];
+        m[j] = f2_fma(k.b1, m[j], f2_mul(k.c1, gj));
+        v[j] = f2_fma(k.b2, v[j], f2_mul(f2_mul(k.c2, gj), gj));
+        float a, b;
+        f2_split(v[j], a, b);
+        r[j] = f2_pack(__fsqrt_rn(a), __fsqrt_rn(b));
+        f2_split(f2_fma(r[j], k.rc2, k.eps), a, b);
+        const f2 step = f2_mul(f2_mul(k.neg_a1, m[j]), f2_pack(rcp_fast(a), rcp_fast(b)));
+        p[j] = f2_fma(k.keep, p[j], step);
+    }
+    store8(t.p, t.pt, i, valid, whole, p);
+    if (t.ct >= 0) store8(t.copy, t.ct, i, valid, whole, p);
+    if constexpr (EIGHT) {
+        unsigned um[8] = {}, uv[8] = {};
+        if (SR) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint64_t u = splitmix_mix(state + (t.first_draw + i + j + 1) * kGolden);
+                um[j] = (unsigned)(u >> 44);
+                uv[j] = (unsigned)(u >> 24) & 0xfffffu;
+            }
+        }
+        // Elements past the end hold zeros throughout, so they leave an amax as
+        // it is. A block whose values are all below 2^-100 is held as zeros
+        // (448 / amax would overflow); one with an Inf or NaN reads back as NaN, so
+        // that it is not mistaken for a state. Half of the warp divides for m,
+        // half for r.
+        const float am = warp_amax(m), ar = warp_amax(r);
+        const float amax = lane < 16 ? am : ar;
+        float inv = 0.0f, s = 1.0f;
+        if (!(amax <= 3.402823466e38f)) {
+            inv = s = __uint_as_float(0x7fffffffu);
+        } else if (amax >= 0x1p-100f) {
+            inv = 448.0f / amax;
+            s = amax / 448.0f;
+        }
+        if (lane == 0) t.ms[block] = s;
+        if (lane == 16) t.vs[block] = s;
+        store_codes<SR>(t.m, i, valid, whole, __shfl_sync(0xffffffffu, inv, 0), m, um);
+        store_codes<SR>(t.v, i, valid, whole, __shfl_sync(0xffffffffu, inv, 16), r, uv);
+    } else {
+        store8(t.m, DRIFT_T_F32, i, valid, whole, m);
+        store8(t.v, DRIFT_T_F32, i, valid, whole, v);
     }
 }
 
@@ -230,59 +395,30 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
     }
     const AdamTensor &t = a.t[lo];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float a1 = a.scal[0], rc2 = a.scal[1], keep = a.scal[2];
-    const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
+    const uint32_t chunk = blockIdx.x - a.first[lo];
+    // This warp's blocks: warp, warp + 8, ... of the CTA's chunk. The next
+    // block's loads are in flight while one is computed.
+    const int64_t blocks = (t.n + kAdamBlock - 1) / kAdamBlock;
+    const int64_t b0 = (int64_t)chunk * (kAdamThreads / 32 * a.per_warp) + warp;
+    const int n = (int)max((int64_t)0, min((int64_t)a.per_warp,
+                                           (blocks - b0 + kAdamThreads / 32 - 1) /
+                                               (kAdamThreads / 32)));
+    if (n == 0) return;
+    Loaded<EIGHT> next;
+    load_block<EIGHT>(t, b0, lane, next);
+    Scalars k;
+    k.b1 = f2_both(a.b1), k.b2 = f2_both(a.b2), k.c1 = f2_both(a.c1), k.c2 = f2_both(a.c2);
+    k.eps = f2_both(a.eps);
+    k.neg_a1 = f2_both(-a.scal[0]), k.rc2 = f2_both(a.scal[1]), k.keep = f2_both(a.scal[2]);
+    k.scaled = a.grad_scale != nullptr;
+    k.gs = f2_both(k.scaled ? *a.grad_scale : 1.0f);
     const uint64_t state = SR ? *a.rng : 0;
-    const bool vec = t.vec;
-    const int64_t base = (int64_t)(blockIdx.x - a.first[lo]) * kAdamChunk;
 #pragma unroll 1
-    for (int b = 0; b < kAdamBlocksPerWarp; b++) {
-        const int64_t block = base / kAdamBlock + b * (kAdamThreads / 32) + warp;
-        if (block * kAdamBlock >= t.n) break;  // the same for the whole warp
-        const int64_t i = block * kAdamBlock + lane * 8;
-        const int valid = (int)max((int64_t)0, min((int64_t)8, t.n - i));
-        float p[8], g[8], m[8], v[8], r[8];
-        load8(t.g, t.gt, i, valid, vec, g);
-        load8(t.p, t.pt, i, valid, vec, p);
-        if (EIGHT) {
-            load_codes(t.m, i, valid, vec, t.ms[block], m);
-            load_codes(t.v, i, valid, vec, t.vs[block], r);
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = r[j] * r[j];
-        } else {
-            load8(t.m, DRIFT_T_F32, i, valid, vec, m);
-            load8(t.v, DRIFT_T_F32, i, valid, vec, v);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float gj = a.grad_scale ? g[j] * gs : g[j];
-            m[j] = a.b1 * m[j] + a.c1 * gj;
-            v[j] = a.b2 * v[j] + (a.c2 * gj) * gj;
-            r[j] = __fsqrt_rn(v[j]);
-            p[j] = keep * p[j] - __fdiv_rn(a1 * m[j], r[j] * rc2 + a.eps);
-        }
-        store8(t.p, t.pt, i, valid, vec, p);
-        if (t.ct >= 0) store8(t.copy, t.ct, i, valid, vec, p);
-        if (EIGHT) {
-            unsigned um[8] = {}, uv[8] = {};
-            if (SR) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint64_t u = splitmix_mix(state + (t.first_draw + i + j + 1) * kGolden);
-                    um[j] = (unsigned)(u >> 44);
-                    uv[j] = (unsigned)(u >> 24) & 0xfffffu;
-                }
-            }
-            // Lanes past the end hold zeros, which leave the amax as it is.
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j >= valid) m[j] = r[j] = 0.0f;
-            store_codes<SR>(t.m, t.ms, i, block, valid, vec, lane, m, um);
-            store_codes<SR>(t.v, t.vs, i, block, valid, vec, lane, r, uv);
-        } else {
-            store8(t.m, DRIFT_T_F32, i, valid, vec, m);
-            store8(t.v, DRIFT_T_F32, i, valid, vec, v);
-        }
+    for (int b = 0; b < n; b++) {
+        const Loaded<EIGHT> now = next;
+        const int64_t block = b0 + b * (kAdamThreads / 32);
+        if (b + 1 < n) load_block<EIGHT>(t, block + kAdamThreads / 32, lane, next);
+        update_block<EIGHT, SR>(t, block, lane, now, k, state);
     }
 }
 
@@ -296,7 +432,11 @@ int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_
     const bool eight = h->state_bits == 8;
     const bool sr = eight && h->rounding == DRIFT_STOCHASTIC;
     uint64_t draws = 0;
-    for (int64_t i = 0; i < count; i++) draws += (uint64_t)tensors[i].n;
+    int64_t blocks = 0;
+    for (int64_t i = 0; i < count; i++) {
+        draws += (uint64_t)tensors[i].n;
+        blocks += (tensors[i].n + kAdamBlock - 1) / kAdamBlock;
+    }
     uint64_t *rng_used = reinterpret_cast<uint64_t *>(d_scalars + 4);
     adamw_prepare_kernel<<<1, 1, 0, st>>>(d_step, h->beta1, h->beta2, h->lr, d_lr,
                                           h->weight_decay, d_scalars, sr ? d_rng : nullptr, draws,
@@ -311,6 +451,13 @@ int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_
     a.rng = rng_used;
     a.grad_scale = d_grad_scale;
     a.count = 0;
+    // Warps take several blocks in turn, loading ahead, once that leaves four
+    // CTAs an SM; few blocks spread over the SMs instead.
+    a.per_warp = 1;
+    while (a.per_warp < kAdamMostBlocks &&
+           blocks >= (int64_t)a.per_warp * 2 * (kAdamThreads / 32) * 4 * sm_count())
+        a.per_warp *= 2;
+    const uint64_t chunk_len = (uint64_t)kAdamBlock * (kAdamThreads / 32) * a.per_warp;
     uint64_t chunks = 0, drawn = 0;
     auto flush = [&]() {
         if (a.count == 0) return;
@@ -325,7 +472,7 @@ int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_
     for (int64_t i = 0; i < count; i++) {
         const drift_adamw_tensor &t = tensors[i];
         if (t.n == 0) continue;
-        const uint64_t c = ((uint64_t)t.n + kAdamChunk - 1) / kAdamChunk;
+        const uint64_t c = ((uint64_t)t.n + chunk_len - 1) / chunk_len;
         if (a.count == kAdamTensors || chunks + c > 0x7fffffffULL) flush();
         AdamTensor &d = a.t[a.count];
         d.p = t.param, d.g = t.grad, d.m = t.m, d.v = t.v;

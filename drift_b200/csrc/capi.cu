@@ -1251,16 +1251,9 @@ int drift_mx4_dequantize_dev(drift_ctx *ctx, const drift_mx4 *q, int type, void 
     return rc ? fail(rc, "mx4 dequantize launch") : DRIFT_OK;
 }
 
-int drift_mx4_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes) {
-    if (!bytes || !mx4_shape_ok(M, K) || !mx4_shape_ok(N, K))
-        return fail(DRIFT_EINVAL, "bad shape");
-    *bytes = mx4_gemm_workspace(M, N, K);
-    return DRIFT_OK;
-}
-
 int drift_mx4_gemm_dev(drift_ctx *ctx, const drift_mx4 *A, const drift_mx4 *B,
-                       const float *d_bias, int type, void *d_C, int64_t c_stride, void *d_ws,
-                       int64_t ws_bytes, void *stream) {
+                       const float *d_bias, int type, void *d_C, int64_t c_stride,
+                       void *stream) {
     DeviceScope scope(ctx);
     if (scope.status) return scope.status;
     int rc = check_mx4(A);
@@ -1270,11 +1263,8 @@ int drift_mx4_gemm_dev(drift_ctx *ctx, const drift_mx4 *A, const drift_mx4 *B,
         return fail(DRIFT_EINVAL, "bad arguments");
     if (A->rows == 0 || B->rows == 0) return DRIFT_OK;
     if (!d_C) return fail(DRIFT_EINVAL, "null pointer");
-    const int64_t need = mx4_gemm_workspace(A->rows, B->rows, A->cols);
-    if (need && (!d_ws || ws_bytes < need || misaligned(d_ws, 256)))
-        return fail(DRIFT_EINVAL, "workspace too small or misaligned");
-    rc = launch_mx4_gemm(A, B, d_bias, type, d_C, A->rows > 1 ? c_stride : B->rows, d_ws,
-                         ctx->d_err(), pick(ctx, stream));
+    rc = launch_mx4_gemm(A, B, d_bias, type, d_C, A->rows > 1 ? c_stride : B->rows, ctx->d_err(),
+                         pick(ctx, stream));
     return rc ? fail(rc, "mx4 gemm launch") : DRIFT_OK;
 }
 
@@ -1341,7 +1331,8 @@ int drift_adamw_dev(drift_ctx *ctx, const drift_adamw *h, const drift_adamw_tens
         misaligned(d_scalars, 8))
         return fail(DRIFT_EINVAL, "bad arguments");
     if ((h->state_bits != 32 && h->state_bits != 8) ||
-        !(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1 && h->eps >= 0))
+        !(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1 &&
+          (h->eps == 0 || (h->eps >= 1e-30 && h->eps <= 1e30))))
         return fail(DRIFT_EINVAL, "bad hyperparameters");
     if (h->rounding != DRIFT_NEAREST_EVEN &&
         (h->rounding != DRIFT_STOCHASTIC || h->state_bits != 8))

@@ -157,9 +157,8 @@ int launch_mx4_quantize(int headroom, int rm, int type, const void *src, int64_t
 int launch_mx4_dequantize(const drift_mx4 *q, int type, void *dst, int64_t stride,
                           cudaStream_t st);
 // mx4_gemm.cu
-int64_t mx4_gemm_workspace(int64_t M, int64_t N, int64_t K);
 int launch_mx4_gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, int type, void *C,
-                    int64_t c_stride, void *ws, int *d_err, cudaStream_t st);
+                    int64_t c_stride, int *d_err, cudaStream_t st);
 // xent.cu
 int64_t xent_workspace(const drift_xent *op, bool grad);
 int launch_xent(const drift_xent *op, float *loss, float *lse, float *mean, void *ws, int *err,

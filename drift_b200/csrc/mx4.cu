@@ -26,26 +26,50 @@ namespace drift {
 
 // ------------------------------------------------------------------ one block's arithmetic
 
+// A source type. `key` of an element orders like its magnitude, its NaNs above
+// its Inf (kInf) and Inf above the rest, and holds its exponent.
 template <int TYPE> struct MxSrc;
 template <> struct MxSrc<DRIFT_T_F64> {
     using T = double;
     using V = double;
+    static constexpr unsigned kInf = 0x7ff00000u;
     __device__ static V get(T x) { return x; }
+    // The high word, with one bit for a low word that is not zero.
+    __device__ static unsigned key(T x) {
+        return ((unsigned)__double2hiint(x) & 0x7fffffffu) | min((unsigned)__double2loint(x), 1u);
+    }
+    __device__ static int exponent(unsigned key) { return (int)(key >> 20) - 1023; }
 };
 template <> struct MxSrc<DRIFT_T_F32> {
     using T = float;
     using V = float;
+    static constexpr unsigned kInf = 0x7f800000u;
     __device__ static V get(T x) { return x; }
+    __device__ static unsigned key(T x) { return __float_as_uint(x) & 0x7fffffffu; }
+    // A subnormal has its own exponent, as its double has.
+    __device__ static int exponent(unsigned key) {
+        return key >> 23 ? (int)(key >> 23) - 127 : -118 - __clz(key);
+    }
 };
 template <> struct MxSrc<DRIFT_T_BF16> {
     using T = __nv_bfloat16;
     using V = float;
+    static constexpr unsigned kInf = 0x7f80u;
     __device__ static V get(T x) { return __bfloat162float(x); }
+    __device__ static V get_bits(unsigned h) { return __uint_as_float(h << 16); }
+    __device__ static int exponent(unsigned key) {
+        return MxSrc<DRIFT_T_F32>::exponent(key << 16);
+    }
 };
 template <> struct MxSrc<DRIFT_T_FP16> {
     using T = __half;
     using V = float;
+    static constexpr unsigned kInf = 0x7c00u;
     __device__ static V get(T x) { return __half2float(x); }
+    __device__ static V get_bits(unsigned h) { return __half2float(__ushort_as_half((uint16_t)h)); }
+    __device__ static int exponent(unsigned key) {
+        return MxSrc<DRIFT_T_F32>::exponent(__float_as_uint(get_bits(key)));
+    }
 };
 
 // Magnitude for amax: NaN counts as nothing (Quant.java:25-34).
@@ -160,6 +184,64 @@ __device__ __forceinline__ unsigned mx_pack8(const V (&x)[8], const MxScale &s, 
     return w;
 }
 
+// Eight consecutive elements as they lie in memory.
+template <int TYPE> struct MxRaw8 {
+    using S = MxSrc<TYPE>;
+    static constexpr int kVecs = sizeof(typename S::T) * 8 / 16;
+    uint4 w[kVecs];
+    __device__ const unsigned *words() const { return reinterpret_cast<const unsigned *>(w); }
+    __device__ unsigned key() const {  // the largest of the eight
+        if constexpr (sizeof(typename S::T) == 2) {
+            const unsigned *u = words();
+            const unsigned m = __vmaxu2(__vmaxu2(u[0] & 0x7fff7fffu, u[1] & 0x7fff7fffu),
+                                        __vmaxu2(u[2] & 0x7fff7fffu, u[3] & 0x7fff7fffu));
+            return max(m & 0xffffu, m >> 16);
+        } else {
+            const typename S::T *x = reinterpret_cast<const typename S::T *>(w);
+            unsigned m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) m = max(m, S::key(x[j]));
+            return m;
+        }
+    }
+    __device__ void values(typename S::V (&x)[8]) const {
+        if constexpr (sizeof(typename S::T) == 2) {
+            const unsigned *u = words();
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = S::get_bits(u[j / 2] >> (j & 1) * 16 & 0xffffu);
+        } else {
+            const typename S::T *t = reinterpret_cast<const typename S::T *>(w);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = t[j];
+        }
+    }
+};
+
+// The scale of a block from its key, and the factor 2^-shared. Key 0 is a block
+// of zeros, which callers hold as +0 whatever the signs.
+template <class V> struct MxFactor {
+    int shared;
+    V down;
+};
+__device__ __forceinline__ float mx_down(int shared, float) {
+    return shared < 127 ? __uint_as_float((unsigned)(127 - shared) << 23) : 0x1p-127f;
+}
+__device__ __forceinline__ double mx_down(int shared, double) { return pow2(-shared); }
+template <int TYPE>
+__device__ __forceinline__ MxFactor<typename MxSrc<TYPE>::V> mx_factor(unsigned key, int headroom) {
+    MxFactor<typename MxSrc<TYPE>::V> f;
+    const int e = MxSrc<TYPE>::exponent(key) - 2 + headroom;
+    f.shared = key ? max(-127, min(127, e)) : 0;
+    f.down = mx_down(f.shared, f.down);
+    return f;
+}
+
+// Codes to nearest of two elements of a block without Inf or NaN.
+template <class V>
+__device__ __forceinline__ unsigned mx_fast2(V lo, V hi, V down) {
+    return mx_rn2(mx_narrow(lo * down), mx_narrow(hi * down)) & 0xffu;
+}
+
 // ------------------------------------------------------------------ the cast
 
 struct MxCast {
@@ -176,23 +258,60 @@ struct MxCast {
 };
 
 template <int TYPE>
-__device__ __forceinline__ void mx_load8(const MxCast &a, int64_t row, int64_t col, int valid,
-                                         typename MxSrc<TYPE>::V (&x)[8]) {
-    using S = MxSrc<TYPE>;
-    const typename S::T *p =
-        static_cast<const typename S::T *>(a.src) + row * a.row_stride + col;
+__device__ __forceinline__ MxRaw8<TYPE> mx_load8(const MxCast &a, int64_t row, int64_t col,
+                                                 int valid) {
+    using T = typename MxSrc<TYPE>::T;
+    const T *p = static_cast<const T *>(a.src) + row * a.row_stride + col;
+    MxRaw8<TYPE> r;
     if (a.vec && valid == 8) {
-        constexpr int kVec = sizeof(typename S::T) * 8 / 16;
-        uint4 w[kVec];
 #pragma unroll
-        for (int j = 0; j < kVec; j++) w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
-        const typename S::T *q = reinterpret_cast<const typename S::T *>(w);
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = S::get(q[j]);
+        for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++)
+            r.w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
     } else {
+        T *t = reinterpret_cast<T *>(r.w);
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = j < valid ? S::get(p[j]) : (typename S::V)0;
+        for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++) r.w[j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < valid) t[j] = p[j];
     }
+    return r;
+}
+
+// Eight elements of a block that four neighbouring lanes share: their codes and
+// the block's shared exponent. Blocks without Inf and NaN, to nearest, take the
+// short way; elements past the end are zeros and change nothing.
+template <int TYPE>
+__device__ __forceinline__ unsigned mx_cast8(const MxCast &a, const MxRaw8<TYPE> &r, int valid,
+                                             uint64_t state, uint64_t draw, int &shared,
+                                             unsigned &clamps, int &err) {
+    using S = MxSrc<TYPE>;
+    using V = typename S::V;
+    unsigned key = r.key();
+    key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
+    key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
+    V x[8];
+    r.values(x);
+    if (__all_sync(0xffffffffu, key < S::kInf) && a.rm == DRIFT_NEAREST_EVEN) {
+        const MxFactor<V> f = mx_factor<TYPE>(key, a.headroom);
+        shared = f.shared;
+        unsigned w = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w |= mx_fast2(x[2 * j], x[2 * j + 1], f.down) << (8 * j);
+        if (a.clamped) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) clamps += fabs(x[j] * f.down) > (V)6;
+        }
+        return key ? w : 0;
+    }
+    V amax = (V)0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) amax = fmax(amax, mx_mag(x[j]));
+    amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const MxScale s = mx_scale(amax, a.headroom);
+    shared = s.shared;
+    return mx_pack8(x, s, a.rm, state, draw, 1, valid, clamps, err);
 }
 
 __device__ __forceinline__ void mx_finish(unsigned clamps, int err, unsigned long long *clamped,
@@ -205,53 +324,111 @@ __device__ __forceinline__ void mx_finish(unsigned clamps, int err, unsigned lon
     }
 }
 
-// Blocks along rows: a warp takes 256 elements of one row (eight blocks, two
-// tiles of scales) at a time. Rows past the end up to the tile's 128, and
-// blocks past the row's end, get their padding bytes.
-template <int TYPE>
+// Blocks along rows: a warp takes U items at a time, each 256 elements of one
+// row (eight blocks, two tiles of scales), with all their loads in flight. Rows
+// past the end up to the tile's 128, and blocks past the row's end, get their
+// padding bytes.
+template <int TYPE, int U>
 __global__ void __launch_bounds__(256) mx4_rows_kernel(const MxCast a, uint32_t per_row,
                                                        uint32_t items) {
-    using V = typename MxSrc<TYPE>::V;
     const int lane = threadIdx.x & 31;
     const int64_t blocks = mx4_blocks(a.cols), row_bytes = blocks * 16;
     const uint64_t state = a.rm == DRIFT_STOCHASTIC ? *a.state : 0;
     unsigned clamps = 0;
     int err = 0;
-    const uint32_t stride = gridDim.x * 8;
-    for (uint32_t it = blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += stride) {
-        const uint32_t row = it / per_row, chunk = it - row * per_row;
-        const int64_t col = (int64_t)chunk * 256 + lane * 8;
-        const int64_t block = col >> 5;
-        const int valid =
-            row < a.rows ? (int)max((int64_t)0, min((int64_t)8, a.cols - col)) : 0;
-        V x[8];
-        mx_load8<TYPE>(a, row, col, valid, x);
-        V amax = (V)0;
+    const uint32_t stride = gridDim.x * 8 * U;
+    for (uint32_t it = (blockIdx.x * 8 + (threadIdx.x >> 5)) * U; it < items; it += stride) {
+        MxRaw8<TYPE> raw[U];
+        uint32_t row[U];
+        int64_t col[U];
+        int valid[U];
 #pragma unroll
-        for (int j = 0; j < 8; j++) amax = fmax(amax, mx_mag(x[j]));
-        amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const MxScale s = mx_scale(amax, a.headroom);
-        const unsigned w = mx_pack8(x, s, a.rm, state, (uint64_t)row * a.cols + col, 1, valid,
-                                    clamps, err);
-        if (row < a.rows && block < blocks)
-            *reinterpret_cast<unsigned *>(a.codes + row * row_bytes + col / 2) = w;
-        // Lanes 0 and 16 gather the four scale bytes of their tile.
-        const unsigned byte = row < a.rows && block < blocks ? (unsigned)(s.shared + 127) : 127u;
-        unsigned four = byte;
-        four |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
-        four |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
-        four |= __shfl_down_sync(0xffffffffu, byte, 12) << 24;
-        if ((lane & 15) == 0)
-            *reinterpret_cast<unsigned *>(a.scales + mx4_scale_offset(row, block, per_row * 2)) =
-                four;
+        for (int u = 0; u < U; u++) {
+            row[u] = (it + u) / per_row;
+            col[u] = (int64_t)(it + u - row[u] * per_row) * 256 + lane * 8;
+            valid[u] = it + u < items && row[u] < a.rows
+                           ? (int)max((int64_t)0, min((int64_t)8, a.cols - col[u])) : 0;
+            raw[u] = mx_load8<TYPE>(a, row[u], col[u], valid[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            int shared;
+            const unsigned w = mx_cast8<TYPE>(a, raw[u], valid[u], state,
+                                              (uint64_t)row[u] * a.cols + col[u], shared, clamps,
+                                              err);
+            const int64_t block = col[u] >> 5;
+            const bool in = it + u < items && row[u] < a.rows && block < blocks;
+            if (in) *reinterpret_cast<unsigned *>(a.codes + row[u] * row_bytes + col[u] / 2) = w;
+            // Lanes 0 and 16 gather the four scale bytes of their tile.
+            const unsigned byte = in ? (unsigned)(shared + 127) : 127u;
+            unsigned four = byte;
+            four |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
+            four |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
+            four |= __shfl_down_sync(0xffffffffu, byte, 12) << 24;
+            if ((lane & 15) == 0 && it + u < items)
+                *reinterpret_cast<unsigned *>(
+                    a.scales + mx4_scale_offset(row[u], block, per_row * 2)) = four;
+        }
     }
     mx_finish(clamps, err, a.clamped, a.err);
 }
 
-// Blocks down columns (and along rows too, where a.codes is given): a CTA
-// stages 128 rows x 64 columns of the source.
-constexpr int kMxTr = 128, kMxTc = 64;
+// Blocks down columns (and along rows too, where a.codes is given). A CTA takes
+// 128 rows of 128 columns (64 of the wider types): the loads' registers give the
+// row cast, shared memory the columns, of which a thread casts one 32-bit word
+// wide (two 16-bit columns) of 32 rows. Codes go back through shared memory, so
+// that a column's 64 bytes leave together.
+constexpr int kMxTr = 128;
+template <int TYPE> struct MxTile {
+    using T = typename MxSrc<TYPE>::T;
+    static constexpr int kWide = sizeof(T) == 2 ? 2 : 1;       // columns a thread casts
+    static constexpr int kCols = 64 * kWide;
+    static constexpr int kLdBytes = kCols * (int)sizeof(T) + 16;
+    static constexpr int kStage = kCols * 80;                  // codes: 64 bytes a column, padded
+    static constexpr int kSmem = kMxTr * kLdBytes > kStage ? kMxTr * kLdBytes : kStage;
+    static constexpr int kLoads = kMxTr * kCols / 8 / 256;     // groups of eight a thread loads
+};
+
+// One column's block of 32 to 16 bytes of codes.
+template <int TYPE>
+__device__ __forceinline__ uint4 mx_cast_col(const MxCast &a, const typename MxSrc<TYPE>::V (&x)[32],
+                                             unsigned key, uint64_t state, uint64_t draw,
+                                             int &shared, unsigned &clamps, int &err) {
+    using S = MxSrc<TYPE>;
+    using V = typename S::V;
+    uint4 w;
+    unsigned *wp = reinterpret_cast<unsigned *>(&w);
+    if (key < S::kInf && a.rm == DRIFT_NEAREST_EVEN) {
+        const MxFactor<V> f = mx_factor<TYPE>(key, a.headroom);
+        shared = f.shared;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            wp[q] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                wp[q] |= mx_fast2(x[q * 8 + 2 * j], x[q * 8 + 2 * j + 1], f.down) << (8 * j);
+            if (!key) wp[q] = 0;
+        }
+        if (a.clamped_t) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) clamps += fabs(x[j] * f.down) > (V)6;
+        }
+        return w;
+    }
+    V amax = (V)0;
+#pragma unroll
+    for (int j = 0; j < 32; j++) amax = fmax(amax, mx_mag(x[j]));
+    const MxScale s = mx_scale(amax, a.headroom);
+    shared = s.shared;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        V y[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = x[q * 8 + j];
+        wp[q] = mx_pack8(y, s, a.rm, state, draw + (uint64_t)q * 8 * a.cols, a.cols, 8, clamps, err);
+    }
+    return w;
+}
 
 template <int TYPE>
 __global__ void __launch_bounds__(256) mx4_cols_kernel(const MxCast a, uint32_t row_tiles,
@@ -259,105 +436,117 @@ __global__ void __launch_bounds__(256) mx4_cols_kernel(const MxCast a, uint32_t 
     using S = MxSrc<TYPE>;
     using T = typename S::T;
     using V = typename S::V;
-    // 8 elements of padding a row: column reads by a warp's 32 lanes then touch
-    // consecutive words of one row.
-    constexpr int kLd = kMxTc + 16 / (int)sizeof(T);
+    using G = MxTile<TYPE>;
     extern __shared__ __align__(16) unsigned char mx_smem[];
-    T *tile = reinterpret_cast<T *>(mx_smem);
     const uint32_t tile_r = blockIdx.x / col_tiles, tile_c = blockIdx.x - tile_r * col_tiles;
-    const int64_t r0 = (int64_t)tile_r * kMxTr, c0 = (int64_t)tile_c * kMxTc;
+    const int64_t r0 = (int64_t)tile_r * kMxTr, c0 = (int64_t)tile_c * G::kCols;
     const int tid = threadIdx.x, lane = tid & 31;
     const uint64_t state = a.rm == DRIFT_STOCHASTIC ? *a.state : 0;
-    constexpr int kPer = 16 / sizeof(T), kVecs = kMxTc / kPer;
-    for (int i = tid; i < kMxTr * kVecs; i += 256) {
-        const int r = i / kVecs, c = i % kVecs * kPer;
-        const T *p = static_cast<const T *>(a.src) + (r0 + r) * a.row_stride + c0 + c;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (r0 + r < a.rows) {
-            if (a.vec && c0 + c + kPer <= a.cols) {
-                w = __ldg(reinterpret_cast<const uint4 *>(p));
-            } else {
-                T *q = reinterpret_cast<T *>(&w);
-#pragma unroll
-                for (int j = 0; j < kPer; j++)
-                    if (c0 + c + j < a.cols) q[j] = p[j];
-            }
-        }
-        *reinterpret_cast<uint4 *>(tile + r * kLd + c) = w;
-    }
-    __syncthreads();
 
-    // Down columns: thread = (column, block of 32 rows).
-    {
-        unsigned clamps = 0;
-        int err = 0;
-        const int c = tid & 63, b = tid >> 6;
-        const int64_t col = c0 + c, row = r0 + b * 32;
-        const int64_t k_tiles = mx4_k_tiles(a.rows), blocks = mx4_blocks(a.rows);
-        V amax = (V)0;
+    constexpr int kGroups = G::kCols / 8;  // groups of eight in a row of the tile
+    MxRaw8<TYPE> raw[G::kLoads];
 #pragma unroll
-        for (int j = 0; j < 32; j++)
-            amax = fmax(amax, mx_mag(S::get(tile[(b * 32 + j) * kLd + c])));
-        const MxScale s = mx_scale(amax, a.headroom);
-        uint4 w;
-        unsigned *wp = reinterpret_cast<unsigned *>(&w);
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            V x[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = S::get(tile[(b * 32 + q * 8 + j) * kLd + c]);
-            wp[q] = mx_pack8(x, s, a.rm, state,
-                             a.draw_t + (uint64_t)(row + q * 8) * a.cols + col, a.cols, 8, clamps,
-                             err);
-        }
-        if (col < a.cols && row < a.rows)
-            *reinterpret_cast<uint4 *>(a.codes_t + col * blocks * 16 + (row >> 5) * 16) = w;
-        // Scale bytes, with the padding of the last tiles: this CTA's columns up
-        // to the tile's 128 rows, and blocks up to a whole pair of tiles.
-        const int64_t last = mx4_row_tiles(a.cols) * 128;
-        if (col < last) {
-            a.scales_t[mx4_scale_offset(col, row >> 5, k_tiles)] =
-                col < a.cols && row < a.rows ? (uint8_t)(s.shared + 127) : (uint8_t)127;
-            if (tile_r + 1 == row_tiles && tile_r % 2 == 0)
-                a.scales_t[mx4_scale_offset(col, (row >> 5) + 4, k_tiles)] = 127;
-        }
-        mx_finish(clamps, err, a.clamped_t, a.err);
+    for (int i = 0; i < G::kLoads; i++) {
+        const int at = i * 256 + tid, r = at / kGroups, c = at % kGroups * 8;
+        const int valid = r0 + r < a.rows
+                              ? (int)max((int64_t)0, min((int64_t)8, a.cols - c0 - c)) : 0;
+        raw[i] = mx_load8<TYPE>(a, r0 + r, c0 + c, valid);
     }
-    if (!a.codes) return;
+#pragma unroll
+    for (int i = 0; i < G::kLoads; i++) {
+        const int at = i * 256 + tid, r = at / kGroups, c = at % kGroups * 8;
+        uint4 *to = reinterpret_cast<uint4 *>(mx_smem + r * G::kLdBytes + c * sizeof(T));
+#pragma unroll
+        for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++) to[j] = raw[i].w[j];
+    }
 
-    // Along rows: eight elements a thread, four threads a block of 32.
-    {
+    if (a.codes) {
         unsigned clamps = 0;
         int err = 0;
         const int64_t blocks = mx4_blocks(a.cols), k_tiles = mx4_k_tiles(a.cols);
 #pragma unroll
-        for (int i = 0; i < kMxTr * kMxTc / 8 / 256; i++) {
-            const int at = i * 256 + tid, r = at >> 3, c = (at & 7) * 8;
-            V x[8];
-            V amax = (V)0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[j] = S::get(tile[r * kLd + c + j]);
-                amax = fmax(amax, mx_mag(x[j]));
-            }
-            amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const MxScale s = mx_scale(amax, a.headroom);
-            const int64_t row = r0 + r, col = c0 + c, block = col >> 5;
-            const unsigned w =
-                mx_pack8(x, s, a.rm, state, (uint64_t)row * a.cols + col, 1, 8, clamps, err);
+        for (int i = 0; i < G::kLoads; i++) {
+            const int at = i * 256 + tid;
+            const int64_t row = r0 + at / kGroups, col = c0 + at % kGroups * 8, block = col >> 5;
+            int shared;
+            const unsigned w = mx_cast8<TYPE>(a, raw[i], 8, state, (uint64_t)row * a.cols + col,
+                                              shared, clamps, err);
             const bool in = row < a.rows && block < blocks;
             if (in) *reinterpret_cast<unsigned *>(a.codes + row * blocks * 16 + col / 2) = w;
             if ((lane & 3) == 0 && block < k_tiles * 4) {
                 a.scales[mx4_scale_offset(row, block, k_tiles)] =
-                    in ? (uint8_t)(s.shared + 127) : (uint8_t)127;
+                    in ? (uint8_t)(shared + 127) : (uint8_t)127;
                 // The last columns' CTA also writes the pair's remaining blocks.
                 if (tile_c + 1 == col_tiles)
-                    for (int64_t b = block + 2; b < k_tiles * 4; b += 2)
+                    for (int64_t b = block + G::kCols / 32; b < k_tiles * 4; b += G::kCols / 32)
                         a.scales[mx4_scale_offset(row, b, k_tiles)] = 127;
             }
         }
         mx_finish(clamps, err, a.clamped, a.err);
+    }
+    __syncthreads();
+
+    // Down columns: thread = (word of columns, block of 32 rows).
+    unsigned clamps = 0;
+    int err = 0;
+    const int word = tid & 63, b = tid >> 6;
+    const int64_t row = r0 + b * 32;
+    uint4 codes[G::kWide];
+    int shared[G::kWide];
+    if constexpr (G::kWide == 2) {
+        unsigned u[32], m = 0;
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            u[j] = *reinterpret_cast<const unsigned *>(mx_smem + (b * 32 + j) * G::kLdBytes +
+                                                       word * 4);
+            m = __vmaxu2(m, u[j] & 0x7fff7fffu);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            V x[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) x[j] = S::get_bits(u[j] >> h * 16 & 0xffffu);
+            codes[h] = mx_cast_col<TYPE>(a, x, m >> h * 16 & 0xffffu, state,
+                                         a.draw_t + (uint64_t)row * a.cols + c0 + word * 2 + h,
+                                         shared[h], clamps, err);
+        }
+    } else {
+        V x[32];
+        unsigned m = 0;
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            x[j] = *reinterpret_cast<const T *>(mx_smem + (b * 32 + j) * G::kLdBytes +
+                                                word * sizeof(T));
+            m = max(m, S::key(x[j]));
+        }
+        codes[0] = mx_cast_col<TYPE>(a, x, m, state, a.draw_t + (uint64_t)row * a.cols + c0 + word,
+                                     shared[0], clamps, err);
+    }
+    __syncthreads();
+    const int64_t k_tiles = mx4_k_tiles(a.rows), blocks = mx4_blocks(a.rows);
+    const int64_t last = mx4_row_tiles(a.cols) * 128;
+#pragma unroll
+    for (int h = 0; h < G::kWide; h++) {
+        const int c = word * G::kWide + h;
+        *reinterpret_cast<uint4 *>(mx_smem + c * 80 + b * 16) = codes[h];
+        // Scale bytes, with the padding of the last tiles: this CTA's columns up to
+        // the tile's 128 rows, and blocks up to a whole pair of tiles.
+        const int64_t col = c0 + c;
+        if (col < last) {
+            a.scales_t[mx4_scale_offset(col, row >> 5, k_tiles)] =
+                col < a.cols && row < a.rows ? (uint8_t)(shared[h] + 127) : (uint8_t)127;
+            if (tile_r + 1 == row_tiles && tile_r % 2 == 0)
+                a.scales_t[mx4_scale_offset(col, (row >> 5) + 4, k_tiles)] = 127;
+        }
+    }
+    mx_finish(clamps, err, a.clamped_t, a.err);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < G::kCols * 4 / 256; i++) {
+        const int at = i * 256 + tid, c = at >> 2, q = at & 3;
+        if (c0 + c < a.cols && r0 + q * 32 < a.rows)
+            *reinterpret_cast<uint4 *>(a.codes_t + (c0 + c) * blocks * 16 + (r0 / 32 + q) * 16) =
+                *reinterpret_cast<const uint4 *>(mx_smem + c * 80 + q * 16);
     }
 }
 
@@ -365,23 +554,29 @@ __global__ void mx4_advance_kernel(uint64_t *state, uint64_t draws) { *state += 
 
 template <int TYPE>
 static int launch_cast(const MxCast &a, cudaStream_t st) {
-    using T = typename MxSrc<TYPE>::T;
     if (!a.codes_t) {
         const uint32_t per_row = (uint32_t)(mx4_k_tiles(a.cols) / 2);
         const uint32_t items = (uint32_t)(mx4_row_tiles(a.rows) * 128) * per_row;
-        const uint32_t grid = std::min<uint32_t>((items + 7) / 8, (uint32_t)sm_count() * 8);
-        mx4_rows_kernel<TYPE><<<grid, 256, 0, st>>>(a, per_row, items);
+        const uint32_t sms = (uint32_t)sm_count();
+        // Four items a warp once that still leaves every SM two CTAs.
+        if (items >= sms * 2 * 8 * 4) {
+            const uint32_t grid = std::min<uint32_t>((items + 31) / 32, sms * 8);
+            mx4_rows_kernel<TYPE, 4><<<grid, 256, 0, st>>>(a, per_row, items);
+        } else {
+            mx4_rows_kernel<TYPE, 1><<<(items + 7) / 8, 256, 0, st>>>(a, per_row, items);
+        }
     } else {
-        constexpr int smem = kMxTr * (kMxTc * (int)sizeof(T) + 16);
-        if (smem > 48 * 1024 &&
+        using G = MxTile<TYPE>;
+        if (G::kSmem > 48 * 1024 &&
             cudaFuncSetAttribute(mx4_cols_kernel<TYPE>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 smem) != cudaSuccess)
+                                 G::kSmem) != cudaSuccess)
             return DRIFT_ECUDA;
         // Columns up to the tile's 128, so that every padding byte is written.
         const uint32_t row_tiles = (uint32_t)mx4_row_tiles(a.rows);
-        const uint32_t col_tiles = (uint32_t)mx4_row_tiles(a.cols) * 2;
-        mx4_cols_kernel<TYPE><<<row_tiles * col_tiles, 256, smem, st>>>(a, row_tiles, col_tiles);
+        const uint32_t col_tiles = (uint32_t)mx4_row_tiles(a.cols) * (128 / G::kCols);
+        mx4_cols_kernel<TYPE><<<row_tiles * col_tiles, 256, G::kSmem, st>>>(a, row_tiles,
+                                                                           col_tiles);
     }
     return DRIFT_OK;
 }
@@ -418,10 +613,13 @@ int launch_mx4_quantize(int headroom, int rm, int type, const void *src, int64_t
 
 // ------------------------------------------------------------------ back to values
 
-__device__ __forceinline__ double mx_value(unsigned code, int shared) {
-    const unsigned m = code & 7;
-    const double v = m < 2 ? 0.5 * m : (double)(2 + (m & 1)) * (double)(1 << (m >> 1)) * 0.25;
-    return (code & 8 ? -v : v) * pow2(shared);  // exact
+// Two elements' values without their scale.
+__device__ __forceinline__ float2 mx_pair(unsigned byte) {
+    unsigned h;
+    asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %1;\n cvt.rn.f16x2.e2m1x2 %0, a;\n}"
+        : "=r"(h)
+        : "r"(byte));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
 // Eight values a thread. A double, float or bf16 holds every value exactly,
@@ -436,15 +634,20 @@ __global__ void __launch_bounds__(256) mx4_values_kernel(const uint8_t *codes,
         for (uint32_t g = blockIdx.x * 256 + threadIdx.x; g < groups; g += gridDim.x * 256) {
             const int64_t col = (int64_t)g * 8;
             const unsigned w =
-                *reinterpret_cast<const unsigned *>(codes + row * row_bytes + col / 2);
+                __ldg(reinterpret_cast<const unsigned *>(codes + row * row_bytes + col / 2));
             const int shared = (int)scales[mx4_scale_offset(row, col >> 5, k_tiles)] - 127;
             __align__(16) T v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const double d = mx_value(w >> (4 * j) & 15, shared);
-                if constexpr (sizeof(T) == 8) v[j] = d;
-                else if constexpr (sizeof(T) == 4) v[j] = (float)d;
-                else v[j] = T((float)d);
+            for (int j = 0; j < 4; j++) {
+                const float2 f = mx_pair(w >> (8 * j) & 0xffu);
+                if constexpr (sizeof(T) == 8) {
+                    const double up = pow2(shared);
+                    v[2 * j] = f.x * up, v[2 * j + 1] = f.y * up;
+                } else {
+                    const float up = shared > -127 ? __uint_as_float((unsigned)(shared + 127) << 23)
+                                                   : 0x1p-127f;
+                    v[2 * j] = T(f.x * up), v[2 * j + 1] = T(f.y * up);
+                }
             }
             T *p = dst + row * stride + col;
             if (vec && col + 8 <= cols) {

@@ -35,11 +35,6 @@ __global__ void __launch_bounds__(256) fill_bias_kernel(T *C, int64_t stride, in
         C[i / cols * stride + i % cols] = T(bias ? bias[i % cols] : 0.0f);
 }
 
-int64_t mx4_gemm_workspace(int64_t M, int64_t N, int64_t K) {
-    (void)M, (void)N, (void)K;
-    return 0;
-}
-
 template <class T>
 static int gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C, int64_t c_stride,
                 int *d_err, cudaStream_t st) {
@@ -62,8 +57,7 @@ static int gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C,
 }
 
 int launch_mx4_gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, int type, void *C,
-                    int64_t c_stride, void *ws, int *d_err, cudaStream_t st) {
-    (void)ws;
+                    int64_t c_stride, int *d_err, cudaStream_t st) {
     switch (type) {
         case DRIFT_T_F64: return gemm(a, b, bias, (double *)C, c_stride, d_err, st);
         case DRIFT_T_F32: return gemm(a, b, bias, (float *)C, c_stride, d_err, st);

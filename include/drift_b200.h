@@ -577,13 +577,11 @@ DRIFT_API int drift_mx4_dequantize_dev(drift_ctx *ctx, const drift_mx4 *q, int t
  * C[i * c_stride + o] = sum over k of a(i, k) b(o, k) (+ d_bias[o]): A->rows x
  * B->rows outputs of `type`, A->cols == B->cols. Products are exact, sums
  * fp32 in the tensor cores' order (contrast drift_gemm_dev, where the order is
- * the policy's). d_ws holds the bytes that drift_mx4_gemm_workspace gives
- * (NULL when 0), 256-byte aligned, untouched by others until the call's work is done.
+ * the policy's).
  */
-DRIFT_API int drift_mx4_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes);
 DRIFT_API int drift_mx4_gemm_dev(drift_ctx *ctx, const drift_mx4 *A, const drift_mx4 *B,
-                       const float *d_bias, int type, void *d_C, int64_t c_stride, void *d_ws,
-                       int64_t ws_bytes, void *stream);
+                       const float *d_bias, int type, void *d_C, int64_t c_stride,
+                       void *stream);
 
 /*
  * A linear layer's softmax cross entropy (Pass.java:134-153) over a vocabulary,
@@ -626,9 +624,10 @@ DRIFT_API int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, c
 /*
  * One AdamW step over `count` tensors (decoupled weight decay; drift_adam_dev's
  * update with weight_decay 0, in 32 bits). Per element, each operation rounded
- * to fp32 on its own:
- *   m' = b1 m + (1-b1) g;  v' = b2 v + ((1-b2) g) g;  r = sqrt(v')
- *   p' = (1 - lr wd) p - (lr / (1 - b1^t) m') / (r / sqrt(1 - b2^t) + eps)
+ * to fp32, fma(a, b, c) once:
+ *   m' = fma(b1, m, (1-b1) g);  v' = fma(b2, v, ((1-b2) g) g);  r = sqrt(v')
+ *   p' = fma(1 - lr wd, p, -(lr / (1 - b1^t) m') / fma(r, 1 / sqrt(1 - b2^t), eps))
+ * the quotient within two units in the last place; eps is 0 or in [1e-30, 1e30].
  * state_bits 32: m and v are floats. state_bits 8: m and r are held as e4m3
  * codes with one float scale per 256 consecutive elements, code =
  * e4m3(x * (448 / amax)), value = code * (amax / 448), rounded to nearest or, with
