@@ -26,6 +26,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "pairs.cuh"
 
 namespace drift {
 
@@ -74,32 +75,6 @@ __global__ void adamw_prepare_kernel(int64_t *step, double b1, double b2, double
     }
 }
 
-// ------------------------------------------------------------------ pairs of floats
-//
-// Two elements an instruction (mul.rn.f32x2, fma.rn.f32x2): each half is rounded
-// as the scalar operation would. There is no f2_add: the assembler contracts a
-// product and an add.rn.f32x2 into one fused operation, against -fmad=false, so
-// the sums are written as the fused operations that they become.
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 f2_pack(float a, float b) {
-    f2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ f2 f2_both(float a) { return f2_pack(a, a); }
-__device__ __forceinline__ void f2_split(f2 x, float &a, float &b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
-}
-__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
-    f2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 __device__ __forceinline__ float rcp_fast(float x) {  // within one unit
     float r;
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));

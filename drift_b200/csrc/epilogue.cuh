@@ -1,5 +1,5 @@
-// epilogue.cuh — epilogues of tc.cuh's products that write a matrix: a thread
-// holds 128 consecutive columns of one row.
+// epilogue.cuh — epilogues of tc.cuh's products that write a matrix. A thread
+// holds 128 consecutive columns of one row, row0 + lane.
 #pragma once
 
 #include <cstdint>
@@ -26,25 +26,55 @@ template <class T> inline bool rows_aligned(const T *p, int64_t stride) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
 }
 
-// Columns c0 .. c0+7 of a thread's row.
-template <class T>
-__device__ __forceinline__ void store8(T *p, const float *x, int64_t left, bool vec) {
-    if (vec && left >= 8) {
-        if constexpr (sizeof(T) == 8) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                reinterpret_cast<double2 *>(p)[j] = make_double2(x[2 * j], x[2 * j + 1]);
-        } else if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-            reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-        } else {
-            *reinterpret_cast<uint4 *>(p) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
-                                                       pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-        }
+// The 16 bytes of columns j .. of a thread's row, in the output's type.
+template <class T> __device__ __forceinline__ uint4 pack16(const float *x) {
+    if constexpr (sizeof(T) == 8) {
+        const double2 d = make_double2(x[0], x[1]);
+        return *reinterpret_cast<const uint4 *>(&d);
+    } else if constexpr (sizeof(T) == 4) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                          __float_as_uint(x[3]));
     } else {
+        return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
+                          pack2<T>(x[6], x[7]));
+    }
+}
+
+__device__ __forceinline__ void smem_store16(unsigned at, uint4 w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z),
+                 "r"(w.w)
+                 : "memory");
+}
+__device__ __forceinline__ uint4 smem_load16(unsigned at) {
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                 : "r"(at)
+                 : "memory");
+    return w;
+}
+
+// Passes a warp's 32 rows x 128 columns (lane = row) through shared memory, 128
+// bytes a row at a time, so that eight lanes hold a row's 128 bytes and a store
+// instruction covers four whole lines: lane by lane a store of 16 bytes would
+// touch 32. The 16-byte units of a row are swizzled by its number against bank
+// conflicts. `put(row, column, word)` gets 16 bytes of row row0 + row.
+template <class T, class Put>
+__device__ __forceinline__ void by_rows(const float (&v)[128], unsigned staging, int lane, Put put) {
+    constexpr int kCols = 128 / (int)sizeof(T), kUnit = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int c = 0; c < 128; c += kCols) {
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (j < left) p[j] = T(x[j]);
+            smem_store16(staging + lane * 128 + ((j ^ (lane & 7)) << 4),
+                         pack16<T>(v + c + j * kUnit));
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int row = i * 4 + (lane >> 3), j = lane & 7;
+            put(row, c + j * kUnit, smem_load16(staging + row * 128 + ((j ^ (row & 7)) << 4)));
+        }
+        __syncwarp();
     }
 }
 
@@ -53,12 +83,14 @@ template <class T> struct StoreEpi {
     T *c;
     int64_t stride, rows, cols;
     const float *bias;
-    const float *alpha;  // a power of two, or null for 1
+    const float *alpha;  // null for 1
+    float beta;          // a power of two, 1 without alpha
     bool vec;
-    __device__ __forceinline__ void run(float (&v)[128], int64_t row, int64_t col, const tc::Work &,
-                                        int) const {
+    __device__ __forceinline__ void run(float (&v)[128], int64_t row0, int64_t col, const tc::Work &,
+                                        int lane, unsigned staging) const {
+        if (col >= cols) return;
         if (alpha) {
-            const float f = *alpha;
+            const float f = *alpha * beta;
 #pragma unroll
             for (int j = 0; j < 128; j++) v[j] *= f;
         }
@@ -67,10 +99,28 @@ template <class T> struct StoreEpi {
             for (int j = 0; j < 128; j++)
                 if (col + j < cols) v[j] += __ldg(bias + col + j);
         }
-        if (row >= rows) return;
-        T *p = c + row * stride + col;
+        if (vec) {
+            T *p = c + row0 * stride + col;
+            const int64_t left = cols - col;
+            by_rows<T>(v, staging, lane, [&](int r, int j, uint4 w) {
+                constexpr int kUnit = 16 / (int)sizeof(T);
+                if (row0 + r >= rows || j >= left) return;
+                T *to = p + r * stride + j;
+                if (j + kUnit <= left) {
+                    *reinterpret_cast<uint4 *>(to) = w;
+                } else {
+                    const T *x = reinterpret_cast<const T *>(&w);
 #pragma unroll
-        for (int j = 0; j < 128; j += 8) store8(p + j, v + j, cols - col - j, vec);
+                    for (int u = 0; u < kUnit; u++)
+                        if (j + u < left) to[u] = x[u];
+                }
+            });
+        } else if (row0 + lane < rows) {
+            T *p = c + (row0 + lane) * stride + col;
+#pragma unroll
+            for (int j = 0; j < 128; j++)
+                if (col + j < cols) p[j] = T(v[j]);
+        }
     }
 };
 
@@ -80,20 +130,21 @@ struct PartEpi {
     float *c;
     int64_t part, stride, rows, cols;  // stride a multiple of 4, c 16-byte aligned
     bool add;
-    __device__ __forceinline__ void run(float (&v)[128], int64_t row, int64_t col,
-                                        const tc::Work &w, int) const {
-        if (row >= rows) return;
-        float *p = c + w.split * part + row * stride + col;
-#pragma unroll
-        for (int j = 0; j < 128; j += 4) {
-            if (col + j >= cols) break;  // the stride's padding columns may be written
+    __device__ __forceinline__ void run(float (&v)[128], int64_t row0, int64_t col,
+                                        const tc::Work &w, int lane, unsigned staging) const {
+        if (col >= cols) return;
+        float *p = c + w.split * part + row0 * stride + col;
+        by_rows<float>(v, staging, lane, [&](int r, int j, uint4 x) {
+            if (row0 + r >= rows || col + j >= cols) return;  // padding columns may be written
+            float *to = p + r * stride + j;
             if (add)
-                asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + j),
-                             "f"(v[j]), "f"(v[j + 1]), "f"(v[j + 2]), "f"(v[j + 3])
+                asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to),
+                             "f"(__uint_as_float(x.x)), "f"(__uint_as_float(x.y)),
+                             "f"(__uint_as_float(x.z)), "f"(__uint_as_float(x.w))
                              : "memory");
             else
-                *reinterpret_cast<float4 *>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        }
+                *reinterpret_cast<uint4 *>(to) = x;
+        });
     }
 };
 

@@ -21,6 +21,7 @@
 #include "codec.cuh"
 #include "internal.h"
 #include "mx4.cuh"
+#include "pairs.cuh"
 
 namespace drift {
 
@@ -115,15 +116,17 @@ __device__ __forceinline__ float mx_narrow(double x) {
     return (double)f == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
 
-// Codes of two values to nearest, ties to the even code, saturating at 6: lo in
-// bits 0-3, hi in bits 4-7.
-__device__ __forceinline__ unsigned mx_rn2(float lo, float hi) {
-    unsigned out;
-    asm("{\n .reg .b8 t, z;\n cvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n"
-        " cvt.rn.satfinite.e2m1x2.f32 z, %3, %3;\n mov.b32 %0, {t, z, z, z};\n}"
-        : "=r"(out)
-        : "f"(hi), "f"(lo), "f"(0.0f));
-    return out;
+// Codes of eight values to nearest, ties to the even code, saturating at 6: value
+// j in bits 4j to 4j+3.
+__device__ __forceinline__ unsigned mx_rn8(const float (&y)[8]) {
+    unsigned w;
+    asm("{\n .reg .b8 a, b, c, d;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+        " mov.b32 %0, {a, b, c, d};\n}"
+        : "=r"(w)
+        : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+    return w;
 }
 
 // The code toward zero of |x| <= 6, and its value.
@@ -172,8 +175,10 @@ __device__ __forceinline__ unsigned mx_pack8(const V (&x)[8], const MxScale &s, 
     }
     unsigned w = 0;
     if (rm == DRIFT_NEAREST_EVEN) {
+        float f[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) w |= (mx_rn2(mx_narrow(y[2 * j]), mx_narrow(y[2 * j + 1])) & 0xffu) << (8 * j);
+        for (int j = 0; j < 8; j++) f[j] = mx_narrow(y[j]);
+        w = mx_rn8(f);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -236,10 +241,20 @@ __device__ __forceinline__ MxFactor<typename MxSrc<TYPE>::V> mx_factor(unsigned 
     return f;
 }
 
-// Codes to nearest of two elements of a block without Inf or NaN.
-template <class V>
-__device__ __forceinline__ unsigned mx_fast2(V lo, V hi, V down) {
-    return mx_rn2(mx_narrow(lo * down), mx_narrow(hi * down)) & 0xffu;
+// Codes to nearest of eight elements of a block without Inf or NaN.
+__device__ __forceinline__ unsigned mx_fast8(const float (&x)[8], float down) {
+    const f2 k = f2_both(down);
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        f2_split(f2_mul(f2_pack(x[2 * j], x[2 * j + 1]), k), y[2 * j], y[2 * j + 1]);
+    return mx_rn8(y);
+}
+__device__ __forceinline__ unsigned mx_fast8(const double (&x)[8], double down) {
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = mx_narrow(x[j] * down);
+    return mx_rn8(y);
 }
 
 // ------------------------------------------------------------------ the cast
@@ -257,13 +272,13 @@ struct MxCast {
     int *err;
 };
 
+// `valid` elements at p, the rest zeros; `vec`: p is 16-byte aligned.
 template <int TYPE>
-__device__ __forceinline__ MxRaw8<TYPE> mx_load8(const MxCast &a, int64_t row, int64_t col,
+__device__ __forceinline__ MxRaw8<TYPE> mx_load8(bool vec, const typename MxSrc<TYPE>::T *p,
                                                  int valid) {
     using T = typename MxSrc<TYPE>::T;
-    const T *p = static_cast<const T *>(a.src) + row * a.row_stride + col;
     MxRaw8<TYPE> r;
-    if (a.vec && valid == 8) {
+    if (vec && valid == 8) {
 #pragma unroll
         for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++)
             r.w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
@@ -278,9 +293,31 @@ __device__ __forceinline__ MxRaw8<TYPE> mx_load8(const MxCast &a, int64_t row, i
     return r;
 }
 
+__device__ __forceinline__ void mx_finish(unsigned clamps, int err, unsigned long long *clamped,
+                                          int *d_err) {
+    clamps = __reduce_add_sync(0xffffffffu, clamps);
+    err = (int)__reduce_or_sync(0xffffffffu, (unsigned)err);
+    if ((threadIdx.x & 31) == 0) {
+        if (clamped && clamps) atomicAdd(clamped, (unsigned long long)clamps);
+        if (err) atomicOr(d_err, err);
+    }
+}
+
+// Everything the short way leaves: blocks with Inf or NaN, and the other roundings.
+// Out of line, since its instructions beside the short way's cost more in fetches
+// than the call.
+template <int TYPE>
+__device__ __noinline__ unsigned mx_slow8(const MxCast &a, const typename MxSrc<TYPE>::V (&x)[8],
+                                          typename MxSrc<TYPE>::V amax, int valid, uint64_t state,
+                                          uint64_t draw, uint64_t step, int &shared,
+                                          unsigned &clamps, int &err) {
+    const MxScale s = mx_scale(amax, a.headroom);
+    shared = s.shared;
+    return mx_pack8(x, s, a.rm, state, draw, step, valid, clamps, err);
+}
+
 // Eight elements of a block that four neighbouring lanes share: their codes and
-// the block's shared exponent. Blocks without Inf and NaN, to nearest, take the
-// short way; elements past the end are zeros and change nothing.
+// the block's shared exponent. Elements past the end are zeros and change nothing.
 template <int TYPE>
 __device__ __forceinline__ unsigned mx_cast8(const MxCast &a, const MxRaw8<TYPE> &r, int valid,
                                              uint64_t state, uint64_t draw, int &shared,
@@ -295,13 +332,11 @@ __device__ __forceinline__ unsigned mx_cast8(const MxCast &a, const MxRaw8<TYPE>
     if (__all_sync(0xffffffffu, key < S::kInf) && a.rm == DRIFT_NEAREST_EVEN) {
         const MxFactor<V> f = mx_factor<TYPE>(key, a.headroom);
         shared = f.shared;
-        unsigned w = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) w |= mx_fast2(x[2 * j], x[2 * j + 1], f.down) << (8 * j);
         if (a.clamped) {
 #pragma unroll
             for (int j = 0; j < 8; j++) clamps += fabs(x[j] * f.down) > (V)6;
         }
+        const unsigned w = mx_fast8(x, f.down);
         return key ? w : 0;
     }
     V amax = (V)0;
@@ -309,65 +344,65 @@ __device__ __forceinline__ unsigned mx_cast8(const MxCast &a, const MxRaw8<TYPE>
     for (int j = 0; j < 8; j++) amax = fmax(amax, mx_mag(x[j]));
     amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const MxScale s = mx_scale(amax, a.headroom);
-    shared = s.shared;
-    return mx_pack8(x, s, a.rm, state, draw, 1, valid, clamps, err);
+    // Copies, so that only this path's live in memory.
+    V y[8];
+    unsigned more = 0;
+    int sh = 0, e = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = x[j];
+    const unsigned w = mx_slow8<TYPE>(a, y, amax, valid, state, draw, 1, sh, more, e);
+    shared = sh;
+    clamps += more;
+    err |= e;
+    return w;
 }
 
-__device__ __forceinline__ void mx_finish(unsigned clamps, int err, unsigned long long *clamped,
-                                          int *d_err) {
-    clamps = __reduce_add_sync(0xffffffffu, clamps);
-    err = (int)__reduce_or_sync(0xffffffffu, (unsigned)err);
-    if ((threadIdx.x & 31) == 0) {
-        if (clamped && clamps) atomicAdd(clamped, (unsigned long long)clamps);
-        if (err) atomicOr(d_err, err);
-    }
-}
-
-// Blocks along rows: a warp takes U items at a time, each 256 elements of one
-// row (eight blocks, two tiles of scales), with all their loads in flight. Rows
-// past the end up to the tile's 128, and blocks past the row's end, get their
-// padding bytes.
+// Blocks along rows: a warp takes U chunks of 256 elements of one row (eight
+// blocks, two tiles of scales each) at a time, with all their loads in flight.
+// Rows past the end up to the tile's 128, and blocks past the row's end, get
+// their padding bytes.
 template <int TYPE, int U>
-__global__ void __launch_bounds__(256) mx4_rows_kernel(const MxCast a, uint32_t per_row,
-                                                       uint32_t items) {
+__global__ void __launch_bounds__(256) mx4_rows_kernel(const __grid_constant__ MxCast a,
+                                                       uint32_t per_row, uint32_t items) {
+    using T = typename MxSrc<TYPE>::T;
     const int lane = threadIdx.x & 31;
-    const int64_t blocks = mx4_blocks(a.cols), row_bytes = blocks * 16;
+    const int64_t blocks = mx4_blocks(a.cols);
+    const int chunks = (int)(mx4_k_tiles(a.cols) / 2);
     const uint64_t state = a.rm == DRIFT_STOCHASTIC ? *a.state : 0;
     unsigned clamps = 0;
     int err = 0;
-    const uint32_t stride = gridDim.x * 8 * U;
-    for (uint32_t it = (blockIdx.x * 8 + (threadIdx.x >> 5)) * U; it < items; it += stride) {
+    const uint32_t stride = gridDim.x * 8;
+    // A lane's block is 0 to 7 of a chunk; its scale's place in the two tiles.
+    const int place = (lane >> 4) * kMxTileBytes + (lane >> 2 & 3);
+    for (uint32_t it = blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += stride) {
+        const uint32_t row = it / per_row;
+        const int first = (int)(it - row * per_row) * U;
+        const int64_t col0 = (int64_t)first * 256 + lane * 8;
+        const bool in_row = row < a.rows;
+        const T *src = static_cast<const T *>(a.src) + row * a.row_stride + col0;
+        uint8_t *codes = a.codes + row * (blocks * 16) + col0 / 2;
+        uint8_t *scales = a.scales + mx4_scale_offset(row, 0, chunks * 2) +
+                          (int64_t)first * 2 * kMxTileBytes + place;
+        // What is left of the row from this lane's first element on.
+        const int64_t left = in_row ? a.cols - col0 : 0;
         MxRaw8<TYPE> raw[U];
-        uint32_t row[U];
-        int64_t col[U];
-        int valid[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            row[u] = (it + u) / per_row;
-            col[u] = (int64_t)(it + u - row[u] * per_row) * 256 + lane * 8;
-            valid[u] = it + u < items && row[u] < a.rows
-                           ? (int)max((int64_t)0, min((int64_t)8, a.cols - col[u])) : 0;
-            raw[u] = mx_load8<TYPE>(a, row[u], col[u], valid[u]);
+            const int valid = (int)max((int64_t)0, min((int64_t)8, left - u * 256));
+            raw[u] = mx_load8<TYPE>(a.vec, src + u * 256, valid);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            if (first + u >= chunks) break;  // the same for the whole warp
             int shared;
-            const unsigned w = mx_cast8<TYPE>(a, raw[u], valid[u], state,
-                                              (uint64_t)row[u] * a.cols + col[u], shared, clamps,
-                                              err);
-            const int64_t block = col[u] >> 5;
-            const bool in = it + u < items && row[u] < a.rows && block < blocks;
-            if (in) *reinterpret_cast<unsigned *>(a.codes + row[u] * row_bytes + col[u] / 2) = w;
-            // Lanes 0 and 16 gather the four scale bytes of their tile.
-            const unsigned byte = in ? (unsigned)(shared + 127) : 127u;
-            unsigned four = byte;
-            four |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
-            four |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
-            four |= __shfl_down_sync(0xffffffffu, byte, 12) << 24;
-            if ((lane & 15) == 0 && it + u < items)
-                *reinterpret_cast<unsigned *>(
-                    a.scales + mx4_scale_offset(row[u], block, per_row * 2)) = four;
+            const int valid = (int)max((int64_t)0, min((int64_t)8, left - u * 256));
+            const unsigned w =
+                mx_cast8<TYPE>(a, raw[u], valid, state,
+                               (uint64_t)row * a.cols + col0 + u * 256, shared, clamps, err);
+            const bool in = in_row && (col0 + u * 256) >> 5 < blocks;
+            if (in) *reinterpret_cast<unsigned *>(codes + u * 128) = w;
+            if ((lane & 3) == 0)
+                scales[u * 2 * kMxTileBytes] = in ? (uint8_t)(shared + 127) : (uint8_t)127;
         }
     }
     mx_finish(clamps, err, a.clamped, a.err);
@@ -403,35 +438,39 @@ __device__ __forceinline__ uint4 mx_cast_col(const MxCast &a, const typename MxS
         shared = f.shared;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            wp[q] = 0;
+            V y[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                wp[q] |= mx_fast2(x[q * 8 + 2 * j], x[q * 8 + 2 * j + 1], f.down) << (8 * j);
-            if (!key) wp[q] = 0;
-        }
-        if (a.clamped_t) {
+            for (int j = 0; j < 8; j++) y[j] = x[q * 8 + j];
+            if (a.clamped_t) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) clamps += fabs(x[j] * f.down) > (V)6;
+                for (int j = 0; j < 8; j++) clamps += fabs(y[j] * f.down) > (V)6;
+            }
+            wp[q] = key ? mx_fast8(y, f.down) : 0;
         }
         return w;
     }
     V amax = (V)0;
 #pragma unroll
     for (int j = 0; j < 32; j++) amax = fmax(amax, mx_mag(x[j]));
-    const MxScale s = mx_scale(amax, a.headroom);
-    shared = s.shared;
+    unsigned more = 0;
+    int sh = 0, e = 0;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         V y[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) y[j] = x[q * 8 + j];
-        wp[q] = mx_pack8(y, s, a.rm, state, draw + (uint64_t)q * 8 * a.cols, a.cols, 8, clamps, err);
+        wp[q] = mx_slow8<TYPE>(a, y, amax, 8, state, draw + (uint64_t)q * 8 * a.cols, a.cols, sh,
+                               more, e);
     }
+    shared = sh;
+    clamps += more;
+    err |= e;
     return w;
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(256) mx4_cols_kernel(const MxCast a, uint32_t row_tiles,
+__global__ void __launch_bounds__(256) mx4_cols_kernel(const __grid_constant__ MxCast a,
+                                                       uint32_t row_tiles,
                                                        uint32_t col_tiles) {
     using S = MxSrc<TYPE>;
     using T = typename S::T;
@@ -450,7 +489,8 @@ __global__ void __launch_bounds__(256) mx4_cols_kernel(const MxCast a, uint32_t 
         const int at = i * 256 + tid, r = at / kGroups, c = at % kGroups * 8;
         const int valid = r0 + r < a.rows
                               ? (int)max((int64_t)0, min((int64_t)8, a.cols - c0 - c)) : 0;
-        raw[i] = mx_load8<TYPE>(a, r0 + r, c0 + c, valid);
+        raw[i] = mx_load8<TYPE>(
+            a.vec, static_cast<const T *>(a.src) + (r0 + r) * a.row_stride + c0 + c, valid);
     }
 #pragma unroll
     for (int i = 0; i < G::kLoads; i++) {
@@ -555,15 +595,19 @@ __global__ void mx4_advance_kernel(uint64_t *state, uint64_t draws) { *state += 
 template <int TYPE>
 static int launch_cast(const MxCast &a, cudaStream_t st) {
     if (!a.codes_t) {
-        const uint32_t per_row = (uint32_t)(mx4_k_tiles(a.cols) / 2);
-        const uint32_t items = (uint32_t)(mx4_row_tiles(a.rows) * 128) * per_row;
+        const uint32_t chunks = (uint32_t)(mx4_k_tiles(a.cols) / 2);
+        const uint32_t rows = (uint32_t)(mx4_row_tiles(a.rows) * 128);
         const uint32_t sms = (uint32_t)sm_count();
-        // Four items a warp once that still leaves every SM two CTAs.
-        if (items >= sms * 2 * 8 * 4) {
-            const uint32_t grid = std::min<uint32_t>((items + 31) / 32, sms * 8);
+        // Four chunks a warp, where the rows have them, once that still leaves every
+        // SM two CTAs; else a warp a chunk.
+        if (chunks >= 4 && rows * (uint64_t)((chunks + 3) / 4) >= sms * 2 * 8) {
+            const uint32_t per_row = (chunks + 3) / 4, items = rows * per_row;
+            const uint32_t grid = std::min<uint32_t>((items + 7) / 8, sms * 8);
             mx4_rows_kernel<TYPE, 4><<<grid, 256, 0, st>>>(a, per_row, items);
         } else {
-            mx4_rows_kernel<TYPE, 1><<<(items + 7) / 8, 256, 0, st>>>(a, per_row, items);
+            const uint32_t items = rows * chunks;
+            mx4_rows_kernel<TYPE, 1><<<std::min<uint32_t>((items + 7) / 8, sms * 64), 256, 0, st>>>(
+                a, chunks, items);
         }
     } else {
         using G = MxTile<TYPE>;

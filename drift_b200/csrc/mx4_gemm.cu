@@ -10,14 +10,15 @@
 #include "epilogue.cuh"
 #include "internal.h"
 #include "mx4.cuh"
+#include "mx4_thin.cuh"
 #include "tc.cuh"
 
 namespace drift {
 
-static bool encode_codes(CUtensorMap *map, const drift_mx4 *q) {
+static bool encode_codes(CUtensorMap *map, const drift_mx4 *q, uint32_t rows) {
     const uint64_t bytes = (uint64_t)mx4_row_bytes(q->cols);
     return tc::encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q->codes, bytes, q->rows, bytes, 128,
-                         128, CU_TENSOR_MAP_SWIZZLE_128B);
+                         rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Rows of scale tiles, 256 words (two tiles) a stage; `box` rows at a time.
@@ -35,6 +36,37 @@ __global__ void __launch_bounds__(256) fill_bias_kernel(T *C, int64_t stride, in
         C[i / cols * stride + i % cols] = T(bias ? bias[i % cols] : 0.0f);
 }
 
+// How many CTAs share a thin tile's contraction: the count, up to a portable
+// cluster's eight, with the least rounds of CTAs times stages a CTA, a round
+// costing some four stages besides.
+static int thin_split(int64_t tiles, int k_stages, int sms) {
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int s = 1; s <= 8 && s <= k_stages; s++) {
+        const int64_t cost = (tiles * s + sms - 1) / sms * ((k_stages + s - 1) / s + 4);
+        if (cost < least) least = cost, best = s;
+    }
+    return best;
+}
+
+template <int NT, class T>
+static int gemm_thin(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C,
+                     int64_t c_stride, int *d_err, cudaStream_t st) {
+    thin::Args args;
+    if (!encode_codes(&args.w, b, 128) || !encode_codes(&args.x, a, NT) ||
+        !encode_scales(&args.sfw, b, 1) || !encode_scales(&args.sfx, a, 1))
+        return DRIFT_ECUDA;
+    args.rows = b->rows, args.tokens = a->rows;
+    args.w_tiles = (int)((b->rows + 127) / 128);
+    args.k_stages = (int)((a->cols + 255) / 256);
+    args.bias = bias;
+    args.c = C, args.stride = c_stride;
+    args.err = d_err;
+    const int t_tiles = (int)((a->rows + NT - 1) / NT);
+    const int split = thin_split((int64_t)args.w_tiles * t_tiles, args.k_stages, sm_count());
+    return thin::launch<NT, T>(args, t_tiles, split, st);
+}
+
 template <class T>
 static int gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C, int64_t c_stride,
                 int *d_err, cudaStream_t st) {
@@ -42,8 +74,17 @@ static int gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C,
         fill_bias_kernel<<<sm_count() * 2, 256, 0, st>>>(C, c_stride, a->rows, b->rows, bias);
         return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
     }
+    // Pair tiles that do not fill the pairs of SMs once leave the product to the
+    // thin kernel's smaller tiles and shared contractions.
+    const int64_t pairs = (a->rows + tc::kTile - 1) / tc::kTile * ((b->rows + tc::kTile - 1) / tc::kTile);
+    if (a->rows <= 128 || pairs < sm_count() / 2) {
+        if (a->rows <= 16) return gemm_thin<16>(a, b, bias, C, c_stride, d_err, st);
+        if (a->rows <= 32) return gemm_thin<32>(a, b, bias, C, c_stride, d_err, st);
+        if (a->rows <= 64) return gemm_thin<64>(a, b, bias, C, c_stride, d_err, st);
+        return gemm_thin<128>(a, b, bias, C, c_stride, d_err, st);
+    }
     tc::Args args;
-    if (!encode_codes(&args.a, a) || !encode_codes(&args.b, b) ||
+    if (!encode_codes(&args.a, a, 128) || !encode_codes(&args.b, b, 128) ||
         !encode_scales(&args.sfa, a, 1) || !encode_scales(&args.sfb, b, 2))
         return DRIFT_ECUDA;
     args.m_tiles = (int)((a->rows + tc::kTile - 1) / tc::kTile);
@@ -51,7 +92,7 @@ static int gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C,
     args.k_stages = (int)((a->cols + 255) / 256);
     args.splits = 1;
     args.err = d_err;
-    const StoreEpi<T> epi{C, c_stride, a->rows, b->rows, bias, nullptr,
+    const StoreEpi<T> epi{C, c_stride, a->rows, b->rows, bias, nullptr, 1.0f,
                           rows_aligned(C, c_stride)};
     return tc::launch<tc::KIND_MX4, false, false, false>(args, epi, sm_count(), st);
 }

@@ -14,7 +14,7 @@
 //
 // Warps: 0-7 epilogue (two per quadrant of TMEM lanes, 128 columns each), 8
 // fetches with TMA, 9 allocates TMEM and, in the pair's first CTA, issues the
-// MMAs. A stage's barrier `full` sits in the first CTA and counts both CTAs'
+// MMAs, 10 and 11 complete the control warpgroup. A stage's barrier `full` sits in the first CTA and counts both CTAs'
 // bytes; a commit of the stage's MMAs frees it in both CTAs. The accumulator
 // passes to the epilogue by `acc_full` (a commit to both) and back by
 // `acc_empty` (first CTA, one arrival an epilogue warp of either). The epilogue
@@ -22,6 +22,14 @@
 // next tile's MMAs overlap its arithmetic and stores. KIND_16 has two
 // accumulators (2 x 256 columns); KIND_MX4 has one, and 24 columns of scales a
 // stage.
+//
+// The tensor cores truncate each sum to fp32, so a long contraction drifts toward
+// zero by half a unit an MMA: 2^-17 of a logit over 4096 elements. KIND_16
+// therefore sums `run` stages (of 64 elements) in TMEM and adds those sums in
+// the epilogue's registers, rounded to nearest; the two accumulators hide it.
+// Under the power cap the reads still cost: 8 % of a long product at 8 stages a
+// run, 1 % at 32. KIND_MX4's products are small multiples of a power of two,
+// whose sums are mostly exact, and it has no room for a second accumulator.
 //
 // Every wait is bounded; one that gives up flags DEV_ERR_TIMEOUT and the
 // kernel drains and returns.
@@ -43,7 +51,12 @@ constexpr int kTile = 256;            // rows and columns of a pair's tile
 constexpr int kStageBytes = 128;      // bytes of k in a stage
 constexpr int kOperand = kRows * kStageBytes;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = (kEpiWarps + 2) * 32;
+constexpr int kThreads = (kEpiWarps + 4) * 32;  // three warpgroups
+// Registers: 384 threads launch with 168 each; the control warpgroup gives 112 a
+// thread back, from which each epilogue thread takes 56: (2 * 224 + 56) * 128 =
+// 168 * 384, exactly the launch's total.
+constexpr int kControlRegs = 56, kEpiRegs = 224;
+static_assert(2 * kEpiRegs + kControlRegs == 3 * 168, "the split must not exceed the launch's");
 constexpr int kWarpTma = kEpiWarps, kWarpMma = kEpiWarps + 1;
 constexpr int kWaitRounds = 1 << 20;
 
@@ -59,14 +72,15 @@ template <> struct Shape<KIND_16> {
 template <> struct Shape<KIND_MX4> {
     static constexpr int stage_k = 256;
     static constexpr int scales = 1024 + 2048;  // A's 128 rows, B's 256 rows
-    static constexpr int stages = 6;
+    static constexpr int stages = 5;
     static constexpr int accs = 1;
     static constexpr int sfa_col = 256, sfb_col = 256 + stages * 8;
 };
 
 template <int KIND> constexpr int stage_bytes() { return 2 * kOperand + Shape<KIND>::scales; }
+constexpr int kStaging = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes
 template <int KIND> constexpr int smem_bytes() {
-    return Shape<KIND>::stages * stage_bytes<KIND>() + 1024 + 256;
+    return Shape<KIND>::stages * stage_bytes<KIND>() + kEpiWarps * kStaging + 1024;
 }
 
 // ------------------------------------------------------------------ PTX
@@ -119,6 +133,18 @@ __device__ __forceinline__ void load_pair(unsigned dst, const CUtensorMap *map, 
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
+// Arrives on the same barrier of both CTAs once this thread's MMAs so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(smem_addr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void copy_scales(unsigned to, uint64_t from) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(from)
+                 : "memory");
+}
 // 32 columns of this warp's 32 TMEM lanes, one lane a thread.
 __device__ __forceinline__ void tmem_load32(unsigned addr, float *v) {
     unsigned *r = reinterpret_cast<unsigned *>(v);
@@ -152,6 +178,7 @@ struct Args {
     int m_tiles, n_tiles;        // pair tiles
     int k_stages;                // stages of the whole contraction
     int splits;                  // the contraction is cut into this many parts
+    int run = 1 << 30;           // KIND_16: stages summed in TMEM before registers take over
     int *err;
 };
 
@@ -218,15 +245,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const unsigned tmem = tmem_base;
     bool ok = true;
 
-    if (warp == kWarpTma) {
-        if (lane == 0) {
-            int it = 0;
+    if (warp >= kEpiWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+        if (warp == kWarpTma && lane == 0) {
+            int s = 0;
+            unsigned ph = 1;  // parity of the empty barrier to wait for
+            int loaded = 0;
             for (int t = first; t < total && ok; t += step) {
                 const Work w = work_at(args, t);
                 const int ra = w.m * kTile + (int)rank * kRows, rb = w.n * kTile + (int)rank * kRows;
-                for (int k = w.k0; k < w.k1 && ok; k++, it++) {
-                    const int s = it % S::stages, ph = it / S::stages & 1;
-                    ok = wait(&empty[s], ph ^ 1);
+                for (int k = w.k0; k < w.k1; k++) {
+                    ok = wait(&empty[s], ph);
                     if (!ok) break;
                     if (rank == 0) mbar_expect_tx(&full[s], 2 * stage_bytes<KIND>());
                     const unsigned bar = map_cta(smem_addr(&full[s]), 0);
@@ -251,118 +280,146 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             load_pair(db, &args.b, kk, rb, bar);
                         }
                     }
+                    loaded = min(loaded + 1, S::stages);
+                    if (++s == S::stages) s = 0, ph ^= 1;
                 }
             }
             // The first CTA's commits also arrive on the second's barriers: stay
-            // until those of the stages in use have.
-            for (int i = max(0, it - S::stages); i < it && ok; i++)
-                ok = wait(&empty[i % S::stages], i / S::stages & 1);
-        }
-        __syncwarp();
-    } else if (warp == kWarpMma) {
-        if (rank == 0 && lane == 0) {
+            // until the last `loaded` stages' have, in the order of their loads.
+            if (loaded < S::stages) s = 0, ph = 0;
+            for (int i = 0; i < loaded && ok; i++) {
+                ok = wait(&empty[s], ph);
+                if (++s == S::stages) s = 0, ph ^= 1;
+            }
+        } else if (warp == kWarpMma && rank == 0 && lane == 0) {
+            // This thread's instructions between two stages are the tensor cores'
+            // pauses, so its indexes run along and descriptors are a base plus a
+            // stage's offset (addresses fit their field's 14 bits of 16 bytes).
             const unsigned idesc = instr_desc<KIND>(BF16, A_MN, B_MN);
-            int it = 0, n_acc = 0;
-            for (int t = first; t < total && ok; t += step, n_acc++) {
+            // MN-major: 64 of i (o) a swizzled row, groups of eight k 1024 bytes apart,
+            // the next 64 of i half an operand further.
+            const uint64_t da0 = A_MN ? smem_desc(base, kOperand / 2, 1024, 2)
+                                      : smem_desc(base, 16, 1024, 2);
+            const uint64_t db0 = B_MN ? smem_desc(base + kOperand, kOperand / 2, 1024, 2)
+                                      : smem_desc(base + kOperand, 16, 1024, 2);
+            constexpr unsigned a_step = A_MN ? 128 : 2, b_step = B_MN ? 128 : 2;
+            int s = 0, acc = 0;
+            unsigned ph = 0, acc_ph = 1;
+            // KIND_MX4: a stage's scales go to TMEM one stage ahead of its MMAs, so that
+            // the copies run beside the stage before and not between the two.
+            bool held = false;
+            int hs = 0;
+            unsigned hd = 0, hmore = 0;
+            const auto mma_mx4 = [&]() {
+                constexpr int sfa_col = Shape<KIND_MX4>::sfa_col, sfb_col = Shape<KIND_MX4>::sfb_col;
+                const unsigned fa = tmem + sfa_col + hs * 8, fb = tmem + sfb_col + hs * 16;
+                const unsigned off = hs * (stage_bytes<KIND>() >> 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    // 64 elements: two scales of a 32-bit column's four.
+                    const unsigned id = (j & 1) * 2;
+                    asm volatile(
+                        "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
+                        " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
+                        " [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(hd),
+                        "l"(da0 + off + j * 2), "l"(db0 + off + j * 2),
+                        "r"(idesc | id << 4 | id << 29), "r"(fa + (j >> 1) * 4),
+                        "r"(fb + (j >> 1) * 8), "r"(j > 0 ? 1u : hmore)
+                        : "memory");
+                }
+                commit_pair(&empty[hs]);
+                held = false;
+            };
+            for (int t = first; t < total && ok; t += step) {
                 const Work w = work_at(args, t);
-                const int acc = n_acc % S::accs;
-                ok = wait(&acc_empty[acc], (n_acc / S::accs & 1) ^ 1);
-                if (!ok) break;
-                fence_after();
-                const unsigned d = tmem + acc * kTile;
-                for (int k = w.k0; k < w.k1; k++, it++) {
-                    const int s = it % S::stages, ph = it / S::stages & 1;
+                int left = KIND == KIND_16 ? args.run : 1 << 30;  // stages until this sum ends
+                unsigned more = 0;
+                for (int k = w.k0; k < w.k1; k++) {
                     ok = wait(&full[s], ph);
                     if (!ok) break;
                     fence_after();
-                    const unsigned sa = base + s * stage_bytes<KIND>(), sb = sa + kOperand;
+                    const unsigned off = s * (stage_bytes<KIND>() >> 4);
                     if (KIND == KIND_MX4) {
-                        constexpr int sfa_col = Shape<KIND_MX4>::sfa_col;
-                        constexpr int sfb_col = Shape<KIND_MX4>::sfb_col;
-                        const unsigned fa = tmem + sfa_col + s * 8, fb = tmem + sfb_col + s * 16;
-                        const unsigned ssa = sb + kOperand, ssb = ssa + 1024;
-                        // A tile of scales: 32 lanes of 16 bytes, to all four lane quadrants.
+                        const unsigned fa = tmem + Shape<KIND_MX4>::sfa_col + s * 8;
+                        const unsigned fb = tmem + Shape<KIND_MX4>::sfb_col + s * 16;
+                        // Tiles of scales: 32 lanes of 16 bytes, to all four lane quadrants.
+                        const uint64_t sc = smem_desc(base + 2 * kOperand, 0, 128, 0) + off;
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const unsigned to[3] = {fa + h * 4, fb + h * 8, fb + h * 8 + 4};
-                            const unsigned from[3] = {ssa + h * 512, ssb + h * 512,
-                                                      ssb + 1024 + h * 512};
-#pragma unroll
-                            for (int j = 0; j < 3; j++)
-                                asm volatile(
-                                    "tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(to[j]),
-                                    "l"(smem_desc(from[j], 0, 128, 0))
-                                    : "memory");
+                            copy_scales(fa + h * 4, sc + h * 32);
+                            copy_scales(fb + h * 8, sc + 64 + h * 32);
+                            copy_scales(fb + h * 8 + 4, sc + 128 + h * 32);
                         }
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            // 64 elements: two scales of a 32-bit column's four.
-                            const unsigned id = (j & 1) * 2;
-                            const unsigned more = k > w.k0 || j > 0;
-                            asm volatile(
-                                "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
-                                " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
-                                " [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-                                "l"(smem_desc(sa + j * 32, 16, 1024, 2)),
-                                "l"(smem_desc(sb + j * 32, 16, 1024, 2)),
-                                "r"(idesc | id << 4 | id << 29), "r"(fa + (j >> 1) * 4),
-                                "r"(fb + (j >> 1) * 8), "r"(more)
-                                : "memory");
-                        }
+                        if (held) mma_mx4();
+                    }
+                    if (more == 0) {
+                        // A sum begins: its accumulator must have been read.
+                        ok = wait(&acc_empty[acc], acc_ph);
+                        if (!ok) break;
+                        fence_after();
+                    }
+                    const unsigned d = tmem + acc * kTile;
+                    if (KIND == KIND_MX4) {
+                        held = true, hs = s, hd = d, hmore = more;
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            // MN-major: 64 of i (o) a swizzled row, groups of eight k 1024
-                            // bytes apart, the next 64 of i half an operand further.
-                            const uint64_t da =
-                                A_MN ? smem_desc(sa + j * 2048, kOperand / 2, 1024, 2)
-                                     : smem_desc(sa + j * 32, 16, 1024, 2);
-                            const uint64_t db =
-                                B_MN ? smem_desc(sb + j * 2048, kOperand / 2, 1024, 2)
-                                     : smem_desc(sb + j * 32, 16, 1024, 2);
-                            const unsigned more = k > w.k0 || j > 0;
+                        for (int j = 0; j < 4; j++)
                             asm volatile(
                                 "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
                                 " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-                                "l"(da), "l"(db), "r"(idesc), "r"(more)
+                                "l"(da0 + off + j * a_step), "l"(db0 + off + j * b_step),
+                                "r"(idesc), "r"(j > 0 ? 1u : more)
                                 : "memory");
-                        }
+                        commit_pair(&empty[s]);
                     }
-                    asm volatile(
-                        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster"
-                        ".multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(&empty[s])),
-                        "h"((uint16_t)3)
-                        : "memory");
+                    more = 1;
+                    if (++s == S::stages) s = 0, ph ^= 1;
+                    if (--left == 0 || k == w.k1 - 1) {
+                        if (KIND == KIND_MX4) mma_mx4();
+                        commit_pair(&acc_full[acc]);
+                        if (++acc == S::accs) acc = 0, acc_ph ^= 1;
+                        left = KIND == KIND_16 ? args.run : 1 << 30;
+                        more = 0;
+                    }
                 }
-                if (!ok) break;
-                asm volatile(
-                    "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster"
-                    ".multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(&acc_full[acc])),
-                    "h"((uint16_t)3)
-                    : "memory");
             }
         }
-        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
         const int quad = warp & 3, half = warp >> 2;
+        const unsigned staging = base + S::stages * stage_bytes<KIND>() + warp * kStaging;
         int n_acc = 0;
-        for (int t = first; t < total; t += step, n_acc++) {
+        for (int t = first; t < total && ok; t += step) {
             const Work w = work_at(args, t);
-            const int acc = n_acc % S::accs;
-            ok = wait(&acc_full[acc], n_acc / S::accs & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            fence_after();
             float v[128];
-            const unsigned at = tmem + acc * kTile + half * 128 + ((unsigned)(quad * 32) << 16);
+            const int run = KIND == KIND_16 ? min(args.run, w.k1 - w.k0) : w.k1 - w.k0;
+            for (int k = w.k0; k < w.k1; k += run, n_acc++) {
+                const int acc = n_acc % S::accs;
+                ok = __all_sync(0xffffffffu, wait(&acc_full[acc], n_acc / S::accs & 1));
+                if (!ok) break;
+                fence_after();
+                const unsigned at = tmem + acc * kTile + half * 128 + ((unsigned)(quad * 32) << 16);
+                if (S::accs == 1 || k == w.k0) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) tmem_load32(at + c * 32, v + c * 32);
-            tmem_wait_load();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_cluster(map_cta(smem_addr(&acc_empty[acc]), 0));
-            const int64_t row = (int64_t)w.m * kTile + (int)rank * kRows + quad * 32 + lane;
-            epi.run(v, row, (int64_t)w.n * kTile + half * 128, w, lane);
+                    for (int c = 0; c < 4; c++) tmem_load32(at + c * 32, v + c * 32);
+                    tmem_wait_load();
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        float x[32];
+                        tmem_load32(at + c * 32, x);
+                        tmem_wait_load();
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[c * 32 + j] += x[j];
+                    }
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_cluster(map_cta(smem_addr(&acc_empty[acc]), 0));
+            }
+            if (!ok) break;
+            const int64_t row0 = (int64_t)w.m * kTile + (int)rank * kRows + quad * 32;
+            epi.run(v, row0, (int64_t)w.n * kTile + half * 128, w, lane, staging);
         }
     }
 

@@ -17,9 +17,9 @@
 //             unit of that type, as the results' own), then dx += d W and
 //             dW = d^T x from it, reading d and W where they lie (MN-major).
 //
-// fp16 holds d times a power of two that brings the largest |g| near 2^15, so
-// that small probabilities keep their bits; the products undo it exactly. bf16
-// has fp32's range and needs none.
+// fp16 holds d times a power of two (2^15, or with weights by row one that brings
+// the largest |g| near 2^15), so that small probabilities keep their bits; the
+// products undo it exactly. bf16 has fp32's range and needs none.
 //
 // Bound: the tensor cores for many tokens (8 T D V operations with the
 // gradient's second computation of the logits, against 6 T D V if they were
@@ -31,6 +31,11 @@
 #include "tc.cuh"
 
 namespace drift {
+
+// Stages of 64 summed in TMEM, whose sums truncate: 2^-18 of a logit's magnitude at
+// most over 16, which moves an fp32 loss by a few units; the gradients' products
+// round to 16 bits, so theirs may be longer.
+constexpr int kLogitRun = 16, kGradRun = 64;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -102,9 +107,10 @@ struct StatsEpi {
     const float *bias;  // of the piece's first column
     int64_t rows, cols, v0;
     XentRows x;
-    __device__ __forceinline__ void run(float (&v)[128], int64_t row, int64_t col, const tc::Work &,
-                                        int) const {
+    __device__ __forceinline__ void run(float (&v)[128], int64_t row0, int64_t col, const tc::Work &,
+                                        int lane, unsigned) const {
         if (col >= cols) return;
+        const int64_t row = row0 + lane;
         finish_logits(v, col, cols, bias);
         float m[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
@@ -138,17 +144,18 @@ template <class T, bool DB> struct GradEpi {
     const float *bias;
     int64_t rows, cols, v0;
     XentRows x;
-    const float *lse, *g;
-    int64_t g_stride;
-    const float *scale;  // fp16: the power of two that d is held times, or null
-    float *sums;         // DB: [row / 32][column]
-    __device__ __forceinline__ void run(float (&v)[128], int64_t row, int64_t col, const tc::Work &,
-                                        int lane) const {
+    const float *lse, *g;  // g: null for 1 throughout
+    const float *scale;    // the power of two that d is held times: device, or null
+    float fixed;           // and the host's
+    float *sums;           // DB: [row / 32][column], not scaled
+    __device__ __forceinline__ void run(float (&v)[128], int64_t row0, int64_t col, const tc::Work &,
+                                        int lane, unsigned staging) const {
         if (col >= cols) return;
+        const int64_t row = row0 + lane;
         finish_logits(v, col, cols, bias);
         bool bad = false;
         const int64_t t = row < rows ? x.at(row, bad) : -1;
-        const float gi = t >= 0 ? g[row * g_stride] : 0.0f;
+        const float gi = t >= 0 ? (g ? g[row] : 1.0f) : 0.0f;
         const float z = t >= 0 ? lse[row] : 0.0f;
         const int64_t at = t - v0 - col;
 #pragma unroll
@@ -177,16 +184,16 @@ template <class T, bool DB> struct GradEpi {
                 if (col + c + lane < cols) sums[(row >> 5) * cols + col + c + lane] = a[0];
             }
         }
-        if (row >= rows) return;
-        if (scale) {
-            const float f = *scale;
+        const float f = scale ? *scale : fixed;
+        if (f != 1.0f) {
 #pragma unroll
             for (int j = 0; j < 128; j++) v[j] *= f;
         }
-        T *p = d + row * ld + col;
-#pragma unroll
-        for (int j = 0; j < 128; j += 8)
-            if (col + j < ld) store8(p + j, v + j, 8, true);  // padding columns get zeros
+        T *p = d + row0 * ld + col;
+        by_rows<T>(v, staging, lane, [&](int r, int j, uint4 w) {
+            if (row0 + r < rows && col + j < ld)  // padding columns get zeros
+                *reinterpret_cast<uint4 *>(p + r * ld + j) = w;
+        });
     }
 };
 
@@ -274,7 +281,8 @@ __global__ void __launch_bounds__(1024) xent_scale_kernel(const float *g, int64_
 
 // db of a piece from the sums of groups of 32 rows, in order.
 __global__ void __launch_bounds__(256) xent_colsum_kernel(const float *sums, int64_t groups,
-                                                          int64_t n, float *db) {
+                                                          int64_t n, const float *alpha,
+                                                          float *db) {
     __shared__ float sh[8][33];
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
     const int64_t v = (int64_t)blockIdx.x * 32 + lane;
@@ -287,7 +295,7 @@ __global__ void __launch_bounds__(256) xent_colsum_kernel(const float *sums, int
     __syncthreads();
     if (slice || v >= n) return;
     for (int i = 1; i < 8; i++) s += sh[i][lane];
-    db[v] = s;
+    db[v] = alpha ? s * *alpha : s;
 }
 
 // Sums the parts of dx and rounds to its type.
@@ -295,8 +303,8 @@ template <class T>
 __global__ void __launch_bounds__(256) xent_dx_kernel(const float *acc, int splits, int64_t part,
                                                       int64_t ld, T *dx, int64_t rows,
                                                       int64_t cols, int64_t stride,
-                                                      const float *alpha) {
-    const float f = alpha ? *alpha : 1.0f;
+                                                      const float *alpha, float beta) {
+    const float f = alpha ? *alpha * beta : beta;
     const int64_t groups = (cols + 3) / 4;
     for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < rows * groups; i += 256LL * gridDim.x) {
         const int64_t r = i / groups, c = (i - r * groups) * 4;
@@ -385,6 +393,7 @@ static bool logit_args(tc::Args &a, const drift_xent *op, int64_t v0, int64_t n,
     a.n_tiles = tiles(n);
     a.k_stages = stages(op->depth);
     a.splits = 1;
+    a.run = kLogitRun;
     a.err = err;
     return tc::encode_16(&a.a, bf16, op->x, op->tokens, op->depth, op->x_stride, true) &&
            tc::encode_16(&a.b, bf16, w, n, op->depth, op->w_stride, true);
@@ -429,9 +438,16 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
     T *d = reinterpret_cast<T *>(ws + p.d);
     float *sums = reinterpret_cast<float *>(ws + p.sums);
     float *acc = reinterpret_cast<float *>(ws + p.acc);
-    float *scale = BF16 ? nullptr : reinterpret_cast<float *>(ws + p.scale);
-    if (scale) xent_scale_kernel<<<1, 1024, 0, st>>>(g, g_stride ? n_t : 1, scale);
-    const float *undo = scale ? scale + 1 : nullptr;
+    // One weight for all rows multiplies the results, and d is the plain p - [v = t]:
+    // its large entries lie just below 1, where the type's steps are finest for their
+    // size. Weights by row go into d.
+    const bool one = g_stride == 0;
+    float *scale = BF16 || one ? nullptr : reinterpret_cast<float *>(ws + p.scale);
+    if (scale) xent_scale_kernel<<<1, 1024, 0, st>>>(g, n_t, scale);
+    const float fixed = !BF16 && one ? 32768.0f : 1.0f;
+    const float *undo = one ? g : scale ? scale + 1 : nullptr, *sum_undo = one ? g : nullptr;
+    const float beta = 1.0f / fixed;
+    const float *row_g = one ? nullptr : g;
     for (int64_t v0 = 0; v0 < op->vocab; v0 += p.piece) {
         const int64_t n = std::min(p.piece, op->vocab - v0);
         tc::Args a;
@@ -439,15 +455,15 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
         const float *bias = op->bias ? op->bias + v0 : nullptr;
         int rc;
         if (db) {
-            const GradEpi<T, true> epi{d,   p.ld, bias, n_t,      n,     v0,  rows,
-                                       lse, g,    g_stride, scale, sums};
+            const GradEpi<T, true> epi{d,   p.ld,  bias,  n_t,   n,   v0, rows,
+                                       lse, row_g, scale, fixed, sums};
             rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
             if (!rc)
                 xent_colsum_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>(
-                    sums, (n_t + 31) / 32, n, db + v0);
+                    sums, (n_t + 31) / 32, n, sum_undo, db + v0);
         } else {
-            const GradEpi<T, false> epi{d,   p.ld, bias, n_t,      n,     v0,  rows,
-                                        lse, g,    g_stride, scale, nullptr};
+            const GradEpi<T, false> epi{d,   p.ld,  bias,  n_t,   n,      v0, rows,
+                                        lse, row_g, scale, fixed, nullptr};
             rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
         }
         if (rc) return rc;
@@ -458,9 +474,10 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
                 !tc::encode_16(&a.b, BF16, w, dep, n, op->w_stride, false))
                 return DRIFT_ECUDA;
             a.m_tiles = tiles(n_t), a.n_tiles = tiles(dep), a.k_stages = stages(n);
+            a.run = kGradRun;
             a.splits = std::min(p.splits, a.k_stages);
             if (p.direct) {
-                const StoreEpi<T> epi{dx, dx_stride, n_t, dep, nullptr, undo,
+                const StoreEpi<T> epi{dx, dx_stride, n_t, dep, nullptr, undo, beta,
                                       rows_aligned(dx, dx_stride)};
                 rc = tc::launch<tc::KIND_16, BF16, false, true>(a, epi, sm_count(), st);
             } else {
@@ -475,16 +492,17 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
                 !tc::encode_16(&a.b, BF16, op->x, dep, n_t, op->x_stride, false))
                 return DRIFT_ECUDA;
             a.m_tiles = tiles(n), a.n_tiles = tiles(dep), a.k_stages = stages(n_t);
-            a.splits = 1;
+            a.splits = 1, a.run = kGradRun;
             T *to = dw + v0 * dw_stride;
-            const StoreEpi<T> epi{to, dw_stride, n, dep, nullptr, undo, rows_aligned(to, dw_stride)};
+            const StoreEpi<T> epi{to,      dw_stride, n,    dep,
+                                  nullptr, undo,      beta, rows_aligned(to, dw_stride)};
             rc = tc::launch<tc::KIND_16, BF16, true, true>(a, epi, sm_count(), st);
             if (rc) return rc;
         }
     }
     if (dx && !p.direct)
         xent_dx_kernel<<<sm_count() * 8, 256, 0, st>>>(acc, p.splits, p.part, p.acc_ld, dx, n_t, dep,
-                                                       dx_stride, undo);
+                                                       dx_stride, undo, beta);
     return done();
 }
 
