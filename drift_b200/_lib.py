@@ -147,6 +147,8 @@ SIGNATURES = {
     "drift_linear_xent_dev": (_int, [_vp, _P(DriftXent), _vp, _vp, _vp, _vp, _i64, _vp]),
     "drift_linear_xent_grad_dev": (_int, [_vp, _P(DriftXent), _vp, _vp, _i64, _vp, _i64, _vp, _i64,
                                           _vp, _vp, _i64, _vp]),
+    "drift_linear_xent_mean_dev": (_int, [_vp, _P(DriftXent), _vp, _vp, _i64, _vp, _i64, _vp, _vp,
+                                          _i64, _vp]),
     "drift_adamw_dev": (_int, [_vp, _P(DriftAdamW), _P(DriftAdamWTensor), _i64, _vp, _vp, _vp, _vp,
                                _vp, _vp]),
     "drift_probe_fp64": (_int, [_vp, _P(_d)]),

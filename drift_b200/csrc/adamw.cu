@@ -27,6 +27,7 @@
 #include "common.cuh"
 #include "internal.h"
 #include "pairs.cuh"
+#include "pdl.cuh"
 
 namespace drift {
 
@@ -63,6 +64,8 @@ struct AdamArgs {
 __global__ void adamw_prepare_kernel(int64_t *step, double b1, double b2, double lr,
                                      const float *d_lr, double wd, float *scal, uint64_t *rng,
                                      uint64_t draws, uint64_t *rng_used) {
+    pdl_trigger();
+    pdl_wait();
     const int64_t t = *step + 1;
     *step = t;
     if (d_lr) lr = (double)*d_lr;
@@ -361,6 +364,8 @@ __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block,
 
 template <bool EIGHT, bool SR>
 __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamArgs a) {
+    pdl_trigger();
+    pdl_wait();
     // The last tensor whose first chunk is not above this one.
     int lo = 0, hi = a.count - 1;
     while (lo < hi) {
@@ -413,9 +418,9 @@ int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_
         blocks += (tensors[i].n + kAdamBlock - 1) / kAdamBlock;
     }
     uint64_t *rng_used = reinterpret_cast<uint64_t *>(d_scalars + 4);
-    adamw_prepare_kernel<<<1, 1, 0, st>>>(d_step, h->beta1, h->beta2, h->lr, d_lr,
-                                          h->weight_decay, d_scalars, sr ? d_rng : nullptr, draws,
-                                          rng_used);
+    int rc = launch_pdl(adamw_prepare_kernel, dim3(1), 1, 0, st, 0, d_step, h->beta1, h->beta2,
+                        h->lr, d_lr, h->weight_decay, d_scalars, sr ? d_rng : nullptr, draws,
+                        rng_used);
     AdamArgs a;
     a.b1 = (float)h->beta1;
     a.b2 = (float)h->beta2;
@@ -437,10 +442,10 @@ int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_
     auto flush = [&]() {
         if (a.count == 0) return;
         a.first[a.count] = (uint32_t)chunks;
-        const unsigned grid = (unsigned)chunks;
-        if (!eight) adamw_kernel<false, false><<<grid, kAdamThreads, 0, st>>>(a);
-        else if (!sr) adamw_kernel<true, false><<<grid, kAdamThreads, 0, st>>>(a);
-        else adamw_kernel<true, true><<<grid, kAdamThreads, 0, st>>>(a);
+        const auto kernel = !eight ? adamw_kernel<false, false>
+                            : !sr  ? adamw_kernel<true, false>
+                                   : adamw_kernel<true, true>;
+        if (!rc) rc = launch_pdl(kernel, dim3((unsigned)chunks), kAdamThreads, 0, st, 0, a);
         a.count = 0;
         chunks = 0;
     };
@@ -463,7 +468,7 @@ int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_
         drawn += (uint64_t)t.n;
     }
     flush();
-    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+    return rc;
 }
 
 }  // namespace drift

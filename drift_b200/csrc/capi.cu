@@ -1283,10 +1283,10 @@ static int check_xent(const drift_xent *op) {
     return DRIFT_OK;
 }
 
-int drift_linear_xent_workspace(const drift_xent *op, int grad, int64_t *bytes) {
-    if (!op || !bytes || op->tokens < 0 || op->depth < 1 || op->vocab < 1)
+int drift_linear_xent_workspace(const drift_xent *op, int mode, int64_t *bytes) {
+    if (!op || !bytes || mode < 0 || mode > 2 || op->tokens < 0 || op->depth < 1 || op->vocab < 1)
         return fail(DRIFT_EINVAL, "bad shape");
-    *bytes = xent_workspace(op, grad != 0);
+    *bytes = xent_workspace(op, mode);
     return DRIFT_OK;
 }
 
@@ -1297,7 +1297,7 @@ int drift_linear_xent_dev(drift_ctx *ctx, const drift_xent *op, float *d_loss, f
     int rc = check_xent(op);
     if (rc) return rc;
     if (op->tokens && !d_lse) return fail(DRIFT_EINVAL, "null pointer");
-    if (!d_ws || ws_bytes < xent_workspace(op, false) || misaligned(d_ws, 256))
+    if (!d_ws || ws_bytes < xent_workspace(op, 0) || misaligned(d_ws, 256))
         return fail(DRIFT_EINVAL, "workspace too small or misaligned");
     rc = launch_xent(op, d_loss, d_lse, d_mean, d_ws, ctx->d_err(), pick(ctx, stream));
     return rc ? fail(rc, "linear cross entropy launch") : DRIFT_OK;
@@ -1315,11 +1315,27 @@ int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, const float
         return fail(DRIFT_EINVAL, "bad arguments");
     if ((d_dx && dx_stride < op->depth) || (d_dw && dw_stride < op->depth))
         return fail(DRIFT_EINVAL, "bad stride");
-    if (!d_ws || ws_bytes < xent_workspace(op, true) || misaligned(d_ws, 256))
+    if (!d_ws || ws_bytes < xent_workspace(op, 1) || misaligned(d_ws, 256))
         return fail(DRIFT_EINVAL, "workspace too small or misaligned");
     rc = launch_xent_grad(op, d_lse, d_dloss, dloss_stride, d_dx, dx_stride, d_dw, dw_stride,
                           d_db, d_ws, ctx->d_err(), pick(ctx, stream));
     return rc ? fail(rc, "linear cross entropy gradient launch") : DRIFT_OK;
+}
+
+int drift_linear_xent_mean_dev(drift_ctx *ctx, const drift_xent *op, float *d_mean, void *d_dx,
+                               int64_t dx_stride, void *d_dw, int64_t dw_stride, float *d_db,
+                               void *d_ws, int64_t ws_bytes, void *stream) {
+    DeviceScope scope(ctx);
+    if (scope.status) return scope.status;
+    int rc = check_xent(op);
+    if (rc) return rc;
+    if (!d_mean || (d_dx && dx_stride < op->depth) || (d_dw && dw_stride < op->depth))
+        return fail(DRIFT_EINVAL, "bad arguments");
+    if (!d_ws || ws_bytes < xent_workspace(op, 2) || misaligned(d_ws, 256))
+        return fail(DRIFT_EINVAL, "workspace too small or misaligned");
+    rc = launch_xent_mean(op, d_mean, d_dx, dx_stride, d_dw, dw_stride, d_db, d_ws, ctx->d_err(),
+                          pick(ctx, stream));
+    return rc ? fail(rc, "linear cross entropy launch") : DRIFT_OK;
 }
 
 int drift_adamw_dev(drift_ctx *ctx, const drift_adamw *h, const drift_adamw_tensor *tensors,

@@ -160,7 +160,10 @@ int launch_mx4_dequantize(const drift_mx4 *q, int type, void *dst, int64_t strid
 int launch_mx4_gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, int type, void *C,
                     int64_t c_stride, int *d_err, cudaStream_t st);
 // xent.cu
-int64_t xent_workspace(const drift_xent *op, bool grad);
+// mode 0: the loss, 1: its gradient, 2: the mean loss with its gradients.
+int64_t xent_workspace(const drift_xent *op, int mode);
+int launch_xent_mean(const drift_xent *op, float *mean, void *dx, int64_t dx_stride, void *dw,
+                     int64_t dw_stride, float *db, void *ws, int *err, cudaStream_t st);
 int launch_xent(const drift_xent *op, float *loss, float *lse, float *mean, void *ws, int *err,
                 cudaStream_t st);
 int launch_xent_grad(const drift_xent *op, const float *lse, const float *g, int64_t g_stride,

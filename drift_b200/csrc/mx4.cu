@@ -14,6 +14,7 @@
 // of 128 x 64 in shared memory; where both directions are wanted they read the
 // same tile, so the source is read once.
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -22,6 +23,7 @@
 #include "internal.h"
 #include "mx4.cuh"
 #include "pairs.cuh"
+#include "pdl.cuh"
 
 namespace drift {
 
@@ -365,6 +367,8 @@ template <int TYPE, int U>
 __global__ void __launch_bounds__(256) mx4_rows_kernel(const __grid_constant__ MxCast a,
                                                        uint32_t per_row, uint32_t items) {
     using T = typename MxSrc<TYPE>::T;
+    pdl_trigger();
+    pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t blocks = mx4_blocks(a.cols);
     const int chunks = (int)(mx4_k_tiles(a.cols) / 2);
@@ -477,6 +481,8 @@ __global__ void __launch_bounds__(256) mx4_cols_kernel(const __grid_constant__ M
     using V = typename S::V;
     using G = MxTile<TYPE>;
     extern __shared__ __align__(16) unsigned char mx_smem[];
+    pdl_trigger();
+    pdl_wait();
     const uint32_t tile_r = blockIdx.x / col_tiles, tile_c = blockIdx.x - tile_r * col_tiles;
     const int64_t r0 = (int64_t)tile_r * kMxTr, c0 = (int64_t)tile_c * G::kCols;
     const int tid = threadIdx.x, lane = tid & 31;
@@ -590,7 +596,11 @@ __global__ void __launch_bounds__(256) mx4_cols_kernel(const __grid_constant__ M
     }
 }
 
-__global__ void mx4_advance_kernel(uint64_t *state, uint64_t draws) { *state += draws * kGolden; }
+__global__ void mx4_advance_kernel(uint64_t *state, uint64_t draws) {
+    pdl_trigger();
+    pdl_wait();
+    *state += draws * kGolden;
+}
 
 template <int TYPE>
 static int launch_cast(const MxCast &a, cudaStream_t st) {
@@ -603,26 +613,23 @@ static int launch_cast(const MxCast &a, cudaStream_t st) {
         if (chunks >= 4 && rows * (uint64_t)((chunks + 3) / 4) >= sms * 2 * 8) {
             const uint32_t per_row = (chunks + 3) / 4, items = rows * per_row;
             const uint32_t grid = std::min<uint32_t>((items + 7) / 8, sms * 8);
-            mx4_rows_kernel<TYPE, 4><<<grid, 256, 0, st>>>(a, per_row, items);
+            return launch_pdl(mx4_rows_kernel<TYPE, 4>, dim3(grid), 256, 0, st, 0, a, per_row, items);
         } else {
             const uint32_t items = rows * chunks;
-            mx4_rows_kernel<TYPE, 1><<<std::min<uint32_t>((items + 7) / 8, sms * 64), 256, 0, st>>>(
-                a, chunks, items);
+            return launch_pdl(mx4_rows_kernel<TYPE, 1>,
+                              dim3(std::min<uint32_t>((items + 7) / 8, sms * 64)), 256, 0, st, 0,
+                              a, chunks, items);
         }
     } else {
         using G = MxTile<TYPE>;
-        if (G::kSmem > 48 * 1024 &&
-            cudaFuncSetAttribute(mx4_cols_kernel<TYPE>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 G::kSmem) != cudaSuccess)
-            return DRIFT_ECUDA;
+        static unsigned long long done = 0;
+        if (!allow_smem(mx4_cols_kernel<TYPE>, G::kSmem, done)) return DRIFT_ECUDA;
         // Columns up to the tile's 128, so that every padding byte is written.
         const uint32_t row_tiles = (uint32_t)mx4_row_tiles(a.rows);
         const uint32_t col_tiles = (uint32_t)mx4_row_tiles(a.cols) * (128 / G::kCols);
-        mx4_cols_kernel<TYPE><<<row_tiles * col_tiles, 256, G::kSmem, st>>>(a, row_tiles,
-                                                                           col_tiles);
+        return launch_pdl(mx4_cols_kernel<TYPE>, dim3(row_tiles * col_tiles), 256, G::kSmem, st, 0,
+                          a, row_tiles, col_tiles);
     }
-    return DRIFT_OK;
 }
 
 int launch_mx4_quantize(int headroom, int rm, int type, const void *src, int64_t rows,
@@ -650,9 +657,9 @@ int launch_mx4_quantize(int headroom, int rm, int type, const void *src, int64_t
     }
     if (rc) return rc;
     if (rm == DRIFT_STOCHASTIC)
-        mx4_advance_kernel<<<1, 1, 0, st>>>(
-            d_state, (uint64_t)rows * cols * ((codes != nullptr) + (codes_t != nullptr)));
-    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+        return launch_pdl(mx4_advance_kernel, dim3(1), 1, 0, st, 0, d_state,
+                          (uint64_t)rows * cols * ((codes != nullptr) + (codes_t != nullptr)));
+    return DRIFT_OK;
 }
 
 // ------------------------------------------------------------------ back to values
@@ -673,6 +680,8 @@ __global__ void __launch_bounds__(256) mx4_values_kernel(const uint8_t *codes,
                                                          const uint8_t *scales, int64_t rows,
                                                          int64_t cols, T *dst, int64_t stride,
                                                          uint32_t groups, bool vec) {
+    pdl_trigger();
+    pdl_wait();
     const int64_t row_bytes = mx4_row_bytes(cols), k_tiles = mx4_k_tiles(cols);
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         for (uint32_t g = blockIdx.x * 256 + threadIdx.x; g < groups; g += gridDim.x * 256) {
@@ -714,24 +723,16 @@ int launch_mx4_dequantize(const drift_mx4 *q, int type, void *dst, int64_t strid
     const bool vec =
         reinterpret_cast<uintptr_t>(dst) % 16 == 0 && stride * size[type] % 16 == 0;
     const dim3 grid((groups + 255) / 256, (unsigned)std::min<int64_t>(q->rows, 65535));
+    const auto run = [&](auto *p) {
+        return launch_pdl(mx4_values_kernel<std::remove_pointer_t<decltype(p)>>, grid, 256, 0, st, 0,
+                          q->codes, q->scales, q->rows, q->cols, p, stride, groups, vec);
+    };
     switch (type) {
-        case DRIFT_T_F64:
-            mx4_values_kernel<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols,
-                                                    (double *)dst, stride, groups, vec);
-            break;
-        case DRIFT_T_F32:
-            mx4_values_kernel<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols,
-                                                    (float *)dst, stride, groups, vec);
-            break;
-        case DRIFT_T_BF16:
-            mx4_values_kernel<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols,
-                                                    (__nv_bfloat16 *)dst, stride, groups, vec);
-            break;
-        default:
-            mx4_values_kernel<<<grid, 256, 0, st>>>(q->codes, q->scales, q->rows, q->cols,
-                                                    (__half *)dst, stride, groups, vec);
+        case DRIFT_T_F64: return run((double *)dst);
+        case DRIFT_T_F32: return run((float *)dst);
+        case DRIFT_T_BF16: return run((__nv_bfloat16 *)dst);
+        default: return run((__half *)dst);
     }
-    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
 }
 
 }  // namespace drift

@@ -61,6 +61,7 @@ static int gemm_thin(const drift_mx4 *a, const drift_mx4 *b, const float *bias, 
     args.k_stages = (int)((a->cols + 255) / 256);
     args.bias = bias;
     args.c = C, args.stride = c_stride;
+    args.vec = rows_aligned(C, c_stride);
     args.err = d_err;
     const int t_tiles = (int)((a->rows + NT - 1) / NT);
     const int split = thin_split((int64_t)args.w_tiles * t_tiles, args.k_stages, sm_count());

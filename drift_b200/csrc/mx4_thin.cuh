@@ -34,6 +34,7 @@ struct Args {
     const float *bias;           // per weight row
     void *c;
     int64_t stride;
+    bool vec;                    // rows of c start 16-byte aligned
     int *err;
 };
 
@@ -56,10 +57,24 @@ __device__ __forceinline__ void copy_scales(unsigned to, uint64_t from) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(from)
                  : "memory");
 }
-__device__ __forceinline__ float load_cluster(unsigned addr) {
-    float f;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 load_cluster(unsigned addr) {
+    float4 f;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                 : "r"(addr)
+                 : "memory");
     return f;
+}
+// Four values, the address aligned to them.
+template <class T> __device__ __forceinline__ void store4(T *p, const float (&y)[4]) {
+    if constexpr (sizeof(T) == 8) {
+        reinterpret_cast<double2 *>(p)[0] = make_double2(y[0], y[1]);
+        reinterpret_cast<double2 *>(p)[1] = make_double2(y[2], y[3]);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(p) = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+    }
 }
 
 template <int NT, class T>
@@ -95,6 +110,8 @@ __global__ void __launch_bounds__(kThreads, 1) thin_kernel(const __grid_constant
     tc::fence_after();
     const unsigned tmem = tmem_base;
     bool ok = true;
+    pdl_trigger();
+    pdl_wait();
 
     if (warp == 4) {
         if (lane == 0) {
@@ -208,24 +225,46 @@ __global__ void __launch_bounds__(kThreads, 1) thin_kernel(const __grid_constant
     __syncthreads();
     if (ranks > 1) {
         tc::cluster_sync();
-        if (threadIdx.x < 128) {
-            const int64_t r = (int64_t)tw * 128 + threadIdx.x;
-            const float b = args.bias && r < args.rows ? __ldg(args.bias + r) : 0.0f;
-            const int t0 = NT * rank / ranks, t1 = NT * (rank + 1) / ranks;
-            for (int t = t0; t < t1; t++) {
-                const int64_t token = (int64_t)tt * NT + t;
-                if (token >= args.tokens) break;
-                float part[8];
+        // A warp a token, four rows a lane, all ranks' loads of two tokens in flight.
+        const int64_t r = (int64_t)tw * 128 + lane * 4;
+        float b[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            b[i] = args.bias && r + i < args.rows ? __ldg(args.bias + r + i) : 0.0f;
+        const int t1 = min((int)(NT * (rank + 1) / ranks),
+                           (int)min(args.tokens - (int64_t)tt * NT, (int64_t)NT));
+        unsigned from[8];
+#pragma unroll
+        for (unsigned q = 0; q < 8; q++) from[q] = tc::map_cta(base + lane * 16, q < ranks ? q : 0);
+        for (int t = (int)(NT * rank / ranks) + warp; t < t1; t += 2 * kThreads / 32) {
+            float4 part[2][8];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (unsigned q = 0; q < 8; q++)
-                    part[q] = q < ranks ? load_cluster(tc::map_cta(
-                                              base + (t * 128 + threadIdx.x) * 4, q))
-                                        : 0.0f;
-                float sum = part[0];
+                    if (q < ranks && t + u * (kThreads / 32) < t1)
+                        part[u][q] = load_cluster(from[q] + (t + u * (kThreads / 32)) * 512);
 #pragma unroll
-                for (int q = 1; q < 8; q++) sum += part[q];
-                if (ok && r < args.rows)
-                    static_cast<T *>(args.c)[token * args.stride + r] = T(sum + b);
+            for (int u = 0; u < 2; u++) {
+                const int tu = t + u * (kThreads / 32);
+                if (tu >= t1) break;
+                float4 sum = part[u][0];
+#pragma unroll
+                for (unsigned q = 1; q < 8; q++)
+                    if (q < ranks) {
+                        sum.x += part[u][q].x, sum.y += part[u][q].y;
+                        sum.z += part[u][q].z, sum.w += part[u][q].w;
+                    }
+                const float y[4] = {sum.x + b[0], sum.y + b[1], sum.z + b[2], sum.w + b[3]};
+                T *c = static_cast<T *>(args.c) + ((int64_t)tt * NT + tu) * args.stride + r;
+                if (!ok) break;
+                if (args.vec && r + 4 <= args.rows) {
+                    store4(c, y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (r + i < args.rows) c[i] = T(y[i]);
+                }
             }
         }
         __syncwarp();
@@ -240,21 +279,10 @@ __global__ void __launch_bounds__(kThreads, 1) thin_kernel(const __grid_constant
 template <int NT, class T>
 inline int launch(Args &args, int t_tiles, int split, cudaStream_t st) {
     const auto kernel = thin_kernel<NT, T>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Shape<NT>::smem) != cudaSuccess)
-        return DRIFT_ECUDA;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(args.w_tiles * t_tiles * split));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Shape<NT>::smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = split;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args) == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+    static unsigned long long done = 0;
+    if (!allow_smem(kernel, Shape<NT>::smem, done)) return DRIFT_ECUDA;
+    return launch_pdl(kernel, dim3((unsigned)(args.w_tiles * t_tiles * split)), kThreads,
+                      Shape<NT>::smem, st, split, args);
 }
 
 }  // namespace thin

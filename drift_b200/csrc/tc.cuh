@@ -41,6 +41,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "pdl.cuh"
 #include "tma.cuh"
 
 namespace drift {
@@ -244,6 +245,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_after();
     const unsigned tmem = tmem_base;
     bool ok = true;
+    pdl_trigger();
+    pdl_wait();
 
     if (warp >= kEpiWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
@@ -465,14 +468,12 @@ inline bool encode_16(CUtensorMap *map, bool bf16, const void *base, int64_t row
 template <int KIND, bool BF16, bool A_MN, bool B_MN, class Epi>
 inline int launch(const Args &args, const Epi &epi, int sms, cudaStream_t st) {
     const auto kernel = pair_kernel<KIND, BF16, A_MN, B_MN, Epi>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             smem_bytes<KIND>()) != cudaSuccess)
-        return DRIFT_ECUDA;
+    static unsigned long long done = 0;
+    if (!allow_smem(kernel, smem_bytes<KIND>(), done)) return DRIFT_ECUDA;
     const int64_t total = (int64_t)args.m_tiles * args.n_tiles * args.splits;
     if (total > 0x7fffffff) return DRIFT_EINVAL;
     const int pairs = (int)(total < sms / 2 ? total : sms / 2);
-    kernel<<<pairs * 2, kThreads, smem_bytes<KIND>(), st>>>(args, epi);
-    return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
+    return launch_pdl(kernel, dim3(pairs * 2), kThreads, smem_bytes<KIND>(), st, 0, args, epi);
 }
 
 }  // namespace tc

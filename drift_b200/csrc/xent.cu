@@ -11,6 +11,8 @@
 //   forward   the logits' tile stays in registers: each thread reduces its 128
 //             columns of a row to a maximum, a sum of exponentials and perhaps the
 //             target's logit; a second kernel joins the parts of a row.
+//             (Where a mean loss is wanted with its gradients and all logits fit in
+//             L2, they are kept in the workspace until d has replaced them.)
 //   gradient  a piece of the vocabulary at a time: the logits again, whose
 //             epilogue writes d in the inputs' type (one rounding, which halves
 //             its bytes and feeds the tensor cores; an element's error is half a
@@ -205,6 +207,8 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const Stat *parts, int n
                                                         Stat *run, bool first, bool last,
                                                         const float *target, XentRows x,
                                                         float *loss, float *lse, int *err) {
+    pdl_trigger();
+    pdl_wait();
     __shared__ Stat sh[8][33];
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
     const int64_t row = (int64_t)blockIdx.x * 32 + lane;
@@ -227,39 +231,14 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const Stat *parts, int n
     const int64_t t = x.at(row, bad);
     if (bad) atomicOr(err, DEV_ERR_INDEX);
     lse[row] = z;
-    if (loss) loss[row] = t >= 0 ? z - target[row] : 0.0f;
-}
-
-// The mean loss over the rows that count, summed in a fixed order by one CTA.
-__global__ void __launch_bounds__(1024) xent_mean_kernel(const float *lse, const float *target,
-                                                         int64_t T, XentRows x, float *mean) {
-    __shared__ float sl[1024];
-    __shared__ int sc[1024];
-    float sum = 0.0f;
-    int count = 0;
-    for (int64_t i = threadIdx.x; i < T; i += 1024) {
-        bool bad = false;
-        if (x.at(i, bad) >= 0) sum += lse[i] - target[i], count++;
-    }
-    sl[threadIdx.x] = sum, sc[threadIdx.x] = count;
-    __syncthreads();
-    for (int o = 512; o; o >>= 1) {
-        if (threadIdx.x < o) {
-            sl[threadIdx.x] += sl[threadIdx.x + o];
-            sc[threadIdx.x] += sc[threadIdx.x + o];
-        }
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        const float c = (float)max(sc[0], 1);
-        mean[0] = sl[0] / c;
-        mean[1] = 1.0f / c;
-    }
+    loss[row] = t >= 0 ? z - target[row] : 0.0f;  // may be target itself
 }
 
 // fp16: the power of two that brings the largest |g| into (2^14, 2^15], and its
 // inverse; 1 where no finite one would help.
 __global__ void __launch_bounds__(1024) xent_scale_kernel(const float *g, int64_t n, float *scale) {
+    pdl_trigger();
+    pdl_wait();
     __shared__ unsigned sm[32];
     unsigned m = 0;
     for (int64_t i = threadIdx.x; i < n; i += 1024)
@@ -279,17 +258,20 @@ __global__ void __launch_bounds__(1024) xent_scale_kernel(const float *g, int64_
     }
 }
 
-// db of a piece from the sums of groups of 32 rows, in order.
+// db of a piece: the sum over `groups` rows of `sums` (each the sum of 32 tokens, or
+// one token's d), in order.
 __global__ void __launch_bounds__(256) xent_colsum_kernel(const float *sums, int64_t groups,
-                                                          int64_t n, const float *alpha,
-                                                          float *db) {
+                                                          int64_t n, int64_t ld,
+                                                          const float *alpha, float *db) {
+    pdl_trigger();
+    pdl_wait();
     __shared__ float sh[8][33];
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
     const int64_t v = (int64_t)blockIdx.x * 32 + lane;
     float s = 0.0f;
     if (v < n) {
 #pragma unroll 4
-        for (int64_t i = slice; i < groups; i += 8) s += sums[i * n + v];
+        for (int64_t i = slice; i < groups; i += 8) s += sums[i * ld + v];
     }
     sh[slice][lane] = s;
     __syncthreads();
@@ -304,6 +286,8 @@ __global__ void __launch_bounds__(256) xent_dx_kernel(const float *acc, int spli
                                                       int64_t ld, T *dx, int64_t rows,
                                                       int64_t cols, int64_t stride,
                                                       const float *alpha, float beta) {
+    pdl_trigger();
+    pdl_wait();
     const float f = alpha ? *alpha * beta : beta;
     const int64_t groups = (cols + 3) / 4;
     for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < rows * groups; i += 256LL * gridDim.x) {
@@ -319,6 +303,79 @@ __global__ void __launch_bounds__(256) xent_dx_kernel(const float *acc, int spli
         for (int j = 0; j < 4; j++)
             if (c + j < cols) p[j] = T(v[j]);
     }
+}
+
+// The mean loss with its gradients where all logits fit the workspace at once: a
+// CTA takes a row, sums the parts of its logits, and replaces them by d, both in
+// fp32 (for db) and in the inputs' type times `scale`. Its loss goes to `row_loss`.
+template <class T>
+__global__ void __launch_bounds__(256) xent_row_kernel(float *logits, int splits, int64_t part,
+                                                       int64_t ld, int64_t n, const float *bias,
+                                                       XentRows x, T *d, float scale, bool keep,
+                                                       float *row_loss, float *lse, int *err) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ Stat sh[8];
+    __shared__ float target;
+    const int64_t row = blockIdx.x;
+    float *l = logits + row * ld;
+    bool bad = false;
+    const int64_t t = x.at(row, bad);
+    Stat r{-INFINITY, 0.0f};
+    for (int64_t v = threadIdx.x; v < n; v += 256) {
+        float y = l[v];
+        for (int k = 1; k < splits; k++) y += l[k * part + v];
+        if (bias) y += bias[v];
+        l[v] = y;  // read again by this thread alone
+        if (v == t) target = y;
+        r = join(r, Stat{y, 1.0f});
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        r = join(r, Stat{__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o)});
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = r;
+    __syncthreads();
+    r = sh[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) r = join(r, sh[i]);
+    const float z = r.m + logf(r.s);
+    for (int64_t v = threadIdx.x; v < n; v += 256) {
+        const float p = exp2_fast((l[v] - z) * kLog2e);
+        const float g = t >= 0 ? (v == t ? p - 1.0f : p) : 0.0f;
+        d[row * ld + v] = T(g * scale);
+        if (keep) l[v] = g;
+    }
+    if (threadIdx.x == 0) {
+        if (bad) atomicOr(err, DEV_ERR_INDEX);
+        row_loss[row] = t >= 0 ? z - target : 0.0f;
+        if (lse) lse[row] = z;
+    }
+}
+
+// The mean of the rows' losses and the inverse count, in a fixed order.
+__global__ void __launch_bounds__(1024) xent_rows_mean_kernel(const float *row_loss, int64_t T,
+                                                              XentRows x, float *mean) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ float sl[32];
+    __shared__ int sc[32];
+    float sum = 0.0f;
+    int count = 0;
+    for (int64_t i = threadIdx.x; i < T; i += blockDim.x) {
+        bool bad = false;
+        sum += row_loss[i];
+        count += x.at(i, bad) >= 0;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    count = (int)__reduce_add_sync(0xffffffffu, count);
+    if ((threadIdx.x & 31) == 0) sl[threadIdx.x >> 5] = sum, sc[threadIdx.x >> 5] = count;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < (int)blockDim.x / 32; i++) sum += sl[i], count += sc[i];
+    const float c = (float)max(count, 1);
+    mean[0] = sum / c;
+    mean[1] = 1.0f / c;
 }
 
 // ------------------------------------------------------------------ plans
@@ -374,13 +431,53 @@ static GradPlan grad_plan(const drift_xent *op) {
     return p;
 }
 
-int64_t xent_workspace(const drift_xent *op, bool grad) {
+// Up to 64 MB of fp32 logits are kept between the loss and its gradient, which
+// then costs 6 T D V operations and not 8: writing and reading them back is 8
+// bytes an element in L2, computing them again 2 D operations. A CTA takes a row,
+// so rows longer than 2^15 (some 20 us) are left to the other way.
+struct KeptPlan {
+    bool use;
+    int64_t ld, part, logits, d, loss, acc, acc_part, acc_ld, bytes;
+    int splits, dx_splits;
+};
+static KeptPlan kept_plan(const drift_xent *op) {
+    KeptPlan p;
+    const int64_t t = std::max<int64_t>(op->tokens, 1);
+    p.ld = up(op->vocab, 8);
+    p.use = op->tokens > 0 && op->vocab <= 32768 && t * p.ld <= (16LL << 20);
+    p.part = t * p.ld;
+    // Few tiles: the contractions are cut, down to two stages a part here, where a
+    // part is a pass over the logits in L2, and 16 for dx.
+    const int lt = tiles(t) * tiles(op->vocab), dt = tiles(t) * tiles(op->depth);
+    p.splits = std::max(1, std::min({stages(op->depth) / 2, 74 / lt, 16}));
+    p.dx_splits = std::max(1, std::min(stages(op->vocab) / 16, 74 / dt));
+    p.logits = 0;
+    p.d = up(p.splits * p.part * 4, 256);
+    p.loss = p.d + up(p.part * 2, 256);
+    p.acc_ld = up(op->depth, 4);
+    p.acc_part = t * p.acc_ld;
+    p.acc = p.loss + up(t * 4, 256);
+    p.bytes = p.acc + (p.dx_splits > 1 ? up(p.dx_splits * p.acc_part * 4, 256) : 0) + 256;
+    return p;
+}
+
+int64_t xent_workspace(const drift_xent *op, int mode) {
+    if (mode == 2) {
+        const KeptPlan k = kept_plan(op);
+        if (k.use) return k.bytes;
+    }
     const int64_t f = forward_plan(op).bytes;
-    return grad ? std::max(f, grad_plan(op).bytes) : f;
+    return mode ? std::max(f, grad_plan(op).bytes + (mode == 2 ? up(op->tokens * 4, 256) : 0)) : f;
 }
 
 static XentRows rows_of(const drift_xent *op) {
     return XentRows{op->targets, op->target_bits == 64, op->ignore_index, op->vocab};
+}
+
+static int rows_mean(const float *row_loss, int64_t n, const XentRows &rows, float *mean,
+                     cudaStream_t st) {
+    return launch_pdl(xent_rows_mean_kernel, dim3(1), n <= 256 ? 256 : 1024, 0, st, 0, row_loss, n,
+                      rows, mean);
 }
 
 static int done() { return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA; }
@@ -408,19 +505,22 @@ static int forward(const drift_xent *op, float *loss, float *lse, float *mean, c
     Stat *parts = reinterpret_cast<Stat *>(ws + p.parts);
     Stat *run = reinterpret_cast<Stat *>(ws + p.run);
     float *target = reinterpret_cast<float *>(ws + p.target);
+    // Where the caller wants no losses but their mean, they take the place of the
+    // targets' logits, which the last join reads just before.
+    float *row_loss = loss ? loss : target;
     for (int64_t v0 = 0; n_t && v0 < op->vocab; v0 += p.piece) {
         const int64_t n = std::min(p.piece, op->vocab - v0);
         tc::Args a;
         if (!logit_args(a, op, v0, n, BF16, err)) return DRIFT_ECUDA;
         const StatsEpi epi{parts, target, op->bias ? op->bias + v0 : nullptr, n_t, n, v0, rows};
-        const int rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
+        int rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
         if (rc) return rc;
-        xent_join_kernel<<<(unsigned)((n_t + 31) / 32), 256, 0, st>>>(
-            parts, (int)((n + 127) / 128), n_t, run, v0 == 0, v0 + n == op->vocab, target, rows,
-            loss, lse, err);
+        rc = launch_pdl(xent_join_kernel, dim3((unsigned)((n_t + 31) / 32)), 256, 0, st, 0, parts,
+                        (int)((n + 127) / 128), n_t, run, v0 == 0, v0 + n == op->vocab, target,
+                        rows, row_loss, lse, err);
+        if (rc) return rc;
     }
-    if (mean) xent_mean_kernel<<<1, 1024, 0, st>>>(lse, target, n_t, rows, mean);
-    return done();
+    return mean ? rows_mean(row_loss, n_t, rows, mean, st) : DRIFT_OK;
 }
 
 template <class T, bool BF16>
@@ -443,7 +543,10 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
     // size. Weights by row go into d.
     const bool one = g_stride == 0;
     float *scale = BF16 || one ? nullptr : reinterpret_cast<float *>(ws + p.scale);
-    if (scale) xent_scale_kernel<<<1, 1024, 0, st>>>(g, n_t, scale);
+    if (scale) {
+        const int rc = launch_pdl(xent_scale_kernel, dim3(1), 1024, 0, st, 0, g, n_t, scale);
+        if (rc) return rc;
+    }
     const float fixed = !BF16 && one ? 32768.0f : 1.0f;
     const float *undo = one ? g : scale ? scale + 1 : nullptr, *sum_undo = one ? g : nullptr;
     const float beta = 1.0f / fixed;
@@ -459,8 +562,8 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
                                        lse, row_g, scale, fixed, sums};
             rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
             if (!rc)
-                xent_colsum_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>(
-                    sums, (n_t + 31) / 32, n, sum_undo, db + v0);
+                rc = launch_pdl(xent_colsum_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, st, 0,
+                                sums, (n_t + 31) / 32, n, n, sum_undo, db + v0);
         } else {
             const GradEpi<T, false> epi{d,   p.ld,  bias,  n_t,   n,      v0, rows,
                                         lse, row_g, scale, fixed, nullptr};
@@ -501,9 +604,81 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
         }
     }
     if (dx && !p.direct)
-        xent_dx_kernel<<<sm_count() * 8, 256, 0, st>>>(acc, p.splits, p.part, p.acc_ld, dx, n_t, dep,
-                                                       dx_stride, undo, beta);
-    return done();
+        return launch_pdl(xent_dx_kernel<T>, dim3(sm_count() * 8), 256, 0, st, 0, acc, p.splits,
+                          p.part, p.acc_ld, dx, n_t, dep, dx_stride, undo, beta);
+    return DRIFT_OK;
+}
+
+template <class T, bool BF16>
+static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx, int64_t dx_stride,
+                     T *dw, int64_t dw_stride, float *db, char *ws, int *err, cudaStream_t st) {
+    const int64_t n_t = op->tokens, dep = op->depth, n = op->vocab;
+    const XentRows rows = rows_of(op);
+    float *logits = reinterpret_cast<float *>(ws + p.logits);
+    float *row_loss = reinterpret_cast<float *>(ws + p.loss);
+    float *acc = reinterpret_cast<float *>(ws + p.acc);
+    T *d = reinterpret_cast<T *>(ws + p.d);
+    const float scale = BF16 ? 1.0f : 32768.0f, beta = 1.0f / scale;
+    tc::Args a;
+    if (!logit_args(a, op, 0, n, BF16, err)) return DRIFT_ECUDA;
+    a.splits = std::min(p.splits, a.k_stages);
+    int rc = tc::launch<tc::KIND_16, BF16, false, false>(
+        a, PartEpi{logits, p.part, p.ld, n_t, n, false}, sm_count(), st);
+    if (rc) return rc;
+    rc = launch_pdl(xent_row_kernel<T>, dim3((unsigned)n_t), 256, 0, st, 0, logits, a.splits, p.part,
+                    p.ld, n, op->bias, rows, d, scale, db != nullptr, row_loss, (float *)nullptr,
+                    err);
+    if (!rc) rc = rows_mean(row_loss, n_t, rows, mean, st);
+    if (!rc && db)
+        rc = launch_pdl(xent_colsum_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, st, 0, logits,
+                        n_t, n, p.ld, mean + 1, db);
+    if (!rc && dx) {
+        if (!tc::encode_16(&a.a, BF16, d, n_t, n, p.ld, true) ||
+            !tc::encode_16(&a.b, BF16, op->w, dep, n, op->w_stride, false))
+            return DRIFT_ECUDA;
+        a.m_tiles = tiles(n_t), a.n_tiles = tiles(dep), a.k_stages = stages(n);
+        a.splits = std::min(p.dx_splits, a.k_stages), a.run = kGradRun;
+        if (a.splits == 1) {
+            const StoreEpi<T> epi{dx,      dx_stride, n_t,  dep,
+                                  nullptr, mean + 1,  beta, rows_aligned(dx, dx_stride)};
+            rc = tc::launch<tc::KIND_16, BF16, false, true>(a, epi, sm_count(), st);
+        } else {
+            const PartEpi epi{acc, p.acc_part, p.acc_ld, n_t, dep, false};
+            rc = tc::launch<tc::KIND_16, BF16, false, true>(a, epi, sm_count(), st);
+            if (!rc)
+                rc = launch_pdl(xent_dx_kernel<T>, dim3(sm_count() * 8), 256, 0, st, 0, acc, a.splits,
+                                p.acc_part, p.acc_ld, dx, n_t, dep, dx_stride, mean + 1, beta);
+        }
+    }
+    if (!rc && dw) {
+        if (!tc::encode_16(&a.a, BF16, d, n, n_t, p.ld, false) ||
+            !tc::encode_16(&a.b, BF16, op->x, dep, n_t, op->x_stride, false))
+            return DRIFT_ECUDA;
+        a.m_tiles = tiles(n), a.n_tiles = tiles(dep), a.k_stages = stages(n_t);
+        a.splits = 1, a.run = kGradRun;
+        const StoreEpi<T> epi{dw,      dw_stride, n,    dep,
+                              nullptr, mean + 1,  beta, rows_aligned(dw, dw_stride)};
+        rc = tc::launch<tc::KIND_16, BF16, true, true>(a, epi, sm_count(), st);
+    }
+    return rc;
+}
+
+int launch_xent_mean(const drift_xent *op, float *mean, void *dx, int64_t dx_stride, void *dw,
+                     int64_t dw_stride, float *db, void *ws, int *err, cudaStream_t st) {
+    const KeptPlan k = kept_plan(op);
+    if (k.use)
+        return op->type == DRIFT_T_BF16
+                   ? mean_kept<__nv_bfloat16, true>(op, k, mean, (__nv_bfloat16 *)dx, dx_stride,
+                                                    (__nv_bfloat16 *)dw, dw_stride, db, (char *)ws,
+                                                    err, st)
+                   : mean_kept<__half, false>(op, k, mean, (__half *)dx, dx_stride, (__half *)dw,
+                                              dw_stride, db, (char *)ws, err, st);
+    float *lse = reinterpret_cast<float *>(
+        (char *)ws + std::max(forward_plan(op).bytes, grad_plan(op).bytes));
+    const int rc = launch_xent(op, nullptr, lse, mean, ws, err, st);
+    return rc ? rc
+              : launch_xent_grad(op, lse, mean + 1, 0, dx, dx_stride, dw, dw_stride, db, ws, err,
+                                 st);
 }
 
 int launch_xent(const drift_xent *op, float *loss, float *lse, float *mean, void *ws, int *err,

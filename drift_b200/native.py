@@ -20,8 +20,10 @@ e2m1, a target outside the vocabulary) are raised by `check_dev`.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
+import operator
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -35,6 +37,7 @@ _F64, _F32, _BF16, _FP16 = range(4)
 torch = None    # imported by the first call: the package itself does not need it
 _LIB = None
 _TYPES = {}
+_DTYPE_OF = operator.attrgetter("dtype")
 
 
 def _start():
@@ -341,15 +344,12 @@ def _xent_ws(call: _Call, op, grad: int):
     return torch.empty(need.value, dtype=torch.uint8, device=call.device)
 
 
-def _xent_backward(call, op, x, lse, g, g_stride, with_bias, ws, need):
-    dx = torch.empty((op.tokens, op.depth), dtype=x.dtype, device=call.device) if need[0] else None
-    dw = torch.empty((op.vocab, op.depth), dtype=x.dtype, device=call.device) if need[1] else None
-    db = torch.empty(op.vocab, dtype=torch.float32, device=call.device) if with_bias else None
-    _lib.check(_LIB.drift_linear_xent_grad_dev(
-        call.handle, op, lse.data_ptr(), g, g_stride, None if dx is None else dx.data_ptr(),
-        op.depth, None if dw is None else dw.data_ptr(), op.depth,
-        None if db is None else db.data_ptr(), ws.data_ptr(), ws.numel(), call.stream))
-    return dx, dw, db
+def _xent_outputs(call, op, x, need_dx, need_dw, with_bias):
+    dev = call.device
+    dx = torch.empty((op.tokens, op.depth), dtype=x.dtype, device=dev) if need_dx else None
+    dw = torch.empty((op.vocab, op.depth), dtype=x.dtype, device=dev) if need_dw else None
+    db = torch.empty(op.vocab, dtype=torch.float32, device=dev) if with_bias else None
+    return dx, dw, db, [None if t is None else t.data_ptr() for t in (dx, dw, db)]
 
 
 @_streamed
@@ -380,25 +380,30 @@ def linear_xent_grad_dev(x, w, targets, lse, d_loss, *, bias=None, ignore_index:
     call.ptr(lse, "lse", torch.float32, op.tokens)
     one = d_loss.numel() == 1
     g = call.ptr(d_loss, "d_loss", torch.float32, None if one else op.tokens)
-    return _xent_backward(call, op, x, lse, g, 0 if one else 1, bias is not None,
-                          _xent_ws(call, op, 1), (need_dx, need_dw))
+    ws = _xent_ws(call, op, 1)
+    dx, dw, db, (px, pw, pb) = _xent_outputs(call, op, x, need_dx, need_dw, bias is not None)
+    _lib.check(_LIB.drift_linear_xent_grad_dev(
+        call.handle, op, lse.data_ptr(), g, 0 if one else 1, px, op.depth, pw, op.depth, pb,
+        ws.data_ptr(), ws.numel(), call.stream))
+    return dx, dw, db
 
 
 @_streamed
 def linear_xent_mean_dev(x, w, targets, *, bias=None, ignore_index: int = -100, ctx=None):
     """mlp.softmax_xent's counterpart for a whole output layer: the mean loss of
     the rows that are not ignored (a float32 scalar tensor; 0 when all are) and its
-    gradients: (loss, dx, dw, db)."""
+    gradients: (loss, dx, dw, db). Up to 2^24 logits in rows of up to 2^15 are kept
+    from the loss to its gradients; beyond, they are computed again, a piece of the
+    vocabulary at a time."""
     call = _Call(x, ctx)
     op, keep = _xent_op(call, x, w, targets, bias, ignore_index)
-    lse = torch.empty(op.tokens, dtype=torch.float32, device=call.device)
     mean = torch.empty(2, dtype=torch.float32, device=call.device)
-    ws = _xent_ws(call, op, 1)
-    _lib.check(_LIB.drift_linear_xent_dev(call.handle, op, None, lse.data_ptr(), mean.data_ptr(),
-                                          ws.data_ptr(), ws.numel(), call.stream))
-    grads = _xent_backward(call, op, x, lse, mean.data_ptr() + 4, 0, bias is not None, ws,
-                           (True, True))
-    return (mean[0], *grads)
+    ws = _xent_ws(call, op, 2)
+    dx, dw, db, (px, pw, pb) = _xent_outputs(call, op, x, True, True, bias is not None)
+    _lib.check(_LIB.drift_linear_xent_mean_dev(
+        call.handle, op, mean.data_ptr(), px, op.depth, pw, op.depth, pb, ws.data_ptr(),
+        ws.numel(), call.stream))
+    return mean[0], dx, dw, db
 
 
 # ------------------------------------------------------------------ AdamW
@@ -442,7 +447,8 @@ class AdamW:
         self.ctx = ctx
         call = _Call(self.params[0], ctx)
         dev = call.device
-        n = self._sizes = [p.numel() for p in self.params]
+        n = self._sizes = self._run = [p.numel() for p in self.params]
+        self._dtypes = None
         if state is None:
             def zeros(dtype, sizes):
                 return [torch.zeros(k, dtype=dtype, device=dev) for k in sizes]
@@ -504,23 +510,32 @@ class AdamW:
             self.hyper.lr = float(lr)
         call = _Call(self.params[0], self.ctx)
         sizes = self._sizes
-        if any(g is None for g in grads):
-            on = [g is not None for g in grads]
+        want = run = sizes
+        try:
+            dtypes = list(map(_DTYPE_OF, grads))
+        except AttributeError:  # some are None
             first = self.params[0]
+            want = [first.numel() if g is None else k for k, g in zip(sizes, grads)]
+            run = [0 if g is None else k for k, g in zip(sizes, grads)]
             grads = [first if g is None else g for g in grads]  # skipped: never read
-            want = [k if u else first.numel() for k, u in zip(sizes, on)]
-            run = [k if u else 0 for k, u in zip(sizes, on)]
-        else:
-            want = run = sizes
-        types = [_TYPES.get(g.dtype, 0) for g in grads]
-        if [g.numel() for g in grads] != want or not all(types) or \
-                any([g.get_device() != call.dev for g in grads]) or \
-                not all([g.is_contiguous() for g in grads]):
-            raise ValueError("grads: expected contiguous float32, bfloat16 or float16 tensors of "
-                             f"the parameters' sizes on {call.device}")
+            dtypes = list(map(_DTYPE_OF, grads))
+        tensor = torch.Tensor
+        if dtypes != self._dtypes:  # as a rule the same as the step before
+            types = [_TYPES.get(t, 0) for t in dtypes]
+            if not all(types):
+                raise ValueError("grads: expected float32, bfloat16 or float16 tensors")
+            self._columns["grad_type"] = types
+            self._dtypes = dtypes
+        if list(map(tensor.numel, grads)) != want or \
+                set(map(tensor.get_device, grads)) != {call.dev} or \
+                not all(map(tensor.is_contiguous, grads)):
+            raise ValueError("grads: expected contiguous tensors of the parameters' sizes on "
+                             f"{call.device}")
         # In whole columns: attribute by attribute the table would cost a microsecond a tensor.
-        cols = self._columns
-        cols["grad"], cols["grad_type"], cols["n"] = [g.data_ptr() for g in grads], types, run
+        self._columns["grad"] = array.array("Q", map(tensor.data_ptr, grads))
+        if run is not self._run:
+            self._columns["n"] = run
+            self._run = run
         _lib.check(_LIB.drift_adamw_dev(
             call.handle, self.hyper, self._table, len(sizes), self._step, self._scalars.data_ptr(),
             call.ptr(d_lr, "d_lr", torch.float32, 1),

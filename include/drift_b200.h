@@ -603,9 +603,9 @@ typedef struct drift_xent {
     int32_t target_bits;   /* 32 or 64 */
     int32_t type;
 } drift_xent;
-/* Workspace bytes of drift_linear_xent_dev (grad 0) and
- * drift_linear_xent_grad_dev (grad 1), which may share one buffer. */
-DRIFT_API int drift_linear_xent_workspace(const drift_xent *op, int grad, int64_t *bytes);
+/* Workspace bytes of drift_linear_xent_dev (mode 0), drift_linear_xent_grad_dev
+ * (1) and drift_linear_xent_mean_dev (2). */
+DRIFT_API int drift_linear_xent_workspace(const drift_xent *op, int mode, int64_t *bytes);
 /* Per row: d_loss (may be NULL) and d_lse, the log of the sum of exponentials.
  * d_mean (may be NULL): two floats, the mean loss of the rows that are not
  * ignored (0 if all are) and 1 / their number (1 if all are). */
@@ -620,6 +620,13 @@ DRIFT_API int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, c
                                const float *d_dloss, int64_t dloss_stride, void *d_dx,
                                int64_t dx_stride, void *d_dw, int64_t dw_stride, float *d_db,
                                void *d_ws, int64_t ws_bytes, void *stream);
+
+/* Both in one call: d_mean as drift_linear_xent_dev's, and that mean's gradients.
+ * Up to 2^24 logits in rows of up to 2^15 are kept in the workspace in between;
+ * beyond, they are computed again. */
+DRIFT_API int drift_linear_xent_mean_dev(drift_ctx *ctx, const drift_xent *op, float *d_mean,
+                               void *d_dx, int64_t dx_stride, void *d_dw, int64_t dw_stride,
+                               float *d_db, void *d_ws, int64_t ws_bytes, void *stream);
 
 /*
  * One AdamW step over `count` tensors (decoupled weight decay; drift_adam_dev's

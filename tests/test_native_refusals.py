@@ -26,6 +26,17 @@ def test_packed_sizes_refuse(rows, cols):
     assert LIB.drift_mx4_sizes(rows, cols, None, None) == _lib.EINVAL
 
 
+@pytest.mark.parametrize("mode", [0, 1, 2])
+@pytest.mark.parametrize("tokens,depth,vocab", [(0, 1, 1), (0, 64, 300), (1, 1, 1), (1, 8, 1 << 24),
+                                                (1 << 22, 8, 3), (100, 4096, 131072)])
+def test_cross_entropy_workspace_of_any_shape(mode, tokens, depth, vocab):
+    op = _lib.DriftXent(tokens=tokens, depth=depth, vocab=vocab)
+    out = ctypes.c_int64()
+    _lib.check(LIB.drift_linear_xent_workspace(ctypes.byref(op), mode, ctypes.byref(out)))
+    assert 0 < out.value < 1 << 36
+    assert LIB.drift_linear_xent_workspace(ctypes.byref(op), 3, ctypes.byref(out)) == _lib.EINVAL
+
+
 def test_a_null_context_is_refused():
     q, x, h = _lib.DriftMx4(), _lib.DriftXent(), _lib.DriftAdamW()
     p = d.policies.by_name("mxfp4").to_c()
