@@ -9,7 +9,8 @@
 //   p' = fma(1 - lr wd, p, -(lr/(1-b1^t) m') / fma(r, 1/sqrt(1-b2^t), eps))
 //
 // The quotient is a product with a reciprocal, within two units in the last
-// place: an IEEE division would be a sixth of the instructions.
+// place, and the root within one: the IEEE forms of both were a third of the
+// instructions, and instructions, not bytes, bounded the 8-bit kernel.
 //
 // In 8 bits the first moment is held as e4m3 codes of m * (448 / amax) and
 // the second as e4m3 codes of its root r, which spans half the binades that v
@@ -33,7 +34,7 @@ namespace drift {
 
 constexpr int kAdamThreads = 256;
 constexpr int kAdamBlock = 256;                     // elements that share a scale
-constexpr int kAdamMostBlocks = 4;                  // blocks that a warp takes in turn
+constexpr int kAdamMostBlocks = 32;                  // blocks that a warp takes in turn
 constexpr int kAdamTensors = 256;                   // tensors of one launch
 
 struct AdamTensor {
@@ -52,7 +53,6 @@ struct AdamArgs {
     AdamTensor t[kAdamTensors];
     uint32_t first[kAdamTensors + 1];  // first chunk of each tensor
     int count;
-    int per_warp;  // blocks a warp takes
     float b1, b2, c1, c2, eps;
     const float *scal;        // lr/(1-b1^t), 1/sqrt(1-b2^t), 1 - lr wd
     const uint64_t *rng;      // Rng state of this step's draws
@@ -83,10 +83,15 @@ __device__ __forceinline__ float rcp_fast(float x) {  // within one unit
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// The larger magnitude; NaN wins.
-__device__ __forceinline__ float max_abs(float a, float b) {
+__device__ __forceinline__ float sqrt_fast(float x) {  // within one unit
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// The largest magnitude of three; NaN wins.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -109,8 +114,8 @@ __device__ __forceinline__ Raw8 load_raw(const void *p, int type, int64_t i, int
     if (type == DRIFT_T_F32) {
         const float *f = static_cast<const float *>(p) + i;
         if (whole) {
-            r.w[0] = __ldcs(reinterpret_cast<const uint4 *>(f));
-            r.w[1] = __ldcs(reinterpret_cast<const uint4 *>(f) + 1);
+            r.w[0] = __ldg(reinterpret_cast<const uint4 *>(f));
+            r.w[1] = __ldg(reinterpret_cast<const uint4 *>(f) + 1);
         } else {
             unsigned *u = reinterpret_cast<unsigned *>(r.w);
 #pragma unroll
@@ -119,7 +124,7 @@ __device__ __forceinline__ Raw8 load_raw(const void *p, int type, int64_t i, int
     } else {
         const uint16_t *h = static_cast<const uint16_t *>(p) + i;
         if (whole) {
-            r.w[0] = __ldcs(reinterpret_cast<const uint4 *>(h));
+            r.w[0] = __ldg(reinterpret_cast<const uint4 *>(h));
         } else {
             unsigned *u = reinterpret_cast<unsigned *>(r.w);
 #pragma unroll
@@ -191,7 +196,7 @@ __device__ __forceinline__ void store8(void *p, int type, int64_t i, int valid, 
 
 __device__ __forceinline__ uint64_t load_codes(const void *p, int64_t i, int valid, bool whole) {
     const uint8_t *c = static_cast<const uint8_t *>(p) + i;
-    if (whole) return __ldcs(reinterpret_cast<const unsigned long long *>(c));
+    if (whole) return __ldg(reinterpret_cast<const unsigned long long *>(c));
     uint64_t w = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++)
@@ -211,13 +216,11 @@ __device__ __forceinline__ void decode(uint64_t w, float scale, f2 (&x)[4]) {
 }
 
 __device__ __forceinline__ float warp_amax(const f2 (&x)[4]) {
-    float m = 0.0f;
+    float a[8];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        float a, b;
-        f2_split(x[j], a, b);
-        m = max_abs(m, max_abs(a, b));
-    }
+    for (int j = 0; j < 4; j++) f2_split(x[j], a[2 * j], a[2 * j + 1]);
+    const float m = max3_abs(max3_abs(a[0], a[1], a[2]), max3_abs(a[3], a[4], a[5]),
+                             max3_abs(a[6], a[7], 0.0f));
     // As bit patterns magnitudes order like integers, NaN above Inf above all else.
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu));
 }
@@ -271,40 +274,41 @@ template <> struct Loaded<true> {
     float ms, vs;
 };
 
-template <bool EIGHT>
+// PT, GT: the types of parameter and gradient, or -1 to look them up. WHOLE: all 256
+// elements exist and are aligned.
+template <bool EIGHT, int PT, int GT, bool WHOLE>
 __device__ __forceinline__ void load_block(const AdamTensor &t, int64_t block, int lane,
                                            Loaded<EIGHT> &l) {
     const int64_t i = block * kAdamBlock + lane * 8;
-    const int valid = (int)max((int64_t)0, min((int64_t)8, t.n - i));
-    const bool whole = t.vec && valid == 8;
-    l.g = load_raw(t.g, t.gt, i, valid, whole);
-    l.p = load_raw(t.p, t.pt, i, valid, whole);
+    const int valid = WHOLE ? 8 : (int)max((int64_t)0, min((int64_t)8, t.n - i));
+    l.g = load_raw(t.g, GT < 0 ? t.gt : GT, i, valid, WHOLE);
+    l.p = load_raw(t.p, PT < 0 ? t.pt : PT, i, valid, WHOLE);
     if constexpr (EIGHT) {
-        l.m = load_codes(t.m, i, valid, whole);
-        l.v = load_codes(t.v, i, valid, whole);
+        l.m = load_codes(t.m, i, valid, WHOLE);
+        l.v = load_codes(t.v, i, valid, WHOLE);
         l.ms = t.ms[block];
         l.vs = t.vs[block];
     } else {
-        l.m = load_raw(t.m, DRIFT_T_F32, i, valid, whole);
-        l.v = load_raw(t.v, DRIFT_T_F32, i, valid, whole);
+        l.m = load_raw(t.m, DRIFT_T_F32, i, valid, WHOLE);
+        l.v = load_raw(t.v, DRIFT_T_F32, i, valid, WHOLE);
     }
 }
 
 struct Scalars {
     f2 b1, b2, c1, c2, eps, neg_a1, rc2, keep, gs;
+    uint64_t state;
     bool scaled;
 };
 
-template <bool EIGHT, bool SR>
+template <bool EIGHT, bool SR, int PT, int GT, bool WHOLE>
 __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block, int lane,
-                                             const Loaded<EIGHT> &l, const Scalars &k,
-                                             uint64_t state) {
+                                             const Loaded<EIGHT> &l, const Scalars &k) {
     const int64_t i = block * kAdamBlock + lane * 8;
-    const int valid = (int)max((int64_t)0, min((int64_t)8, t.n - i));
-    const bool whole = t.vec && valid == 8;
+    const int valid = WHOLE ? 8 : (int)max((int64_t)0, min((int64_t)8, t.n - i));
+    const int pt = PT < 0 ? t.pt : PT, gt = GT < 0 ? t.gt : GT;
     f2 p[4], g[4], m[4], v[4], r[4];
-    unpack(l.g, t.gt, g);
-    unpack(l.p, t.pt, p);
+    unpack(l.g, gt, g);
+    unpack(l.p, pt, p);
     if constexpr (EIGHT) {
         decode(l.m, l.ms, m);
         decode(l.v, l.vs, r);
@@ -321,19 +325,19 @@ __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block,
         v[j] = f2_fma(k.b2, v[j], f2_mul(f2_mul(k.c2, gj), gj));
         float a, b;
         f2_split(v[j], a, b);
-        r[j] = f2_pack(__fsqrt_rn(a), __fsqrt_rn(b));
+        r[j] = f2_pack(sqrt_fast(a), sqrt_fast(b));
         f2_split(f2_fma(r[j], k.rc2, k.eps), a, b);
         const f2 step = f2_mul(f2_mul(k.neg_a1, m[j]), f2_pack(rcp_fast(a), rcp_fast(b)));
         p[j] = f2_fma(k.keep, p[j], step);
     }
-    store8(t.p, t.pt, i, valid, whole, p);
-    if (t.ct >= 0) store8(t.copy, t.ct, i, valid, whole, p);
+    store8(t.p, pt, i, valid, WHOLE, p);
+    if (t.ct >= 0) store8(t.copy, t.ct, i, valid, WHOLE, p);
     if constexpr (EIGHT) {
         unsigned um[8] = {}, uv[8] = {};
         if (SR) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const uint64_t u = splitmix_mix(state + (t.first_draw + i + j + 1) * kGolden);
+                const uint64_t u = splitmix_mix(k.state + (t.first_draw + i + j + 1) * kGolden);
                 um[j] = (unsigned)(u >> 44);
                 uv[j] = (unsigned)(u >> 24) & 0xfffffu;
             }
@@ -350,20 +354,39 @@ __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block,
             inv = s = __uint_as_float(0x7fffffffu);
         } else if (amax >= 0x1p-100f) {
             inv = 448.0f / amax;
-            s = amax / 448.0f;
+            s = amax * (1.0f / 448.0f);
         }
         if (lane == 0) t.ms[block] = s;
         if (lane == 16) t.vs[block] = s;
-        store_codes<SR>(t.m, i, valid, whole, __shfl_sync(0xffffffffu, inv, 0), m, um);
-        store_codes<SR>(t.v, i, valid, whole, __shfl_sync(0xffffffffu, inv, 16), r, uv);
+        store_codes<SR>(t.m, i, valid, WHOLE, __shfl_sync(0xffffffffu, inv, 0), m, um);
+        store_codes<SR>(t.v, i, valid, WHOLE, __shfl_sync(0xffffffffu, inv, 16), r, uv);
     } else {
-        store8(t.m, DRIFT_T_F32, i, valid, whole, m);
-        store8(t.v, DRIFT_T_F32, i, valid, whole, v);
+        store8(t.m, DRIFT_T_F32, i, valid, WHOLE, m);
+        store8(t.v, DRIFT_T_F32, i, valid, WHOLE, v);
     }
 }
 
+// `n` whole blocks, `step` apart; the next one's loads are in flight while one is
+// computed.
+template <bool EIGHT, bool SR, int PT, int GT>
+__device__ __forceinline__ void run_blocks(const AdamTensor &t, int64_t block, int n, int64_t step,
+                                           int lane, const Scalars &k) {
+    Loaded<EIGHT> next;
+    load_block<EIGHT, PT, GT, true>(t, block, lane, next);
+#pragma unroll 1
+    for (int b = 0; b < n; b++) {
+        const Loaded<EIGHT> now = next;
+        if (b + 1 < n)
+            load_block<EIGHT, PT, GT, true>(t, block + step, lane, next);
+        update_block<EIGHT, SR, PT, GT, true>(t, block, lane, now, k);
+        block += step;
+    }
+}
+
+// 8-bit moments: 64 registers and four CTAs an SM; 32-bit ones hold more in flight
+// a thread and run as fast with two.
 template <bool EIGHT, bool SR>
-__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamArgs a) {
+__global__ void __launch_bounds__(kAdamThreads, EIGHT && !SR ? 4 : 2) adamw_kernel(const __grid_constant__ AdamArgs a) {
     pdl_trigger();
     pdl_wait();
     // The last tensor whose first chunk is not above this one.
@@ -375,30 +398,40 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
     }
     const AdamTensor &t = a.t[lo];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t chunk = blockIdx.x - a.first[lo];
-    // This warp's blocks: warp, warp + 8, ... of the CTA's chunk. The next
-    // block's loads are in flight while one is computed.
-    const int64_t blocks = (t.n + kAdamBlock - 1) / kAdamBlock;
-    const int64_t b0 = (int64_t)chunk * (kAdamThreads / 32 * a.per_warp) + warp;
-    const int n = (int)max((int64_t)0, min((int64_t)a.per_warp,
-                                           (blocks - b0 + kAdamThreads / 32 - 1) /
-                                               (kAdamThreads / 32)));
-    if (n == 0) return;
-    Loaded<EIGHT> next;
-    load_block<EIGHT>(t, b0, lane, next);
+    constexpr int kWarps = kAdamThreads / 32;
+    // This warp's blocks: b0, b0 + step, ..., the tensor's CTAs side by side, so that
+    // all that run at a time sweep one stretch of memory.
+    const int64_t b0 = (int64_t)(blockIdx.x - a.first[lo]) * kWarps + warp;
+    const int64_t step = (int64_t)(a.first[lo + 1] - a.first[lo]) * kWarps;
+    const auto count = [&](int64_t blocks) {  // of them below `blocks`
+        return blocks > b0 ? (int)((blocks - b0 + step - 1) / step) : 0;
+    };
+    const int n = count((t.n + kAdamBlock - 1) / kAdamBlock);
+    int whole = t.vec ? count(t.n / kAdamBlock) : 0;
     Scalars k;
     k.b1 = f2_both(a.b1), k.b2 = f2_both(a.b2), k.c1 = f2_both(a.c1), k.c2 = f2_both(a.c2);
     k.eps = f2_both(a.eps);
     k.neg_a1 = f2_both(-a.scal[0]), k.rc2 = f2_both(a.scal[1]), k.keep = f2_both(a.scal[2]);
     k.scaled = a.grad_scale != nullptr;
     k.gs = f2_both(k.scaled ? *a.grad_scale : 1.0f);
-    const uint64_t state = SR ? *a.rng : 0;
+    k.state = SR ? *a.rng : 0;
+    // The usual types have code of their own; fp16, unaligned tensors and the last,
+    // partial block of one take the general form.
+    if (whole) {
+        if (t.pt == DRIFT_T_F32 && t.gt == DRIFT_T_F32)
+            run_blocks<EIGHT, SR, DRIFT_T_F32, DRIFT_T_F32>(t, b0, whole, step, lane, k);
+        else if (t.pt == DRIFT_T_F32 && t.gt == DRIFT_T_BF16)
+            run_blocks<EIGHT, SR, DRIFT_T_F32, DRIFT_T_BF16>(t, b0, whole, step, lane, k);
+        else if (t.pt == DRIFT_T_BF16 && t.gt == DRIFT_T_BF16)
+            run_blocks<EIGHT, SR, DRIFT_T_BF16, DRIFT_T_BF16>(t, b0, whole, step, lane, k);
+        else
+            whole = 0;
+    }
 #pragma unroll 1
-    for (int b = 0; b < n; b++) {
-        const Loaded<EIGHT> now = next;
-        const int64_t block = b0 + b * (kAdamThreads / 32);
-        if (b + 1 < n) load_block<EIGHT>(t, block + kAdamThreads / 32, lane, next);
-        update_block<EIGHT, SR>(t, block, lane, now, k, state);
+    for (int b = whole; b < n; b++) {
+        Loaded<EIGHT> now;
+        load_block<EIGHT, -1, -1, false>(t, b0 + b * step, lane, now);
+        update_block<EIGHT, SR, -1, -1, false>(t, b0 + b * step, lane, now, k);
     }
 }
 
@@ -431,13 +464,13 @@ int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_
     a.rng = rng_used;
     a.grad_scale = d_grad_scale;
     a.count = 0;
-    // Warps take several blocks in turn, loading ahead, once that leaves four
-    // CTAs an SM; few blocks spread over the SMs instead.
-    a.per_warp = 1;
-    while (a.per_warp < kAdamMostBlocks &&
-           blocks >= (int64_t)a.per_warp * 2 * (kAdamThreads / 32) * 4 * sm_count())
-        a.per_warp *= 2;
-    const uint64_t chunk_len = (uint64_t)kAdamBlock * (kAdamThreads / 32) * a.per_warp;
+    // Warps take several blocks in turn, loading ahead, once that leaves twelve
+    // CTAs an SM (three waves or more); few blocks spread over the SMs instead.
+    int per_warp = 1;
+    while (per_warp < kAdamMostBlocks &&
+           blocks >= (int64_t)per_warp * 2 * (kAdamThreads / 32) * 12 * sm_count())
+        per_warp *= 2;
+    const uint64_t chunk_len = (uint64_t)kAdamBlock * (kAdamThreads / 32) * per_warp;
     uint64_t chunks = 0, drawn = 0;
     auto flush = [&]() {
         if (a.count == 0) return;

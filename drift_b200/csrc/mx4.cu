@@ -473,7 +473,7 @@ __device__ __forceinline__ uint4 mx_cast_col(const MxCast &a, const typename MxS
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(256) mx4_cols_kernel(const __grid_constant__ MxCast a,
+__global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 : 3) mx4_cols_kernel(const __grid_constant__ MxCast a,
                                                        uint32_t row_tiles,
                                                        uint32_t col_tiles) {
     using S = MxSrc<TYPE>;
@@ -509,23 +509,31 @@ __global__ void __launch_bounds__(256) mx4_cols_kernel(const __grid_constant__ M
     if (a.codes) {
         unsigned clamps = 0;
         int err = 0;
-        const int64_t blocks = mx4_blocks(a.cols), k_tiles = mx4_k_tiles(a.cols);
+        const int blocks = (int)mx4_blocks(a.cols), k_tiles = (int)mx4_k_tiles(a.cols);
+        const int64_t row_bytes = (int64_t)blocks * 16;
+        const int r = tid / kGroups, block = (int)(c0 >> 5) + tid % kGroups / 4;
+        const bool in_cols = block < blocks;
+        uint8_t *codes = a.codes + (r0 + r) * row_bytes + c0 / 2 + tid % kGroups * 4;
+        uint8_t *scales = a.scales + ((int64_t)tile_r * k_tiles + block / 4) * kMxTileBytes +
+                          block % 4;
+        uint64_t draw = (uint64_t)(r0 + r) * a.cols + c0 + tid % kGroups * 8;
 #pragma unroll
         for (int i = 0; i < G::kLoads; i++) {
-            const int at = i * 256 + tid;
-            const int64_t row = r0 + at / kGroups, col = c0 + at % kGroups * 8, block = col >> 5;
+            constexpr int kStep = 256 / kGroups;  // rows from one load to the next
+            const int at = r + i * kStep;
             int shared;
-            const unsigned w = mx_cast8<TYPE>(a, raw[i], 8, state, (uint64_t)row * a.cols + col,
-                                              shared, clamps, err);
-            const bool in = row < a.rows && block < blocks;
-            if (in) *reinterpret_cast<unsigned *>(a.codes + row * blocks * 16 + col / 2) = w;
+            const unsigned w = mx_cast8<TYPE>(a, raw[i], 8, state, draw, shared, clamps, err);
+            const bool in = in_cols && r0 + at < a.rows;
+            if (in) *reinterpret_cast<unsigned *>(codes) = w;
+            codes += kStep * row_bytes;
+            draw += (uint64_t)kStep * a.cols;
             if ((lane & 3) == 0 && block < k_tiles * 4) {
-                a.scales[mx4_scale_offset(row, block, k_tiles)] =
-                    in ? (uint8_t)(shared + 127) : (uint8_t)127;
+                uint8_t *to = scales + at % 32 * 16 + at / 32 * 4;
+                *to = in ? (uint8_t)(shared + 127) : (uint8_t)127;
                 // The last columns' CTA also writes the pair's remaining blocks.
                 if (tile_c + 1 == col_tiles)
-                    for (int64_t b = block + G::kCols / 32; b < k_tiles * 4; b += G::kCols / 32)
-                        a.scales[mx4_scale_offset(row, b, k_tiles)] = 127;
+                    for (int b = block + G::kCols / 32; b < k_tiles * 4; b += G::kCols / 32)
+                        to[(b / 4 - block / 4) * kMxTileBytes + b % 4 - block % 4] = 127;
             }
         }
         mx_finish(clamps, err, a.clamped, a.err);
@@ -569,21 +577,20 @@ __global__ void __launch_bounds__(256) mx4_cols_kernel(const __grid_constant__ M
                                      shared[0], clamps, err);
     }
     __syncthreads();
-    const int64_t k_tiles = mx4_k_tiles(a.rows), blocks = mx4_blocks(a.rows);
-    const int64_t last = mx4_row_tiles(a.cols) * 128;
+    const int64_t blocks = mx4_blocks(a.rows);
+    const int k_tiles = (int)mx4_k_tiles(a.rows);
+    // The transpose's tile of scales: its rows are columns here, its blocks rows.
+    uint8_t *scales_t =
+        a.scales_t + ((c0 / 128) * k_tiles + tile_r) * (int64_t)kMxTileBytes + b;
 #pragma unroll
     for (int h = 0; h < G::kWide; h++) {
-        const int c = word * G::kWide + h;
+        const int c = word * G::kWide + h, in_tile = (int)(c0 % 128) + c;
         *reinterpret_cast<uint4 *>(mx_smem + c * 80 + b * 16) = codes[h];
-        // Scale bytes, with the padding of the last tiles: this CTA's columns up to
-        // the tile's 128 rows, and blocks up to a whole pair of tiles.
-        const int64_t col = c0 + c;
-        if (col < last) {
-            a.scales_t[mx4_scale_offset(col, row >> 5, k_tiles)] =
-                col < a.cols && row < a.rows ? (uint8_t)(shared[h] + 127) : (uint8_t)127;
-            if (tile_r + 1 == row_tiles && tile_r % 2 == 0)
-                a.scales_t[mx4_scale_offset(col, (row >> 5) + 4, k_tiles)] = 127;
-        }
+        // With the padding of the last tiles: columns up to the tile's 128 rows (the
+        // grid's columns end with them), blocks up to a whole pair of tiles.
+        uint8_t *to = scales_t + in_tile % 32 * 16 + in_tile / 32 * 4;
+        *to = c0 + c < a.cols && row < a.rows ? (uint8_t)(shared[h] + 127) : (uint8_t)127;
+        if (tile_r + 1 == row_tiles && tile_r % 2 == 0) to[kMxTileBytes] = 127;
     }
     mx_finish(clamps, err, a.clamped_t, a.err);
     __syncthreads();

@@ -110,7 +110,6 @@ __global__ void __launch_bounds__(kThreads, 1) thin_kernel(const __grid_constant
     tc::fence_after();
     const unsigned tmem = tmem_base;
     bool ok = true;
-    pdl_trigger();
     pdl_wait();
 
     if (warp == 4) {
@@ -218,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1) thin_kernel(const __grid_constant
         tc::fence_before();
     }
 
+    pdl_trigger();
     if (!ok) {
         atomicOr(args.err, DEV_ERR_TIMEOUT);
         for (int i = 0; i < 2000; i++) __nanosleep(1000);

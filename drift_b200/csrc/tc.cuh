@@ -245,7 +245,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_after();
     const unsigned tmem = tmem_base;
     bool ok = true;
-    pdl_trigger();
     pdl_wait();
 
     if (warp >= kEpiWarps) {
@@ -426,6 +425,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     }
 
+    // Not before: a small kernel set up early would crowd on the first SMs to fall
+    // free (a join of 32 CTAs then takes twice its time).
+    pdl_trigger();
     if (!ok) {
         atomicOr(args.err, DEV_ERR_TIMEOUT);
         // Give copies and MMAs in flight time to land before TMEM and shared

@@ -201,26 +201,36 @@ template <class T, bool DB> struct GradEpi {
 
 // ------------------------------------------------------------------ small kernels
 
-// Joins a row's parts, and the running statistics of the pieces before, with 32
-// threads a row; the last piece gives its log sum and loss.
-__global__ void __launch_bounds__(256) xent_join_kernel(const Stat *parts, int n_parts, int64_t T,
-                                                        Stat *run, bool first, bool last,
-                                                        const float *target, XentRows x,
-                                                        float *loss, float *lse, int *err) {
+// Joins a row's parts, and the running statistics of the pieces before; the last
+// piece gives its log sum and loss. Many rows: a CTA takes 32 of them, 32 threads a
+// row, so that a warp reads 32 rows' part i together. Few rows (ROWS 1): a CTA a row.
+template <int ROWS>
+__global__ void __launch_bounds__(1024) xent_join_kernel(const Stat *parts, int n_parts, int64_t T,
+                                                         Stat *run, bool first, bool last,
+                                                         const float *target, XentRows x,
+                                                         float *loss, float *lse, int *err) {
     pdl_trigger();
     pdl_wait();
-    __shared__ Stat sh[8][33];
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+    __shared__ Stat sh[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS == 1 ? 0 : lane);
     Stat r{-INFINITY, 0.0f};
     if (row < T) {
+        const int from = ROWS == 1 ? (int)threadIdx.x : warp;
+        const int step = ROWS == 1 ? (int)blockDim.x : warps;
 #pragma unroll 4
-        for (int i = slice; i < n_parts; i += 8) r = join(r, parts[(int64_t)i * T + row]);
+        for (int i = from; i < n_parts; i += step) r = join(r, parts[(int64_t)i * T + row]);
     }
-    sh[slice][lane] = r;
+    if (ROWS == 1) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            r = join(r, Stat{__shfl_xor_sync(0xffffffffu, r.m, o),
+                             __shfl_xor_sync(0xffffffffu, r.s, o)});
+    }
+    sh[warp][lane] = r;
     __syncthreads();
-    if (slice || row >= T) return;
-    for (int i = 1; i < 8; i++) r = join(r, sh[i][lane]);
+    if (warp || row >= T || (ROWS == 1 && lane)) return;
+    for (int i = 1; i < warps; i++) r = join(r, sh[i][lane]);
     if (!first) r = join(run[row], r);
     if (!last) {
         run[row] = r;
@@ -515,9 +525,12 @@ static int forward(const drift_xent *op, float *loss, float *lse, float *mean, c
         const StatsEpi epi{parts, target, op->bias ? op->bias + v0 : nullptr, n_t, n, v0, rows};
         int rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
         if (rc) return rc;
-        rc = launch_pdl(xent_join_kernel, dim3((unsigned)((n_t + 31) / 32)), 256, 0, st, 0, parts,
-                        (int)((n + 127) / 128), n_t, run, v0 == 0, v0 + n == op->vocab, target,
-                        rows, row_loss, lse, err);
+        const int n_parts = (int)((n + 127) / 128);
+        const bool few = n_t < 1024;
+        rc = launch_pdl(few ? xent_join_kernel<1> : xent_join_kernel<32>,
+                        dim3((unsigned)(few ? n_t : (n_t + 31) / 32)), few ? 128 : 1024, 0, st, 0,
+                        parts, n_parts, n_t, run, v0 == 0, v0 + n == op->vocab, target, rows,
+                        row_loss, lse, err);
         if (rc) return rc;
     }
     return mean ? rows_mean(row_loss, n_t, rows, mean, st) : DRIFT_OK;

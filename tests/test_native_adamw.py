@@ -25,7 +25,7 @@ def to8(x):
         inv = np.where(tiny, F(0), F(448) / amax)
     y = np.clip(b * inv, F(-448), F(448))
     code = torch.from_numpy(y.reshape(-1)[:n].copy()).to(torch.float8_e4m3fn)
-    return code, np.where(tiny, F(1), amax / F(448))[:, 0].astype(F)
+    return code, np.where(tiny, F(1), amax * (F(1) / F(448)))[:, 0].astype(F)
 
 
 def from8(code, scale):
@@ -63,13 +63,14 @@ def tensors(sizes, pt, gt, seed, offset=0):
 
 def near(got, want, u, dtype):
     """The two scalars of a step come from the device's pow, each within a unit of
-    fp32 of numpy's; the quotient is a product with a reciprocal, within two; the
-    plain quotient has its own half: the update is within five units. Then one
+    fp32 of numpy's; the quotient is a product with a reciprocal, within two, of a
+    root within one; the plain quotient and root have their own halves: the update is
+    within six units. Then one
     rounding to the type (and its subnormals), where the plain value's own rounding
     may fall on the other side."""
     err = np.abs(got.double().cpu().numpy() - want.astype(np.float64))
     eps = torch.finfo(dtype).eps
-    assert (err <= 5 * 2.0 ** -23 * np.abs(u) + eps * np.abs(want) + 2.0 ** -24).all()
+    assert (err <= 6 * 2.0 ** -23 * np.abs(u) + eps * np.abs(want) + 2.0 ** -24).all()
 
 
 @pytest.mark.parametrize("pt,gt", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"),
@@ -105,10 +106,20 @@ def test_moments_in_8_bits(pt, gt, offset):
             m, r = from8(*held[0][i]), from8(*held[1][i])
             want, m, _, r, u = update(before[i], grads[i].float().cpu().numpy(), m, r * r, t)
             held[0][i], held[1][i] = to8(m), to8(r)
-            for k, (code, scale) in enumerate((held[0][i], held[1][i])):
-                assert (opt.state[2 * k][i].cpu().view(torch.uint8) == code.view(torch.uint8)).all()
-                assert (opt.state[2 * k + 1][i].cpu().numpy() == scale).all()
             near(params[i], want, u, DT[pt])
+            code, scale = (opt.state[k][i].cpu() for k in (0, 1))
+            assert (code.view(torch.uint8) == held[0][i][0].view(torch.uint8)).all()
+            assert (scale.numpy() == held[0][i][1]).all()
+            # The root is within a unit of the nearest float, and so is a block's
+            # largest, its scale with it: x / scale is within 3 units of the plain one,
+            # and the code within that of a nearest one. The device's state goes on.
+            code, scale = opt.state[2][i].cpu(), opt.state[3][i].cpu().numpy()
+            assert (np.abs(scale - held[1][i][1]) <= 2 * 2.0 ** -23 * scale).all()
+            y = r / np.repeat(held[1][i][1], 256)[:r.size].astype(np.float64)
+            got = code.double().numpy()
+            step = 2.0 ** np.maximum(np.floor(np.log2(np.maximum(got, 2.0 ** -9))) - 3, -9)
+            assert (np.abs(got - y) <= step / 2 + 4 * 2.0 ** -23 * y).all()
+            held[1][i] = (code, scale)
 
 
 def test_against_the_formula_in_64_bits():
