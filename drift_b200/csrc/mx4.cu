@@ -60,6 +60,24 @@ template <> struct MxSrc<DRIFT_T_BF16> {
     static constexpr unsigned kInf = 0x7f80u;
     __device__ static V get(T x) { return __bfloat162float(x); }
     __device__ static V get_bits(unsigned h) { return __uint_as_float(h << 16); }
+    // Of each half, the larger magnitude, signs left in place; a NaN stays one.
+    __device__ static unsigned max2(unsigned a, unsigned b) {
+        unsigned m;
+        asm("{\n .reg .b32 x, y;\n abs.bf16x2 x, %1;\n abs.bf16x2 y, %2;\n"
+            " max.NaN.bf16x2 %0, x, y;\n}"
+            : "=r"(m)
+            : "r"(a), "r"(b));
+        return m;
+    }
+    // Both halves times powers of two, in fp32: exact, but for results far below the
+    // smallest code. A product and a -0 fused keep the sign of a zero.
+    __device__ static void scaled2(unsigned w, float lo, float hi, float &a, float &b) {
+        asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n fma.rn.f32.bf16 %0, l, %3, %5;\n"
+            " fma.rn.f32.bf16 %1, h, %4, %5;\n}"
+            : "=f"(a), "=f"(b)
+            : "r"(w), "h"((unsigned short)(__float_as_uint(lo) >> 16)),
+              "h"((unsigned short)(__float_as_uint(hi) >> 16)), "f"(-0.0f));
+    }
     __device__ static int exponent(unsigned key) {
         return MxSrc<DRIFT_T_F32>::exponent(key << 16);
     }
@@ -70,6 +88,13 @@ template <> struct MxSrc<DRIFT_T_FP16> {
     static constexpr unsigned kInf = 0x7c00u;
     __device__ static V get(T x) { return __half2float(x); }
     __device__ static V get_bits(unsigned h) { return __half2float(__ushort_as_half((uint16_t)h)); }
+    __device__ static unsigned max2(unsigned a, unsigned b) {
+        return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu);
+    }
+    __device__ static void scaled2(unsigned w, float lo, float hi, float &a, float &b) {
+        a = get_bits(w & 0xffffu) * lo;
+        b = get_bits(w >> 16) * hi;
+    }
     __device__ static int exponent(unsigned key) {
         return MxSrc<DRIFT_T_F32>::exponent(__float_as_uint(get_bits(key)));
     }
@@ -200,8 +225,8 @@ template <int TYPE> struct MxRaw8 {
     __device__ unsigned key() const {  // the largest of the eight
         if constexpr (sizeof(typename S::T) == 2) {
             const unsigned *u = words();
-            const unsigned m = __vmaxu2(__vmaxu2(u[0] & 0x7fff7fffu, u[1] & 0x7fff7fffu),
-                                        __vmaxu2(u[2] & 0x7fff7fffu, u[3] & 0x7fff7fffu));
+            const unsigned m =
+                S::max2(S::max2(u[0], u[1]), S::max2(u[2], u[3])) & 0x7fff7fffu;
             return max(m & 0xffffu, m >> 16);
         } else {
             const typename S::T *x = reinterpret_cast<const typename S::T *>(w);
@@ -259,6 +284,23 @@ __device__ __forceinline__ unsigned mx_fast8(const double (&x)[8], double down) 
     return mx_rn8(y);
 }
 
+template <int TYPE>
+__device__ __forceinline__ unsigned mx_fast8(const MxRaw8<TYPE> &r,
+                                             typename MxSrc<TYPE>::V down) {
+    using S = MxSrc<TYPE>;
+    if constexpr (sizeof(typename S::T) == 2) {
+        const unsigned *u = r.words();
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) S::scaled2(u[j], down, down, y[2 * j], y[2 * j + 1]);
+        return mx_rn8(y);
+    } else {
+        typename S::V x[8];
+        r.values(x);
+        return mx_fast8(x, down);
+    }
+}
+
 // ------------------------------------------------------------------ the cast
 
 struct MxCast {
@@ -274,24 +316,28 @@ struct MxCast {
     int *err;
 };
 
+// Eight elements at p, 16-byte aligned.
+template <int TYPE>
+__device__ __forceinline__ MxRaw8<TYPE> mx_load_whole(const typename MxSrc<TYPE>::T *p) {
+    MxRaw8<TYPE> r;
+#pragma unroll
+    for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++)
+        r.w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
+    return r;
+}
 // `valid` elements at p, the rest zeros; `vec`: p is 16-byte aligned.
 template <int TYPE>
 __device__ __forceinline__ MxRaw8<TYPE> mx_load8(bool vec, const typename MxSrc<TYPE>::T *p,
                                                  int valid) {
     using T = typename MxSrc<TYPE>::T;
+    if (vec && valid == 8) return mx_load_whole<TYPE>(p);
     MxRaw8<TYPE> r;
-    if (vec && valid == 8) {
+    T *t = reinterpret_cast<T *>(r.w);
 #pragma unroll
-        for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++)
-            r.w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
-    } else {
-        T *t = reinterpret_cast<T *>(r.w);
+    for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++) r.w[j] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++) r.w[j] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < valid) t[j] = p[j];
-    }
+    for (int j = 0; j < 8; j++)
+        if (j < valid) t[j] = p[j];
     return r;
 }
 
@@ -330,17 +376,18 @@ __device__ __forceinline__ unsigned mx_cast8(const MxCast &a, const MxRaw8<TYPE>
     key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
     key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
     V x[8];
-    r.values(x);
     if (__all_sync(0xffffffffu, key < S::kInf) && a.rm == DRIFT_NEAREST_EVEN) {
         const MxFactor<V> f = mx_factor<TYPE>(key, a.headroom);
         shared = f.shared;
         if (a.clamped) {
+            r.values(x);
 #pragma unroll
             for (int j = 0; j < 8; j++) clamps += fabs(x[j] * f.down) > (V)6;
         }
-        const unsigned w = mx_fast8(x, f.down);
+        const unsigned w = mx_fast8<TYPE>(r, f.down);
         return key ? w : 0;
     }
+    r.values(x);
     V amax = (V)0;
 #pragma unroll
     for (int j = 0; j < 8; j++) amax = fmax(amax, mx_mag(x[j]));
@@ -389,25 +436,33 @@ __global__ void __launch_bounds__(256) mx4_rows_kernel(const __grid_constant__ M
                           (int64_t)first * 2 * kMxTileBytes + place;
         // What is left of the row from this lane's first element on.
         const int64_t left = in_row ? a.cols - col0 : 0;
-        MxRaw8<TYPE> raw[U];
+        const auto cast = [&](auto is_whole) {
+            // Whole: all U chunks are elements of a row, aligned.
+            constexpr bool kWhole = decltype(is_whole)::value;
+            MxRaw8<TYPE> raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int valid = (int)max((int64_t)0, min((int64_t)8, left - u * 256));
-            raw[u] = mx_load8<TYPE>(a.vec, src + u * 256, valid);
-        }
+            for (int u = 0; u < U; u++)
+                raw[u] = kWhole ? mx_load_whole<TYPE>(src + u * 256)
+                                : mx_load8<TYPE>(a.vec, src + u * 256,
+                                                 (int)max((int64_t)0,
+                                                          min((int64_t)8, left - u * 256)));
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (first + u >= chunks) break;  // the same for the whole warp
-            int shared;
-            const int valid = (int)max((int64_t)0, min((int64_t)8, left - u * 256));
-            const unsigned w =
-                mx_cast8<TYPE>(a, raw[u], valid, state,
-                               (uint64_t)row * a.cols + col0 + u * 256, shared, clamps, err);
-            const bool in = in_row && (col0 + u * 256) >> 5 < blocks;
-            if (in) *reinterpret_cast<unsigned *>(codes + u * 128) = w;
-            if ((lane & 3) == 0)
-                scales[u * 2 * kMxTileBytes] = in ? (uint8_t)(shared + 127) : (uint8_t)127;
-        }
+            for (int u = 0; u < U; u++) {
+                if (!kWhole && first + u >= chunks) break;  // the same for the whole warp
+                int shared;
+                const int valid =
+                    kWhole ? 8 : (int)max((int64_t)0, min((int64_t)8, left - u * 256));
+                const unsigned w =
+                    mx_cast8<TYPE>(a, raw[u], valid, state,
+                                   (uint64_t)row * a.cols + col0 + u * 256, shared, clamps, err);
+                const bool in = kWhole || (in_row && (col0 + u * 256) >> 5 < blocks);
+                if (in) *reinterpret_cast<unsigned *>(codes + u * 128) = w;
+                if ((lane & 3) == 0)
+                    scales[u * 2 * kMxTileBytes] = in ? (uint8_t)(shared + 127) : (uint8_t)127;
+            }
+        };
+        if (a.vec && in_row && (int64_t)(first + U) * 256 <= a.cols) cast(std::true_type{});
+        else cast(std::false_type{});
     }
     mx_finish(clamps, err, a.clamped, a.err);
 }
@@ -428,31 +483,15 @@ template <int TYPE> struct MxTile {
     static constexpr int kLoads = kMxTr * kCols / 8 / 256;     // groups of eight a thread loads
 };
 
-// One column's block of 32 to 16 bytes of codes.
+// One column's block of 32, the long way: 16 bytes of codes.
 template <int TYPE>
-__device__ __forceinline__ uint4 mx_cast_col(const MxCast &a, const typename MxSrc<TYPE>::V (&x)[32],
-                                             unsigned key, uint64_t state, uint64_t draw,
-                                             int &shared, unsigned &clamps, int &err) {
-    using S = MxSrc<TYPE>;
-    using V = typename S::V;
+__device__ __forceinline__ uint4 mx_slow_col(const MxCast &a,
+                                             const typename MxSrc<TYPE>::V (&x)[32],
+                                             uint64_t state, uint64_t draw, int &shared,
+                                             unsigned &clamps, int &err) {
+    using V = typename MxSrc<TYPE>::V;
     uint4 w;
     unsigned *wp = reinterpret_cast<unsigned *>(&w);
-    if (key < S::kInf && a.rm == DRIFT_NEAREST_EVEN) {
-        const MxFactor<V> f = mx_factor<TYPE>(key, a.headroom);
-        shared = f.shared;
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            V y[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = x[q * 8 + j];
-            if (a.clamped_t) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) clamps += fabs(y[j] * f.down) > (V)6;
-            }
-            wp[q] = key ? mx_fast8(y, f.down) : 0;
-        }
-        return w;
-    }
     V amax = (V)0;
 #pragma unroll
     for (int j = 0; j < 32; j++) amax = fmax(amax, mx_mag(x[j]));
@@ -489,14 +528,15 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
     const uint64_t state = a.rm == DRIFT_STOCHASTIC ? *a.state : 0;
 
     constexpr int kGroups = G::kCols / 8;  // groups of eight in a row of the tile
+    const bool whole = a.vec && r0 + kMxTr <= a.rows && c0 + G::kCols <= a.cols;
     MxRaw8<TYPE> raw[G::kLoads];
 #pragma unroll
     for (int i = 0; i < G::kLoads; i++) {
         const int at = i * 256 + tid, r = at / kGroups, c = at % kGroups * 8;
         const int valid = r0 + r < a.rows
                               ? (int)max((int64_t)0, min((int64_t)8, a.cols - c0 - c)) : 0;
-        raw[i] = mx_load8<TYPE>(
-            a.vec, static_cast<const T *>(a.src) + (r0 + r) * a.row_stride + c0 + c, valid);
+        const T *p = static_cast<const T *>(a.src) + (r0 + r) * a.row_stride + c0 + c;
+        raw[i] = whole ? mx_load_whole<TYPE>(p) : mx_load8<TYPE>(a.vec, p, valid);
     }
 #pragma unroll
     for (int i = 0; i < G::kLoads; i++) {
@@ -547,34 +587,72 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
     const int64_t row = r0 + b * 32;
     uint4 codes[G::kWide];
     int shared[G::kWide];
+    const uint64_t draw = a.draw_t + (uint64_t)row * a.cols + c0 + word * G::kWide;
     if constexpr (G::kWide == 2) {
         unsigned u[32], m = 0;
 #pragma unroll
         for (int j = 0; j < 32; j++) {
             u[j] = *reinterpret_cast<const unsigned *>(mx_smem + (b * 32 + j) * G::kLdBytes +
                                                        word * 4);
-            m = __vmaxu2(m, u[j] & 0x7fff7fffu);
+            m = S::max2(m, u[j]);
         }
+        const unsigned key[2] = {m & 0x7fffu, m >> 16 & 0x7fffu};
+        if (max(key[0], key[1]) < S::kInf && a.rm == DRIFT_NEAREST_EVEN) {
+            const MxFactor<V> f0 = mx_factor<TYPE>(key[0], a.headroom);
+            const MxFactor<V> f1 = mx_factor<TYPE>(key[1], a.headroom);
+            shared[0] = f0.shared, shared[1] = f1.shared;
+            unsigned *w0 = reinterpret_cast<unsigned *>(&codes[0]);
+            unsigned *w1 = reinterpret_cast<unsigned *>(&codes[1]);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            V x[32];
+            for (int q = 0; q < 4; q++) {
+                float y0[8], y1[8];
 #pragma unroll
-            for (int j = 0; j < 32; j++) x[j] = S::get_bits(u[j] >> h * 16 & 0xffffu);
-            codes[h] = mx_cast_col<TYPE>(a, x, m >> h * 16 & 0xffffu, state,
-                                         a.draw_t + (uint64_t)row * a.cols + c0 + word * 2 + h,
-                                         shared[h], clamps, err);
+                for (int j = 0; j < 8; j++)
+                    S::scaled2(u[q * 8 + j], f0.down, f1.down, y0[j], y1[j]);
+                if (a.clamped_t) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        clamps += (fabsf(y0[j]) > 6.0f) + (fabsf(y1[j]) > 6.0f);
+                }
+                w0[q] = key[0] ? mx_rn8(y0) : 0;
+                w1[q] = key[1] ? mx_rn8(y1) : 0;
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                V x[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) x[j] = S::get_bits(u[j] >> h * 16 & 0xffffu);
+                codes[h] = mx_slow_col<TYPE>(a, x, state, draw + h, shared[h], clamps, err);
+            }
         }
     } else {
         V x[32];
-        unsigned m = 0;
+        unsigned key = 0;
 #pragma unroll
         for (int j = 0; j < 32; j++) {
             x[j] = *reinterpret_cast<const T *>(mx_smem + (b * 32 + j) * G::kLdBytes +
                                                 word * sizeof(T));
-            m = max(m, S::key(x[j]));
+            key = max(key, S::key(x[j]));
         }
-        codes[0] = mx_cast_col<TYPE>(a, x, m, state, a.draw_t + (uint64_t)row * a.cols + c0 + word,
-                                     shared[0], clamps, err);
+        if (key < S::kInf && a.rm == DRIFT_NEAREST_EVEN) {
+            const MxFactor<V> f = mx_factor<TYPE>(key, a.headroom);
+            shared[0] = f.shared;
+            unsigned *wp = reinterpret_cast<unsigned *>(&codes[0]);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                V y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = x[q * 8 + j];
+                if (a.clamped_t) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) clamps += fabs(y[j] * f.down) > (V)6;
+                }
+                wp[q] = key ? mx_fast8(y, f.down) : 0;
+            }
+        } else {
+            codes[0] = mx_slow_col<TYPE>(a, x, state, draw, shared[0], clamps, err);
+        }
     }
     __syncthreads();
     const int64_t blocks = mx4_blocks(a.rows);

@@ -93,6 +93,12 @@ def test_exponents_clamp_and_subnormals_cast():
                       [3.0e38, -1e38, 1.0, 2e37] + [0.0] * 28], device="cuda")
     want, _ = oracle_rows(x.double().cpu().numpy(), p)
     assert (d.mx4_dequantize_dev(d.mx4_quantize_dev(p, x)).cpu().numpy() == want).all()
+    x = x.bfloat16()
+    want, _ = oracle_rows(x.double().cpu().numpy(), p)
+    assert (d.mx4_dequantize_dev(d.mx4_quantize_dev(p, x)).cpu().numpy() == want).all()
+    x = x.T.contiguous()  # the same rows as columns
+    got = d.mx4_dequantize_dev(d.mx4_quantize_dev(p, x, axis=0)).cpu().numpy()
+    assert (got.view(np.int64) == want.view(np.int64)).all()
     y = torch.tensor([[1e300, -1e290, 5e-324, 1.0] + [0.0] * 28, [1e-300] * 32], device="cuda",
                      dtype=torch.float64)
     want, _ = oracle_rows(y.cpu().numpy(), p)
