@@ -36,16 +36,21 @@ __global__ void __launch_bounds__(256) fill_bias_kernel(T *C, int64_t stride, in
         C[i / cols * stride + i % cols] = T(bias ? bias[i % cols] : 0.0f);
 }
 
-// How many CTAs share a thin tile's contraction: the count, up to a portable
-// cluster's eight, with the least rounds of CTAs times stages a CTA, a round
-// costing some four stages besides.
-static int thin_split(int64_t tiles, int k_stages, int sms) {
+// Estimated tenths of a microsecond, from products of 129x2048x2048 to
+// 2048x4096x4096 measured both ways (within a fifth of either): a wave of pair
+// tiles takes 6.6 a stage and 35, a wave of thin CTAs 5 a stage and 65.
+static int64_t pair_cost(int64_t m, int64_t n, int64_t stages, int sms) {
+    const int64_t tiles = (m + tc::kTile - 1) / tc::kTile * ((n + tc::kTile - 1) / tc::kTile);
+    return (tiles + sms / 2 - 1) / (sms / 2) * (66 * stages + 350);
+}
+static int64_t thin_cost(int64_t tiles, int64_t stages, int split, int sms) {
+    return (tiles * split + sms - 1) / sms * (50 * ((stages + split - 1) / split) + 650);
+}
+// How many CTAs, up to a portable cluster's eight, share a thin tile's contraction.
+static int thin_split(int64_t tiles, int64_t stages, int sms) {
     int best = 1;
-    int64_t least = INT64_MAX;
-    for (int s = 1; s <= 8 && s <= k_stages; s++) {
-        const int64_t cost = (tiles * s + sms - 1) / sms * ((k_stages + s - 1) / s + 4);
-        if (cost < least) least = cost, best = s;
-    }
+    for (int s = 2; s <= 8 && s <= stages; s++)
+        if (thin_cost(tiles, stages, s, sms) < thin_cost(tiles, stages, best, sms)) best = s;
     return best;
 }
 
@@ -75,10 +80,13 @@ static int gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C,
         fill_bias_kernel<<<sm_count() * 2, 256, 0, st>>>(C, c_stride, a->rows, b->rows, bias);
         return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA;
     }
-    // Pair tiles that do not fill the pairs of SMs once leave the product to the
-    // thin kernel's smaller tiles and shared contractions.
-    const int64_t pairs = (a->rows + tc::kTile - 1) / tc::kTile * ((b->rows + tc::kTile - 1) / tc::kTile);
-    if (a->rows <= 128 || pairs < sm_count() / 2) {
+    // Up to 128 rows the thin kernel wastes no lanes; beyond, few pair tiles leave SMs
+    // idle that its smaller tiles and shared contractions reach.
+    const int sms = sm_count();
+    const int64_t stages = (a->cols + 255) / 256;
+    const int64_t thin_tiles = (a->rows + 127) / 128 * ((b->rows + 127) / 128);
+    if (a->rows <= 128 || thin_cost(thin_tiles, stages, thin_split(thin_tiles, stages, sms), sms) <
+                              pair_cost(a->rows, b->rows, stages, sms)) {
         if (a->rows <= 16) return gemm_thin<16>(a, b, bias, C, c_stride, d_err, st);
         if (a->rows <= 32) return gemm_thin<32>(a, b, bias, C, c_stride, d_err, st);
         if (a->rows <= 64) return gemm_thin<64>(a, b, bias, C, c_stride, d_err, st);
@@ -95,7 +103,7 @@ static int gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, T *C,
     args.err = d_err;
     const StoreEpi<T> epi{C, c_stride, a->rows, b->rows, bias, nullptr, 1.0f,
                           rows_aligned(C, c_stride)};
-    return tc::launch<tc::KIND_MX4, false, false, false>(args, epi, sm_count(), st);
+    return tc::launch<tc::KIND_MX4, false, false, false>(args, epi, sms, st);
 }
 
 int launch_mx4_gemm(const drift_mx4 *a, const drift_mx4 *b, const float *bias, int type, void *C,

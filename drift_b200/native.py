@@ -202,15 +202,15 @@ class Mx4:
 
 
 def _mx4_policy(p: NumericPolicy):
-    """The policy as it crosses the ABI, checked once and kept with the (frozen)
-    policy."""
+    """The policy as it crosses the ABI and its input rounding, checked once and
+    kept with the (frozen) policy."""
     c = p.__dict__.get("_mx4")
     if c is None:
         if p.scaling != Scaling.MX_BLOCK or p.scale_block != 32 or \
                 Formats.E2M1 not in (p.input_format, p.grad_format):
             raise ValueError("the packed cast needs a policy with e2m1 elements and MX blocks of "
                              "32")
-        c = p.__dict__["_mx4"] = p.to_c()
+        c = p.__dict__["_mx4"] = (p.to_c(), int(p.input_rounding))
     return c
 
 
@@ -226,16 +226,20 @@ def mx4_quantize_dev(p: NumericPolicy, src, rm: Optional[Rounding] = None, *,
     input rounding; stochastic rounding needs d_rng_state (int64, one element),
     which is advanced by src.numel() draws a direction. Clamp counts are
     added to d_clamped (blocks along rows) and d_clamped_t (down columns)."""
-    pc = _mx4_policy(p)
-    if axis not in (0, 1, None):
+    pc, rounding = _mx4_policy(p)
+    if axis != 1 and axis is not None and axis != 0:
         raise ValueError("axis must be 0, 1 or None")
     if src.dim() != 2:
         raise ValueError("src: expected a matrix")
     call = _Call(src, ctx)
     t = _type_of(src.dtype, "src")
-    rng = call.ptr(d_rng_state, "d_rng_state", torch.int64, 1)
-    cl = call.ptr(d_clamped, "d_clamped", torch.int64, 1)
-    cl_t = call.ptr(d_clamped_t, "d_clamped_t", torch.int64, 1)
+    rng = cl = cl_t = None
+    if d_rng_state is not None:
+        rng = call.ptr(d_rng_state, "d_rng_state", torch.int64, 1)
+    if d_clamped is not None:
+        cl = call.ptr(d_clamped, "d_clamped", torch.int64, 1)
+    if d_clamped_t is not None:
+        cl_t = call.ptr(d_clamped_t, "d_clamped_t", torch.int64, 1)
     rows, cols = src.shape
     stride, step = src.stride()
     if (cols > 1 and step != 1) or (rows > 1 and stride < cols):
@@ -246,7 +250,7 @@ def mx4_quantize_dev(p: NumericPolicy, src, rm: Optional[Rounding] = None, *,
     a, b = (row.c.codes, row.c.scales) if row is not None else (None, None)
     c, d = (col.c.codes, col.c.scales) if col is not None else (None, None)
     _lib.check(_LIB.drift_mx4_quantize_dev(
-        call.handle, pc, p.input_rounding if rm is None else Rounding(rm), t, src.data_ptr(), rows,
+        call.handle, pc, rounding if rm is None else int(Rounding(rm)), t, src.data_ptr(), rows,
         cols, stride if rows > 1 else cols, a, b, c, d, rng, cl, cl_t, call.stream))
     return (row, col) if axis is None else row if axis == 1 else col
 
