@@ -307,7 +307,7 @@ struct MxCast {
     const void *src;
     int64_t rows, cols, row_stride;
     int headroom, rm;
-    bool vec;                          // rows start 16-byte aligned
+    bool vec, wide;                    // rows start 16-byte, 32-byte aligned
     uint8_t *codes, *scales;           // blocks along rows
     uint8_t *codes_t, *scales_t;       // blocks down columns: the transpose, packed
     uint64_t draw_t;                   // first draw of the transposed cast
@@ -316,13 +316,23 @@ struct MxCast {
     int *err;
 };
 
-// Eight elements at p, 16-byte aligned.
+// Eight elements at p, 16-byte aligned; `wide`: 32-byte aligned, so that the wider
+// types' lanes take whole sectors an instruction.
 template <int TYPE>
-__device__ __forceinline__ MxRaw8<TYPE> mx_load_whole(const typename MxSrc<TYPE>::T *p) {
+__device__ __forceinline__ MxRaw8<TYPE> mx_load_whole(const typename MxSrc<TYPE>::T *p, bool wide) {
     MxRaw8<TYPE> r;
+    constexpr int kVecs = MxRaw8<TYPE>::kVecs;
+    if (kVecs > 1 && wide) {
 #pragma unroll
-    for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++)
-        r.w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
+        for (int j = 0; j + 1 < kVecs; j += 2)
+            asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                : "=r"(r.w[j].x), "=r"(r.w[j].y), "=r"(r.w[j].z), "=r"(r.w[j].w),
+                  "=r"(r.w[j + 1].x), "=r"(r.w[j + 1].y), "=r"(r.w[j + 1].z), "=r"(r.w[j + 1].w)
+                : "l"(reinterpret_cast<const uint4 *>(p) + j));
+    } else {
+#pragma unroll
+        for (int j = 0; j < kVecs; j++) r.w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
+    }
     return r;
 }
 // `valid` elements at p, the rest zeros; `vec`: p is 16-byte aligned.
@@ -330,7 +340,7 @@ template <int TYPE>
 __device__ __forceinline__ MxRaw8<TYPE> mx_load8(bool vec, const typename MxSrc<TYPE>::T *p,
                                                  int valid) {
     using T = typename MxSrc<TYPE>::T;
-    if (vec && valid == 8) return mx_load_whole<TYPE>(p);
+    if (vec && valid == 8) return mx_load_whole<TYPE>(p, false);
     MxRaw8<TYPE> r;
     T *t = reinterpret_cast<T *>(r.w);
 #pragma unroll
@@ -442,7 +452,7 @@ __global__ void __launch_bounds__(256) mx4_rows_kernel(const __grid_constant__ M
             MxRaw8<TYPE> raw[U];
 #pragma unroll
             for (int u = 0; u < U; u++)
-                raw[u] = kWhole ? mx_load_whole<TYPE>(src + u * 256)
+                raw[u] = kWhole ? mx_load_whole<TYPE>(src + u * 256, a.wide)
                                 : mx_load8<TYPE>(a.vec, src + u * 256,
                                                  (int)max((int64_t)0,
                                                           min((int64_t)8, left - u * 256)));
@@ -536,7 +546,7 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
         const int valid = r0 + r < a.rows
                               ? (int)max((int64_t)0, min((int64_t)8, a.cols - c0 - c)) : 0;
         const T *p = static_cast<const T *>(a.src) + (r0 + r) * a.row_stride + c0 + c;
-        raw[i] = whole ? mx_load_whole<TYPE>(p) : mx_load8<TYPE>(a.vec, p, valid);
+        raw[i] = whole ? mx_load_whole<TYPE>(p, a.wide) : mx_load8<TYPE>(a.vec, p, valid);
     }
 #pragma unroll
     for (int i = 0; i < G::kLoads; i++) {
@@ -689,16 +699,20 @@ __global__ void mx4_advance_kernel(uint64_t *state, uint64_t draws) {
 
 template <int TYPE>
 static int launch_cast(const MxCast &a, cudaStream_t st) {
+    using T = typename MxSrc<TYPE>::T;
     if (!a.codes_t) {
         const uint32_t chunks = (uint32_t)(mx4_k_tiles(a.cols) / 2);
         const uint32_t rows = (uint32_t)(mx4_row_tiles(a.rows) * 128);
         const uint32_t sms = (uint32_t)sm_count();
-        // Four chunks a warp, where the rows have them, once that still leaves every
-        // SM two CTAs; else a warp a chunk.
-        if (chunks >= 4 && rows * (uint64_t)((chunks + 3) / 4) >= sms * 2 * 8) {
-            const uint32_t per_row = (chunks + 3) / 4, items = rows * per_row;
+        // Four chunks a warp (two of doubles, whose loads fill as many registers), where
+        // the rows have them, once that still leaves every SM two CTAs; else a warp a
+        // chunk.
+        constexpr uint32_t kU = sizeof(T) == 8 ? 2 : 4;
+        if (chunks >= kU && rows * (uint64_t)((chunks + kU - 1) / kU) >= sms * 2 * 8) {
+            const uint32_t per_row = (chunks + kU - 1) / kU, items = rows * per_row;
             const uint32_t grid = std::min<uint32_t>((items + 7) / 8, sms * 8);
-            return launch_pdl(mx4_rows_kernel<TYPE, 4>, dim3(grid), 256, 0, st, 0, a, per_row, items);
+            return launch_pdl(mx4_rows_kernel<TYPE, kU>, dim3(grid), 256, 0, st, 0, a, per_row,
+                              items);
         } else {
             const uint32_t items = rows * chunks;
             return launch_pdl(mx4_rows_kernel<TYPE, 1>,
@@ -727,7 +741,8 @@ int launch_mx4_quantize(int headroom, int rm, int type, const void *src, int64_t
     a.src = src;
     a.rows = rows, a.cols = cols, a.row_stride = row_stride;
     a.headroom = headroom, a.rm = rm;
-    a.vec = reinterpret_cast<uintptr_t>(src) % 16 == 0 && row_stride * size[type] % 16 == 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src) | (uintptr_t)(row_stride * size[type]);
+    a.vec = at % 16 == 0, a.wide = at % 32 == 0;
     a.codes = codes, a.scales = scales, a.codes_t = codes_t, a.scales_t = scales_t;
     a.draw_t = codes ? (uint64_t)rows * cols : 0;
     a.state = d_state;
@@ -789,9 +804,20 @@ __global__ void __launch_bounds__(256) mx4_values_kernel(const uint8_t *codes,
             }
             T *p = dst + row * stride + col;
             if (vec && col + 8 <= cols) {
+                const uint4 *w = reinterpret_cast<const uint4 *>(v);
+                if constexpr (sizeof(T) == 2) {
+                    *reinterpret_cast<uint4 *>(p) = w[0];
+                } else {
+                    // Whole sectors an instruction (vec: 32-byte aligned).
 #pragma unroll
-                for (int j = 0; j < (int)sizeof(T) / 2; j++)
-                    reinterpret_cast<uint4 *>(p)[j] = reinterpret_cast<const uint4 *>(v)[j];
+                    for (int j = 0; j < (int)sizeof(T) / 4; j++)
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                                         reinterpret_cast<uint4 *>(p) + 2 * j),
+                                     "r"(w[2 * j].x), "r"(w[2 * j].y), "r"(w[2 * j].z),
+                                     "r"(w[2 * j].w), "r"(w[2 * j + 1].x), "r"(w[2 * j + 1].y),
+                                     "r"(w[2 * j + 1].z), "r"(w[2 * j + 1].w)
+                                     : "memory");
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
@@ -805,8 +831,8 @@ int launch_mx4_dequantize(const drift_mx4 *q, int type, void *dst, int64_t strid
                           cudaStream_t st) {
     static const int size[4] = {8, 4, 2, 2};
     const uint32_t groups = (uint32_t)((q->cols + 7) / 8);
-    const bool vec =
-        reinterpret_cast<uintptr_t>(dst) % 16 == 0 && stride * size[type] % 16 == 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(dst) | (uintptr_t)(stride * size[type]);
+    const bool vec = at % (size[type] == 2 ? 16 : 32) == 0;
     const dim3 grid((groups + 255) / 256, (unsigned)std::min<int64_t>(q->rows, 65535));
     const auto run = [&](auto *p) {
         return launch_pdl(mx4_values_kernel<std::remove_pointer_t<decltype(p)>>, grid, 256, 0, st, 0,

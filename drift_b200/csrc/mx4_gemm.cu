@@ -43,14 +43,16 @@ static int64_t pair_cost(int64_t m, int64_t n, int64_t stages, int sms) {
     const int64_t tiles = (m + tc::kTile - 1) / tc::kTile * ((n + tc::kTile - 1) / tc::kTile);
     return (tiles + sms / 2 - 1) / (sms / 2) * (66 * stages + 350);
 }
-static int64_t thin_cost(int64_t tiles, int64_t stages, int split, int sms) {
-    return (tiles * split + sms - 1) / sms * (50 * ((stages + split - 1) / split) + 650);
+static int64_t thin_cost(int64_t tiles, int64_t stages, int split, int slots) {
+    return (tiles * split + slots - 1) / slots * (50 * ((stages + split - 1) / split) + 650);
 }
-// How many CTAs, up to a portable cluster's eight, share a thin tile's contraction.
-static int thin_split(int64_t tiles, int64_t stages, int sms) {
+// How many CTAs share a thin tile's contraction: up to four, or a portable
+// cluster's eight where tiles are few. (Sixteen clusters of eight did not all fit
+// the GPU at once: 64 x 2048 x 2048 took 9.8 us with them and 4.7 with fours.)
+static int thin_split(int64_t tiles, int64_t stages, int slots) {
     int best = 1;
-    for (int s = 2; s <= 8 && s <= stages; s++)
-        if (thin_cost(tiles, stages, s, sms) < thin_cost(tiles, stages, best, sms)) best = s;
+    for (int s = 2; s <= (tiles <= 9 ? 8 : 4) && s <= stages; s++)
+        if (thin_cost(tiles, stages, s, slots) < thin_cost(tiles, stages, best, slots)) best = s;
     return best;
 }
 
@@ -69,7 +71,8 @@ static int gemm_thin(const drift_mx4 *a, const drift_mx4 *b, const float *bias, 
     args.vec = rows_aligned(C, c_stride);
     args.err = d_err;
     const int t_tiles = (int)((a->rows + NT - 1) / NT);
-    const int split = thin_split((int64_t)args.w_tiles * t_tiles, args.k_stages, sm_count());
+    const int split = thin_split((int64_t)args.w_tiles * t_tiles, args.k_stages,
+                                 sm_count() * thin::Shape<NT>::per_sm);
     return thin::launch<NT, T>(args, t_tiles, split, st);
 }
 

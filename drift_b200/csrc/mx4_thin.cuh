@@ -21,7 +21,10 @@ constexpr int kScaleCol = 128;
 
 template <int NT> struct Shape {
     static constexpr int stage = 16384 + NT * 128 + 2048;
-    static constexpr int stages = NT <= 32 ? 8 : NT == 64 ? 7 : 6;
+    // Up to 32 tokens two CTAs share an SM: one's scale copies and start fill the
+    // other's waits.
+    static constexpr int per_sm = NT <= 32 ? 2 : 1;
+    static constexpr int stages = NT == 16 ? 5 : NT == 32 ? 4 : NT == 64 ? 7 : 6;
     static constexpr int smem = stage * stages + 1024;
     static_assert(NT * 512 <= stage * stages, "the partial tile reuses the stages");
     static_assert(NT <= kScaleCol && kScaleCol + stages * 16 <= kTmemCols, "TMEM columns");
@@ -78,7 +81,7 @@ template <class T> __device__ __forceinline__ void store4(T *p, const float (&y)
 }
 
 template <int NT, class T>
-__global__ void __launch_bounds__(kThreads, 1) thin_kernel(const __grid_constant__ Args args) {
+__global__ void __launch_bounds__(kThreads, Shape<NT>::per_sm) thin_kernel(const __grid_constant__ Args args) {
     using S = Shape<NT>;
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full[S::stages], empty[S::stages], acc_full;
