@@ -362,11 +362,10 @@ __global__ void __launch_bounds__(256) xent_row_kernel(float *logits, int splits
     }
 }
 
-// The mean of the rows' losses and the inverse count, in a fixed order.
-__global__ void __launch_bounds__(1024) xent_rows_mean_kernel(const float *row_loss, int64_t T,
-                                                              XentRows x, float *mean) {
-    pdl_trigger();
-    pdl_wait();
+// The mean of the rows' losses, and 1 / their number, by one CTA in a fixed order.
+// Returns the latter to every thread.
+__device__ __forceinline__ float rows_mean(const float *row_loss, int64_t T, const XentRows &x,
+                                           float *mean, float *inv) {
     __shared__ float sl[32];
     __shared__ int sc[32];
     float sum = 0.0f;
@@ -381,11 +380,43 @@ __global__ void __launch_bounds__(1024) xent_rows_mean_kernel(const float *row_l
     count = (int)__reduce_add_sync(0xffffffffu, count);
     if ((threadIdx.x & 31) == 0) sl[threadIdx.x >> 5] = sum, sc[threadIdx.x >> 5] = count;
     __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < (int)blockDim.x / 32; i++) sum += sl[i], count += sc[i];
+    sum = 0.0f, count = 0;
+    for (int i = 0; i < (int)blockDim.x / 32; i++) sum += sl[i], count += sc[i];
     const float c = (float)max(count, 1);
-    mean[0] = sum / c;
-    mean[1] = 1.0f / c;
+    if (threadIdx.x == 0 && mean) {
+        *mean = sum / c;
+        *inv = 1.0f / c;
+    }
+    return 1.0f / c;
+}
+__global__ void __launch_bounds__(1024) xent_mean_kernel(const float *row_loss, int64_t T,
+                                                         XentRows x, float *mean, float *inv) {
+    pdl_trigger();
+    pdl_wait();
+    rows_mean(row_loss, T, x, mean, inv);
+}
+
+// db of the kept logits' d, and the mean: every CTA counts the rows for itself, the
+// first one writes the mean and the inverse count.
+__global__ void __launch_bounds__(256) xent_mean_db_kernel(const float *row_loss, int64_t T,
+                                                           XentRows x, float *mean, float *inv,
+                                                           const float *d, int64_t n, int64_t ld,
+                                                           float *db) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ float sh[8][33];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t v = (int64_t)blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (v < n) {
+#pragma unroll 4
+        for (int64_t i = slice; i < T; i += 8) s += d[i * ld + v];
+    }
+    sh[slice][lane] = s;
+    const float k = rows_mean(row_loss, T, x, blockIdx.x == 0 ? mean : nullptr, inv);  // syncs
+    if (slice || v >= n) return;
+    for (int i = 1; i < 8; i++) s += sh[i][lane];
+    db[v] = s * k;
 }
 
 // ------------------------------------------------------------------ plans
@@ -447,7 +478,7 @@ static GradPlan grad_plan(const drift_xent *op) {
 // so rows longer than 2^15 (some 20 us) are left to the other way.
 struct KeptPlan {
     bool use;
-    int64_t ld, part, logits, d, loss, acc, acc_part, acc_ld, bytes;
+    int64_t ld, part, logits, d, loss, inv, acc, acc_part, acc_ld, bytes;
     int splits, dx_splits;
 };
 static KeptPlan kept_plan(const drift_xent *op) {
@@ -466,7 +497,8 @@ static KeptPlan kept_plan(const drift_xent *op) {
     p.loss = p.d + up(p.part * 2, 256);
     p.acc_ld = up(op->depth, 4);
     p.acc_part = t * p.acc_ld;
-    p.acc = p.loss + up(t * 4, 256);
+    p.inv = p.loss + up(t * 4, 256);
+    p.acc = p.inv + 256;
     p.bytes = p.acc + (p.dx_splits > 1 ? up(p.dx_splits * p.acc_part * 4, 256) : 0) + 256;
     return p;
 }
@@ -477,17 +509,17 @@ int64_t xent_workspace(const drift_xent *op, int mode) {
         if (k.use) return k.bytes;
     }
     const int64_t f = forward_plan(op).bytes;
-    return mode ? std::max(f, grad_plan(op).bytes + (mode == 2 ? up(op->tokens * 4, 256) : 0)) : f;
+    return mode ? std::max(f, grad_plan(op).bytes) + (mode == 2 ? up(op->tokens * 4, 256) + 256 : 0) : f;
 }
 
 static XentRows rows_of(const drift_xent *op) {
     return XentRows{op->targets, op->target_bits == 64, op->ignore_index, op->vocab};
 }
 
-static int rows_mean(const float *row_loss, int64_t n, const XentRows &rows, float *mean,
-                     cudaStream_t st) {
-    return launch_pdl(xent_rows_mean_kernel, dim3(1), n <= 256 ? 256 : 1024, 0, st, 0, row_loss, n,
-                      rows, mean);
+static int launch_mean(const float *row_loss, int64_t n, const XentRows &rows, float *mean,
+                       float *inv, cudaStream_t st) {
+    return launch_pdl(xent_mean_kernel, dim3(1), n <= 256 ? 256 : 1024, 0, st, 0, row_loss, n, rows,
+                      mean, inv);
 }
 
 static int done() { return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA; }
@@ -507,8 +539,8 @@ static bool logit_args(tc::Args &a, const drift_xent *op, int64_t v0, int64_t n,
 }
 
 template <bool BF16>
-static int forward(const drift_xent *op, float *loss, float *lse, float *mean, char *ws, int *err,
-                   cudaStream_t st) {
+static int forward(const drift_xent *op, float *loss, float *lse, float *mean, float *inv, char *ws,
+                   int *err, cudaStream_t st) {
     const ForwardPlan p = forward_plan(op);
     const int64_t n_t = op->tokens;
     const XentRows rows = rows_of(op);
@@ -533,7 +565,7 @@ static int forward(const drift_xent *op, float *loss, float *lse, float *mean, c
                         row_loss, lse, err);
         if (rc) return rc;
     }
-    return mean ? rows_mean(row_loss, n_t, rows, mean, st) : DRIFT_OK;
+    return mean ? launch_mean(row_loss, n_t, rows, mean, inv, st) : DRIFT_OK;
 }
 
 template <class T, bool BF16>
@@ -631,6 +663,7 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
     float *row_loss = reinterpret_cast<float *>(ws + p.loss);
     float *acc = reinterpret_cast<float *>(ws + p.acc);
     T *d = reinterpret_cast<T *>(ws + p.d);
+    float *inv = reinterpret_cast<float *>(ws + p.inv);
     const float scale = BF16 ? 1.0f : 32768.0f, beta = 1.0f / scale;
     tc::Args a;
     if (!logit_args(a, op, 0, n, BF16, err)) return DRIFT_ECUDA;
@@ -641,10 +674,16 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
     rc = launch_pdl(xent_row_kernel<T>, dim3((unsigned)n_t), 256, 0, st, 0, logits, a.splits, p.part,
                     p.ld, n, op->bias, rows, d, scale, db != nullptr, row_loss, (float *)nullptr,
                     err);
-    if (!rc) rc = rows_mean(row_loss, n_t, rows, mean, st);
-    if (!rc && db)
-        rc = launch_pdl(xent_colsum_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, st, 0, logits,
-                        n_t, n, p.ld, mean + 1, db);
+    // Few rows: one kernel for the mean and db, whose CTAs all read the targets.
+    if (!rc && db && n_t <= 4096) {
+        rc = launch_pdl(xent_mean_db_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, st, 0,
+                        row_loss, n_t, rows, mean, inv, logits, n, p.ld, db);
+    } else {
+        if (!rc) rc = launch_mean(row_loss, n_t, rows, mean, inv, st);
+        if (!rc && db)
+            rc = launch_pdl(xent_colsum_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, st, 0,
+                            logits, n_t, n, p.ld, inv, db);
+    }
     if (!rc && dx) {
         if (!tc::encode_16(&a.a, BF16, d, n_t, n, p.ld, true) ||
             !tc::encode_16(&a.b, BF16, op->w, dep, n, op->w_stride, false))
@@ -653,14 +692,14 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
         a.splits = std::min(p.dx_splits, a.k_stages), a.run = kGradRun;
         if (a.splits == 1) {
             const StoreEpi<T> epi{dx,      dx_stride, n_t,  dep,
-                                  nullptr, mean + 1,  beta, rows_aligned(dx, dx_stride)};
+                                  nullptr, inv,       beta, rows_aligned(dx, dx_stride)};
             rc = tc::launch<tc::KIND_16, BF16, false, true>(a, epi, sm_count(), st);
         } else {
             const PartEpi epi{acc, p.acc_part, p.acc_ld, n_t, dep, false};
             rc = tc::launch<tc::KIND_16, BF16, false, true>(a, epi, sm_count(), st);
             if (!rc)
                 rc = launch_pdl(xent_dx_kernel<T>, dim3(sm_count() * 8), 256, 0, st, 0, acc, a.splits,
-                                p.acc_part, p.acc_ld, dx, n_t, dep, dx_stride, mean + 1, beta);
+                                p.acc_part, p.acc_ld, dx, n_t, dep, dx_stride, inv, beta);
         }
     }
     if (!rc && dw) {
@@ -670,7 +709,7 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
         a.m_tiles = tiles(n), a.n_tiles = tiles(dep), a.k_stages = stages(n_t);
         a.splits = 1, a.run = kGradRun;
         const StoreEpi<T> epi{dw,      dw_stride, n,    dep,
-                              nullptr, mean + 1,  beta, rows_aligned(dw, dw_stride)};
+                              nullptr, inv,       beta, rows_aligned(dw, dw_stride)};
         rc = tc::launch<tc::KIND_16, BF16, true, true>(a, epi, sm_count(), st);
     }
     return rc;
@@ -686,18 +725,19 @@ int launch_xent_mean(const drift_xent *op, float *mean, void *dx, int64_t dx_str
                                                     err, st)
                    : mean_kept<__half, false>(op, k, mean, (__half *)dx, dx_stride, (__half *)dw,
                                               dw_stride, db, (char *)ws, err, st);
-    float *lse = reinterpret_cast<float *>(
-        (char *)ws + std::max(forward_plan(op).bytes, grad_plan(op).bytes));
-    const int rc = launch_xent(op, nullptr, lse, mean, ws, err, st);
+    char *more = (char *)ws + std::max(forward_plan(op).bytes, grad_plan(op).bytes);
+    float *inv = reinterpret_cast<float *>(more), *lse = reinterpret_cast<float *>(more + 256);
+    const int rc = op->type == DRIFT_T_BF16
+                       ? forward<true>(op, nullptr, lse, mean, inv, (char *)ws, err, st)
+                       : forward<false>(op, nullptr, lse, mean, inv, (char *)ws, err, st);
     return rc ? rc
-              : launch_xent_grad(op, lse, mean + 1, 0, dx, dx_stride, dw, dw_stride, db, ws, err,
-                                 st);
+              : launch_xent_grad(op, lse, inv, 0, dx, dx_stride, dw, dw_stride, db, ws, err, st);
 }
 
 int launch_xent(const drift_xent *op, float *loss, float *lse, float *mean, void *ws, int *err,
                 cudaStream_t st) {
-    return op->type == DRIFT_T_BF16 ? forward<true>(op, loss, lse, mean, (char *)ws, err, st)
-                                    : forward<false>(op, loss, lse, mean, (char *)ws, err, st);
+    return op->type == DRIFT_T_BF16 ? forward<true>(op, loss, lse, mean, mean + 1, (char *)ws, err, st)
+                                    : forward<false>(op, loss, lse, mean, mean + 1, (char *)ws, err, st);
 }
 
 int launch_xent_grad(const drift_xent *op, const float *lse, const float *g, int64_t g_stride,

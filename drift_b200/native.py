@@ -401,13 +401,13 @@ def linear_xent_mean_dev(x, w, targets, *, bias=None, ignore_index: int = -100, 
     vocabulary at a time."""
     call = _Call(x, ctx)
     op, keep = _xent_op(call, x, w, targets, bias, ignore_index)
-    mean = torch.empty(2, dtype=torch.float32, device=call.device)
+    mean = torch.empty((), dtype=torch.float32, device=call.device)
     ws = _xent_ws(call, op, 2)
     dx, dw, db, (px, pw, pb) = _xent_outputs(call, op, x, True, True, bias is not None)
     _lib.check(_LIB.drift_linear_xent_mean_dev(
         call.handle, op, mean.data_ptr(), px, op.depth, pw, op.depth, pb, ws.data_ptr(),
         ws.numel(), call.stream))
-    return mean[0], dx, dw, db
+    return mean, dx, dw, db
 
 
 # ------------------------------------------------------------------ AdamW

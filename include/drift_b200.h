@@ -621,7 +621,8 @@ DRIFT_API int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, c
                                int64_t dx_stride, void *d_dw, int64_t dw_stride, float *d_db,
                                void *d_ws, int64_t ws_bytes, void *stream);
 
-/* Both in one call: d_mean as drift_linear_xent_dev's, and that mean's gradients.
+/* Both in one call: *d_mean, one float, and that mean's gradients (the mean as
+ * drift_linear_xent_dev's).
  * Up to 2^24 logits in rows of up to 2^15 are kept in the workspace in between;
  * beyond, they are computed again. */
 DRIFT_API int drift_linear_xent_mean_dev(drift_ctx *ctx, const drift_xent *op, float *d_mean,
