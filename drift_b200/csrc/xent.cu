@@ -558,7 +558,7 @@ static int forward(const drift_xent *op, float *loss, float *lse, float *mean, f
         int rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
         if (rc) return rc;
         const int n_parts = (int)((n + 127) / 128);
-        const bool few = n_t < 1024;
+        const bool few = n_t < 256;
         rc = launch_pdl(few ? xent_join_kernel<1> : xent_join_kernel<32>,
                         dim3((unsigned)(few ? n_t : (n_t + 31) / 32)), few ? 128 : 1024, 0, st, 0,
                         parts, n_parts, n_t, run, v0 == 0, v0 + n == op->vocab, target, rows,
