@@ -4,6 +4,7 @@ Each policy differs from a named parent in one field (Policies.java:14-16).
 """
 from __future__ import annotations
 
+import functools
 from typing import Dict
 
 from .fmt import Formats, Rounding
@@ -71,8 +72,14 @@ def main_sweep() -> Dict[str, NumericPolicy]:
     return {k: v for k, v in all_policies().items() if k not in FOLLOW_UP}
 
 
+@functools.lru_cache(maxsize=None)
+def _registry() -> Dict[str, NumericPolicy]:
+    """all_policies(), built once: the policies are immutable."""
+    return all_policies()
+
+
 def by_name(name: str) -> NumericPolicy:
-    p = all_policies().get(name)
+    p = _registry().get(name)
     if p is None:
-        raise ValueError(f"unknown policy {name}; known: {list(all_policies())}")
+        raise ValueError(f"unknown policy {name}; known: {list(_registry())}")
     return p
