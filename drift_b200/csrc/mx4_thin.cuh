@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(kThreads, Shape<NT>::per_sm) thin_kernel(const
         }
         __syncwarp();
     } else {
-        ok = __all_sync(0xffffffffu, tc::wait(&acc_full, 0));
+        ok = __all_sync(0xffffffffu,
+                        tc::wait(&acc_full, 0, (long long)(k1 - k0) * tc::kRoundsPerStage));
         tc::fence_after();
         const int64_t r = (int64_t)tw * 128 + warp * 32 + lane;
         const float b = args.bias && r < args.rows ? __ldg(args.bias + r) : 0.0f;

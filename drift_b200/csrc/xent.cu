@@ -315,14 +315,37 @@ __global__ void __launch_bounds__(256) xent_dx_kernel(const float *acc, int spli
     }
 }
 
+// The x that dW = d^T x reads: an ignored row's d is 0, but 0 times an Inf or NaN
+// that a padded position may hold is not, so those rows are copied as zeros. The
+// copy is 4 bytes an element of x beside 2 V operations.
+struct CopyRows {
+    const uint4 *from;  // null: no copy
+    uint4 *to;
+    int64_t from_ld, to_ld, units;  // in units of 16 bytes
+    __device__ __forceinline__ void copy_row(int64_t row, bool on) const {
+        if (!from) return;
+        const uint4 *f = from + row * from_ld;
+        uint4 *t = to + row * to_ld;
+        for (int64_t i = threadIdx.x; i < units; i += blockDim.x)
+            t[i] = on ? __ldg(f + i) : make_uint4(0, 0, 0, 0);
+    }
+};
+__global__ void __launch_bounds__(128) xent_copy_kernel(CopyRows xs, XentRows x) {
+    pdl_trigger();
+    pdl_wait();
+    bool bad = false;
+    xs.copy_row(blockIdx.x, x.at(blockIdx.x, bad) >= 0);
+}
+
 // The mean loss with its gradients where all logits fit the workspace at once: a
 // CTA takes a row, sums the parts of its logits, and replaces them by d, both in
 // fp32 (for db) and in the inputs' type times `scale`. Its loss goes to `row_loss`.
+// With `xs` the CTA also copies its row of x, an ignored one as zeros (copy_row).
 template <class T>
 __global__ void __launch_bounds__(256) xent_row_kernel(float *logits, int splits, int64_t part,
                                                        int64_t ld, int64_t n, const float *bias,
                                                        XentRows x, T *d, float scale, bool keep,
-                                                       float *row_loss, float *lse, int *err) {
+                                                       float *row_loss, CopyRows xs, int *err) {
     pdl_trigger();
     pdl_wait();
     __shared__ Stat sh[8];
@@ -358,8 +381,8 @@ __global__ void __launch_bounds__(256) xent_row_kernel(float *logits, int splits
     if (threadIdx.x == 0) {
         if (bad) atomicOr(err, DEV_ERR_INDEX);
         row_loss[row] = t >= 0 ? z - target : 0.0f;
-        if (lse) lse[row] = z;
     }
+    xs.copy_row(row, t >= 0);
 }
 
 // The mean of the rows' losses, and 1 / their number, by one CTA in a fixed order.
@@ -445,7 +468,7 @@ static ForwardPlan forward_plan(const drift_xent *op) {
 // dx that each piece costs (8 bytes an element of dx) is small beside the
 // piece's products, small enough to be no burden beside W.
 struct GradPlan {
-    int64_t piece, ld, d, sums, acc, part, acc_ld, scale, bytes;
+    int64_t piece, ld, d, sums, acc, part, acc_ld, scale, x, x_ld, bytes;
     int pieces, splits;
     bool direct;  // dx in one product, rounded by its epilogue
 };
@@ -468,7 +491,9 @@ static GradPlan grad_plan(const drift_xent *op) {
     p.sums = up(t * p.ld * 2, 256);
     p.acc = p.sums + (op->bias ? up(up(t, 256) / 32 * p.ld * 4, 256) : 0);
     p.scale = p.acc + (p.direct ? 0 : up(p.splits * p.part * 4, 256));
-    p.bytes = p.scale + 256;
+    p.x_ld = up(op->depth, 8);
+    p.x = p.scale + 256;
+    p.bytes = p.x + up(t * p.x_ld * 2, 256);
     return p;
 }
 
@@ -478,7 +503,7 @@ static GradPlan grad_plan(const drift_xent *op) {
 // so rows longer than 2^15 (some 20 us) are left to the other way.
 struct KeptPlan {
     bool use;
-    int64_t ld, part, logits, d, loss, inv, acc, acc_part, acc_ld, bytes;
+    int64_t ld, part, logits, d, loss, inv, acc, acc_part, acc_ld, x, x_ld, bytes;
     int splits, dx_splits;
 };
 static KeptPlan kept_plan(const drift_xent *op) {
@@ -499,7 +524,9 @@ static KeptPlan kept_plan(const drift_xent *op) {
     p.acc_part = t * p.acc_ld;
     p.inv = p.loss + up(t * 4, 256);
     p.acc = p.inv + 256;
-    p.bytes = p.acc + (p.dx_splits > 1 ? up(p.dx_splits * p.acc_part * 4, 256) : 0) + 256;
+    p.x_ld = up(op->depth, 8);
+    p.x = p.acc + (p.dx_splits > 1 ? up(p.dx_splits * p.acc_part * 4, 256) : 0);
+    p.bytes = p.x + up(t * p.x_ld * 2, 256);
     return p;
 }
 
@@ -520,6 +547,12 @@ static int launch_mean(const float *row_loss, int64_t n, const XentRows &rows, f
                        float *inv, cudaStream_t st) {
     return launch_pdl(xent_mean_kernel, dim3(1), n <= 256 ? 256 : 1024, 0, st, 0, row_loss, n, rows,
                       mean, inv);
+}
+
+// x's rows are whole units of 16 bytes (its stride is), and so are the copy's.
+static CopyRows copy_rows(const drift_xent *op, void *to, int64_t to_ld) {
+    return CopyRows{static_cast<const uint4 *>(op->x), static_cast<uint4 *>(to), op->x_stride / 8,
+                    to_ld / 8, (op->depth + 7) / 8};
 }
 
 static int done() { return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA; }
@@ -596,6 +629,12 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
     const float *undo = one ? g : scale ? scale + 1 : nullptr, *sum_undo = one ? g : nullptr;
     const float beta = 1.0f / fixed;
     const float *row_g = one ? nullptr : g;
+    T *x = reinterpret_cast<T *>(ws + p.x);
+    if (dw) {
+        const int rc = launch_pdl(xent_copy_kernel, dim3((unsigned)n_t), 128, 0, st, 0,
+                                  copy_rows(op, x, p.x_ld), rows);
+        if (rc) return rc;
+    }
     for (int64_t v0 = 0; v0 < op->vocab; v0 += p.piece) {
         const int64_t n = std::min(p.piece, op->vocab - v0);
         tc::Args a;
@@ -637,7 +676,7 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
         if (dw) {
             // dW (piece x D) contracts the tokens: rows of d and of x are k.
             if (!tc::encode_16(&a.a, BF16, d, n, n_t, p.ld, false) ||
-                !tc::encode_16(&a.b, BF16, op->x, dep, n_t, op->x_stride, false))
+                !tc::encode_16(&a.b, BF16, x, dep, n_t, p.x_ld, false))
                 return DRIFT_ECUDA;
             a.m_tiles = tiles(n), a.n_tiles = tiles(dep), a.k_stages = stages(n_t);
             a.splits = 1, a.run = kGradRun;
@@ -664,6 +703,7 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
     float *acc = reinterpret_cast<float *>(ws + p.acc);
     T *d = reinterpret_cast<T *>(ws + p.d);
     float *inv = reinterpret_cast<float *>(ws + p.inv);
+    T *x = reinterpret_cast<T *>(ws + p.x);
     const float scale = BF16 ? 1.0f : 32768.0f, beta = 1.0f / scale;
     tc::Args a;
     if (!logit_args(a, op, 0, n, BF16, err)) return DRIFT_ECUDA;
@@ -672,8 +712,8 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
         a, PartEpi{logits, p.part, p.ld, n_t, n, false}, sm_count(), st);
     if (rc) return rc;
     rc = launch_pdl(xent_row_kernel<T>, dim3((unsigned)n_t), 256, 0, st, 0, logits, a.splits, p.part,
-                    p.ld, n, op->bias, rows, d, scale, db != nullptr, row_loss, (float *)nullptr,
-                    err);
+                    p.ld, n, op->bias, rows, d, scale, db != nullptr, row_loss,
+                    dw ? copy_rows(op, x, p.x_ld) : CopyRows{}, err);
     // Few rows: one kernel for the mean and db, whose CTAs all read the targets.
     if (!rc && db && n_t <= 4096) {
         rc = launch_pdl(xent_mean_db_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, st, 0,
@@ -704,7 +744,7 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
     }
     if (!rc && dw) {
         if (!tc::encode_16(&a.a, BF16, d, n, n_t, p.ld, false) ||
-            !tc::encode_16(&a.b, BF16, op->x, dep, n_t, op->x_stride, false))
+            !tc::encode_16(&a.b, BF16, x, dep, n_t, p.x_ld, false))
             return DRIFT_ECUDA;
         a.m_tiles = tiles(n), a.n_tiles = tiles(dep), a.k_stages = stages(n_t);
         a.splits = 1, a.run = kGradRun;

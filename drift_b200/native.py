@@ -103,6 +103,9 @@ def _streamed(fn):
             _start()
         if stream is None:
             return fn(*args, **kw)
+        ctx = kw.get("ctx") or getattr(args[0], "ctx", None) or _lib.Context.current()
+        if stream.device.index != ctx.device:
+            raise ValueError(f"stream on {stream.device}, context on device {ctx.device}")
         with torch.cuda.stream(stream):
             return fn(*args, **kw)
 
@@ -173,8 +176,9 @@ class Mx4:
     @staticmethod
     def from_parts(codes, scales, cols: Optional[int] = None) -> "Mx4":
         """From plain arrays, as a file holds them: `codes` uint8 (rows, ceil(cols/32)*16),
-        the even element in the low nibble and padding codes 0, and `scales`
-        uint8 (rows, ceil(cols/32)), exponent + 127, none of them 255."""
+        the even element in the low nibble, and `scales`
+        uint8 (rows, ceil(cols/32)), exponent + 127, none of them 255. Both are
+        copied; codes past `cols` are read as 0."""
         if torch is None:
             _start()
         rows, blocks = scales.shape
@@ -189,8 +193,12 @@ class Mx4:
         full[:rows, :blocks] = scales
         # Row r, block b of a 128 x 4 tile is byte (r % 32) * 16 + (r / 32) * 4 + b.
         tiled = full.view(tiles_r, 4, 32, tiles_k, 4).permute(0, 3, 2, 1, 4).contiguous()
-        # Copies of its own, so that both arrays are aligned.
-        return Mx4(codes.clone(memory_format=torch.contiguous_format), tiled.view(-1), rows, cols)
+        # Copies of its own, so that both arrays are aligned and the padding is zero.
+        own = codes.clone(memory_format=torch.contiguous_format)
+        own[:, (cols + 1) // 2:] = 0
+        if cols % 2:
+            own[:, cols // 2] &= 15
+        return Mx4(own, tiled.view(-1), rows, cols)
 
     def to_parts(self):
         """The plain arrays that from_parts takes."""
@@ -243,7 +251,7 @@ def mx4_quantize_dev(p: NumericPolicy, src, rm: Optional[Rounding] = None, *,
     rows, cols = src.shape
     stride, step = src.stride()
     if (cols > 1 and step != 1) or (rows > 1 and stride < cols):
-        src = src.contiguous()
+        src = src.detach().contiguous()
         stride = cols
     row = Mx4._empty(call.device, rows, cols) if axis != 0 else None
     col = Mx4._empty(call.device, cols, rows) if axis != 1 else None
@@ -319,7 +327,7 @@ def _xent_rows(call: _Call, t, what: str):
     if (d == 1 or s1 == 1) and t.data_ptr() % 16 == 0 and s0 % 8 == 0 and s0 >= d:
         return t, s0
     pad = torch.empty((rows, (d + 7) // 8 * 8), dtype=t.dtype, device=t.device)
-    pad[:, :d] = t
+    pad[:, :d] = t.detach()
     return pad, pad.shape[1]
 
 
@@ -500,6 +508,12 @@ class AdamW:
             if c is not None:
                 t.copy = call.ptr(c, f"copies[{i}]", numel=n[i])
                 t.copy_type = _type_of(c.dtype, f"copies[{i}]", low)
+        # Everything a step writes, in order of address: no two may share memory.
+        written = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size())
+                         for part in (self.params, *self.state, self.copies) for x in part
+                         if x is not None and x.numel())
+        if any(a[1] > b[0] for a, b in zip(written, written[1:])):
+            raise ValueError("parameters, moments and copies must not share memory")
 
     @_streamed
     def step(self, grads: Sequence, *, lr: Optional[float] = None, d_lr=None,

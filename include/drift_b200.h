@@ -589,7 +589,7 @@ DRIFT_API int drift_mx4_gemm_dev(drift_ctx *ctx, const drift_mx4 *A, const drift
  * W: vocab x depth, both of `type` (DRIFT_T_BF16 or DRIFT_T_FP16), rows x_stride
  * and w_stride elements apart; bases and rows 16-byte aligned. bias: vocab
  * floats or NULL. targets: int32 or int64 (target_bits); rows whose target is
- * ignore_index have loss 0 and no gradient; any other target outside the
+ * ignore_index have loss 0 and no gradient, whatever x holds there; any other target outside the
  * vocabulary is treated so too and reported by drift_check_dev as
  * DRIFT_EINVAL.
  */

@@ -265,5 +265,16 @@ def test_refusals():
         d.AdamW([torch.zeros(8, dtype=torch.float64, device="cuda")])
     with pytest.raises(ValueError):
         d.AdamW([torch.zeros(4, 4, device="cuda").T[:2].T])
+    with pytest.raises(ValueError):
+        d.AdamW([p, p])
+    with pytest.raises(ValueError):
+        d.AdamW([p, p[4:]])
+    m = torch.zeros(8, device="cuda")
+    with pytest.raises(ValueError):
+        d.AdamW([p], state=[[m], [m]])
+    with pytest.raises(ValueError):
+        d.AdamW([p], copies=[p])
+    with pytest.raises(d.DriftError):
+        d.AdamW([p], eps=1e-35).step([torch.zeros(8, device="cuda")])
     with pytest.raises(d.DriftError):
         d.AdamW([p], betas=(1.0, 0.9)).step([torch.zeros(8, device="cuda")])

@@ -280,6 +280,23 @@ def test_product_overflows_to_infinity_and_keeps_exact_zeros():
     assert not d.mx4_gemm_dev(q, z).any()
 
 
+@pytest.mark.parametrize("m,n,k", [(3, 200, 300), (400, 300, 300)])
+@pytest.mark.parametrize("ea,eb", [(-100, 90), (-125, 120), (-128, 120), (-133, 120), (120, -126)])
+def test_scales_at_both_ends_of_their_range(m, n, k, ea, eb):
+    """Small values times large ones, down to the scale byte 0 (2^-127) and up to
+    those near 254: products in fp32's normal range keep their bits. (At 2^-133 the
+    exponent is clamped at -127 and every element rounds to zero.)"""
+    rs = np.random.default_rng(1)
+    A, B = (d.mx4_quantize_dev(P["nearest"], torch.from_numpy(rs.standard_normal((r, k))
+                                                              * 2.0 ** e).cuda())
+            for r, e in ((m, ea), (n, eb)))
+    a, b = d.mx4_dequantize_dev(A), d.mx4_dequantize_dev(B)
+    want = a @ b.T
+    got = d.mx4_gemm_dev(A, B).double()
+    assert ((got - want).abs() <= bound(a, b, want, torch.float32)).all()
+    assert want.any() == (ea > -133)
+
+
 def test_refusals():
     A, B = packed(4, 64, 1), packed(6, 96, 2)
     with pytest.raises(ValueError):

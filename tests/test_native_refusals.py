@@ -101,9 +101,12 @@ def test_plain_arrays_round_trip_through_the_tiled_scales(rows, cols):
     128 x 4 tile and pads with 127; to_parts undoes it."""
     rs = np.random.default_rng(rows * 1000 + cols)
     blocks = (cols + 31) // 32
-    codes = torch.from_numpy(rs.integers(0, 256, (rows, blocks * 16), dtype=np.uint8))
+    codes = rs.integers(0, 256, (rows, blocks * 16), dtype=np.uint8)
+    nib = np.stack((codes & 15, codes >> 4), -1).reshape(rows, -1)
+    nib[:, cols:] = 0
+    dirty, codes = torch.from_numpy(codes), torch.from_numpy(nib[:, 0::2] | nib[:, 1::2] << 4)
     scales = torch.from_numpy(rs.integers(0, 255, (rows, blocks), dtype=np.uint8))
-    q = d.Mx4.from_parts(codes, scales, cols)
+    q = d.Mx4.from_parts(dirty, scales, cols)  # padding codes are dropped
     k_tiles = (cols + 255) // 256 * 2
     want = np.full((rows + 127) // 128 * k_tiles * 512, 127, dtype=np.uint8)
     for r in range(rows):

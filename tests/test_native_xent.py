@@ -205,6 +205,27 @@ def test_a_row_without_any_entry_and_nan_inputs():
     assert not torch.isfinite(lse).any() and not torch.isfinite(loss).any()
 
 
+@pytest.mark.parametrize("t,v", [(70, 300), (70, 40000)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_ignored_rows_may_hold_anything(t, v, bad):
+    """Padded positions full of NaN or Inf: losses and gradients as with zeros there."""
+    x, w, tg, b = inputs(t, 72, v, ignored=0.3, seed=9)
+    clean, dirty = x.clone(), x.clone()
+    clean[tg == IG] = 0
+    dirty[tg == IG] = bad
+    for bias in (None, b):
+        want = d.linear_xent_mean_dev(clean, w, tg, bias=bias)
+        got = d.linear_xent_mean_dev(dirty, w, tg, bias=bias)
+        for a, c in zip(got, want):
+            assert (a is None and c is None) or torch.equal(a, c)
+        loss, lse = d.linear_xent_dev(dirty, w, tg, bias=bias)
+        assert torch.equal(loss, d.linear_xent_dev(clean, w, tg, bias=bias)[0])
+        g = torch.randn(t, device="cuda")
+        for a, c in zip(d.linear_xent_grad_dev(dirty, w, tg, lse, g, bias=bias),
+                        d.linear_xent_grad_dev(clean, w, tg, lse, g, bias=bias)):
+            assert (a is None and c is None) or torch.equal(a, c)
+
+
 def test_targets_outside_the_vocabulary():
     x, w, tg, b = inputs(20, 32, 50, ignored=0.0, seed=7)
     for wrong in (50, -1, 2 ** 40, -2 ** 40):
