@@ -3,7 +3,7 @@
 //
 // Every element does, in 32 bits, with fma(a, b, c) one rounding and every other
 // operation its own (this is the definition, so the same operations elsewhere
-// give the moments' bits):
+// give m's and v's bits):
 //
 //   m' = fma(b1, m, (1-b1) g)     v' = fma(b2, v, ((1-b2) g) g)   r = sqrt(v')
 //   p' = fma(1 - lr wd, p, -(lr/(1-b1^t) m') / fma(r, 1/sqrt(1-b2^t), eps))
@@ -18,9 +18,16 @@
 //
 // Bound: HBM bytes. 32-bit moments with fp32 parameters and bf16 gradients
 // move 26 bytes an element, 8-bit moments with bf16 parameters and gradients
-// 10.1. One warp owns a block of 256 elements, eight a lane, so a block's
-// amax is five shuffles and every access is one or two 16-byte loads or
+// 10.1. One warp owns a block of 256 elements, eight a lane, so a block's amax is
+// a handful of instructions and every access is one or two 16-byte loads or
 // stores a lane.
+//
+// Measured on one B200: 400M bf16 parameters with 8-bit moments in 690 us (5.86
+// TB/s, 91 % of the copy rate), 8.6M fp32 ones with 32-bit moments in 41 us (5.9
+// TB/s). Each CTA on a stretch of its own took 1143 us for the first: the CTAs in
+// flight then touch as many stretches of seven arrays, where side by side they
+// sweep one of each. 68 instructions an element (scalar operations, IEEE root and
+// quotient) took 1083 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -11,8 +11,13 @@
 // Bound: HBM bytes (the source once, 17/32 byte an element out, for each
 // direction of blocks). Along rows a lane takes eight elements, so four lanes
 // share a block and its amax is two shuffles. Down columns a CTA stages a tile
-// of 128 x 64 in shared memory; where both directions are wanted they read the
-// same tile, so the source is read once.
+// of 128 x 128 (64 of the wider types) in shared memory; where both directions are
+// wanted they read the same tile, so the source is read once.
+//
+// Measured on one B200: rows of 4096 x 4096 fp32 in 12.4 us (6.15 TB/s, 95 % of the
+// copy rate), of 8192 x 8192 bf16 in 35 us (4.8 TB/s), both axes in 75 us (2.7 TB/s).
+// 16-bit sources are bound by instructions, 12 an element and axis: a conversion
+// instruction makes two codes, and each element is widened and scaled on the way.
 #include <algorithm>
 #include <type_traits>
 

@@ -25,7 +25,9 @@
 //
 // Bound: the tensor cores for many tokens (8 T D V operations with the
 // gradient's second computation of the logits, against 6 T D V if they were
-// kept); the bytes of W for few.
+// kept); the bytes of W for few. Measured on one B200: 4096 tokens x 131072 entries
+// x 4096 with gradients in 14.2 to 15.2 ms (1.16 to 1.24 PFLOP/s under the power
+// cap), the loss of 64 tokens x 131072 x 4096 in 224 us (4.8 TB/s).
 #include <algorithm>
 
 #include "epilogue.cuh"
