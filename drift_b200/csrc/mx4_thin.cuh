@@ -7,9 +7,9 @@
 // keeps 160 KB and more of B in flight. Measured on one B200, back to back: one token
 // through 8192 x 8192 7.5 us (35.7 MB, 4.8 TB/s), 64 through 2048 x 2048 4.7 us, 1 x
 // 1 x 64 2.6 us. One CTA an SM with eight stages took 10.4 us for the first.
-// The cluster's partial tiles meet in
-// shared memory: CTA r adds up tokens [NT r / S, NT (r + 1) / S) of all S, in
-// order, so results do not depend on timing.
+//
+// The cluster's partial tiles meet in shared memory: CTA r adds up tokens
+// [NT r / S, NT (r + 1) / S) of all S, in order, so results do not depend on timing.
 #pragma once
 
 #include "epilogue.cuh"
