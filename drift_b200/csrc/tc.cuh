@@ -65,7 +65,7 @@ constexpr int kThreads = (kEpiWarps + 4) * 32;  // three warpgroups
 // 168 * 384, exactly the launch's total.
 constexpr int kControlRegs = 56, kEpiRegs = 224;
 static_assert(2 * kEpiRegs + kControlRegs == 3 * 168, "the split must not exceed the launch's");
-constexpr int kWarpTma = kEpiWarps, kWarpMma = kEpiWarps + 1;
+constexpr int kWarpTma = kEpiWarps, kWarpMma = kEpiWarps + 1, kWarpScales = kEpiWarps + 2;
 // A round of a wait is some 30 ns at the least, a stage of a contraction about 700 ns:
 // 30 ms for a wait on one stage, and 64 rounds more for every stage that a wait spans.
 constexpr int kWaitRounds = 1 << 20, kRoundsPerStage = 64;
@@ -152,6 +152,12 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar) {
         "h"((uint16_t)3)
         : "memory");
 }
+// Arrives on a barrier of this CTA once this thread's copies so far are done.
+__device__ __forceinline__ void commit_one(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                     smem_addr(bar))
+                 : "memory");
+}
 __device__ __forceinline__ void copy_scales(unsigned to, uint64_t from) {
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(from)
                  : "memory");
@@ -229,6 +235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     using S = Shape<KIND>;
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full[S::stages], empty[S::stages], acc_full[S::accs], acc_empty[S::accs];
+    __shared__ uint64_t sf_full[S::stages];  // KIND_MX4: a stage's scales are in TMEM
     __shared__ unsigned tmem_base;
     const unsigned base = (smem_addr(raw) + 1023) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -237,7 +244,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int s = 0; s < S::stages; s++)
+            mbar_init(&full[s], 1), mbar_init(&empty[s], 1), mbar_init(&sf_full[s], 1);
         for (int s = 0; s < S::accs; s++)
             mbar_init(&acc_full[s], 1), mbar_init(&acc_empty[s], 2 * kEpiWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -303,6 +311,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 ok = wait(&empty[s], ph);
                 if (++s == S::stages) s = 0, ph ^= 1;
             }
+        } else if (KIND == KIND_MX4 && warp == kWarpScales && rank == 0 && lane == 0) {
+            // Scales from shared memory to TMEM, in both CTAs, as soon as they are there.
+            if constexpr (KIND == KIND_MX4) {
+                int s = 0;
+                unsigned ph = 0;
+                for (int t = first; t < total && ok; t += step) {
+                    const Work w = work_at(args, t);
+                    for (int k = w.k0; k < w.k1; k++) {
+                        ok = wait(&full[s], ph);
+                        if (!ok) break;
+                        fence_after();
+                        const unsigned fa = tmem + S::sfa_col + s * 8;
+                        const unsigned fb = tmem + S::sfb_col + s * 16;
+                        // Tiles of scales: 32 lanes of 16 bytes, to all four lane quadrants.
+                        const uint64_t sc =
+                            smem_desc(base + s * stage_bytes<KIND>() + 2 * kOperand, 0, 128, 0);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            copy_scales(fa + h * 4, sc + h * 32);
+                            copy_scales(fb + h * 8, sc + 64 + h * 32);
+                            copy_scales(fb + h * 8 + 4, sc + 128 + h * 32);
+                        }
+                        commit_one(&sf_full[s]);
+                        if (++s == S::stages) s = 0, ph ^= 1;
+                    }
+                }
+            }
         } else if (warp == kWarpMma && rank == 0 && lane == 0) {
             // This thread's instructions between two stages are the tensor cores'
             // pauses, so its indexes run along and descriptors are a base plus a
@@ -317,53 +352,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             constexpr unsigned a_step = A_MN ? 128 : 2, b_step = B_MN ? 128 : 2;
             int s = 0, acc = 0;
             unsigned ph = 0, acc_ph = 1;
-            // KIND_MX4: a stage's scales go to TMEM one stage ahead of its MMAs, so that
-            // no MMA waits for the copies just before it.
-            bool held = false;
-            int hs = 0;
-            unsigned hd = 0, hmore = 0;
-            const auto mma_mx4 = [&]() {
-                constexpr int sfa_col = Shape<KIND_MX4>::sfa_col, sfb_col = Shape<KIND_MX4>::sfb_col;
-                const unsigned fa = tmem + sfa_col + hs * 8, fb = tmem + sfb_col + hs * 16;
-                const unsigned off = hs * (stage_bytes<KIND>() >> 4);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    // 64 elements: two scales of a 32-bit column's four.
-                    const unsigned id = (j & 1) * 2;
-                    asm volatile(
-                        "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
-                        " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
-                        " [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(hd),
-                        "l"(da0 + off + j * 2), "l"(db0 + off + j * 2),
-                        "r"(idesc | id << 4 | id << 29), "r"(fa + (j >> 1) * 4),
-                        "r"(fb + (j >> 1) * 8), "r"(j > 0 ? 1u : hmore)
-                        : "memory");
-                }
-                commit_pair(&empty[hs]);
-                held = false;
-            };
             for (int t = first; t < total && ok; t += step) {
                 const Work w = work_at(args, t);
                 int left = KIND == KIND_16 ? args.run : 1 << 30;  // stages until this sum ends
                 unsigned more = 0;
                 for (int k = w.k0; k < w.k1; k++) {
-                    ok = wait(&full[s], ph);
+                    // The scales' barrier completes after the operands'.
+                    ok = wait(KIND == KIND_MX4 ? &sf_full[s] : &full[s], ph);
                     if (!ok) break;
                     fence_after();
                     const unsigned off = s * (stage_bytes<KIND>() >> 4);
-                    if (KIND == KIND_MX4) {
-                        const unsigned fa = tmem + Shape<KIND_MX4>::sfa_col + s * 8;
-                        const unsigned fb = tmem + Shape<KIND_MX4>::sfb_col + s * 16;
-                        // Tiles of scales: 32 lanes of 16 bytes, to all four lane quadrants.
-                        const uint64_t sc = smem_desc(base + 2 * kOperand, 0, 128, 0) + off;
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            copy_scales(fa + h * 4, sc + h * 32);
-                            copy_scales(fb + h * 8, sc + 64 + h * 32);
-                            copy_scales(fb + h * 8 + 4, sc + 128 + h * 32);
-                        }
-                        if (held) mma_mx4();
-                    }
                     if (more == 0) {
                         // A sum begins: its accumulator must have been read.
                         ok = wait(&acc_empty[acc], acc_ph);
@@ -371,8 +369,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         fence_after();
                     }
                     const unsigned d = tmem + acc * kTile;
-                    if (KIND == KIND_MX4) {
-                        held = true, hs = s, hd = d, hmore = more;
+                    if constexpr (KIND == KIND_MX4) {
+                        const unsigned fa = tmem + S::sfa_col + s * 8;
+                        const unsigned fb = tmem + S::sfb_col + s * 16;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            // 64 elements: two scales of a 32-bit column's four.
+                            const unsigned id = (j & 1) * 2;
+                            asm volatile(
+                                "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
+                                " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
+                                " [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+                                "l"(da0 + off + j * 2), "l"(db0 + off + j * 2),
+                                "r"(idesc | id << 4 | id << 29), "r"(fa + (j >> 1) * 4),
+                                "r"(fb + (j >> 1) * 8), "r"(j > 0 ? 1u : more)
+                                : "memory");
+                        }
                     } else {
 #pragma unroll
                         for (int j = 0; j < 4; j++)
@@ -382,12 +394,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 "l"(da0 + off + j * a_step), "l"(db0 + off + j * b_step),
                                 "r"(idesc), "r"(j > 0 ? 1u : more)
                                 : "memory");
-                        commit_pair(&empty[s]);
                     }
+                    commit_pair(&empty[s]);
                     more = 1;
                     if (++s == S::stages) s = 0, ph ^= 1;
                     if (--left == 0 || k == w.k1 - 1) {
-                        if (KIND == KIND_MX4) mma_mx4();
                         commit_pair(&acc_full[acc]);
                         if (++acc == S::accs) acc = 0, acc_ph ^= 1;
                         left = KIND == KIND_16 ? args.run : 1 << 30;
@@ -403,6 +414,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int n_acc = 0;
         for (int t = first; t < total && ok; t += step) {
             const Work w = work_at(args, t);
+            const int64_t row0 = (int64_t)w.m * kTile + (int)rank * kRows + quad * 32;
+            const int64_t col = (int64_t)w.n * kTile + half * 128;
+            const bool live = row0 < epi.rows && col < epi.cols;  // else nothing to do
             float v[128];
             const int run = KIND == KIND_16 ? min(args.run, w.k1 - w.k0) : w.k1 - w.k0;
             for (int k = w.k0; k < w.k1; k += run, n_acc++) {
@@ -412,7 +426,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (!ok) break;
                 fence_after();
                 const unsigned at = tmem + acc * kTile + half * 128 + ((unsigned)(quad * 32) << 16);
-                if (S::accs == 1 || k == w.k0) {
+                if (!live) {
+                } else if (S::accs == 1 || k == w.k0) {
 #pragma unroll
                     for (int c = 0; c < 4; c++) tmem_load32(at + c * 32, v + c * 32);
                     tmem_wait_load();
@@ -431,8 +446,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (lane == 0) arrive_cluster(map_cta(smem_addr(&acc_empty[acc]), 0));
             }
             if (!ok) break;
-            const int64_t row0 = (int64_t)w.m * kTile + (int)rank * kRows + quad * 32;
-            epi.run(v, row0, (int64_t)w.n * kTile + half * 128, w, lane, staging);
+            if (live) epi.run(v, row0, col, w, lane, staging);
         }
     }
 
