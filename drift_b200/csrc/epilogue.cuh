@@ -54,6 +54,22 @@ __device__ __forceinline__ uint4 smem_load16(unsigned at) {
     return w;
 }
 
+template <class T> __device__ __forceinline__ T smem_load(unsigned at) {
+    if constexpr (sizeof(T) == 8) {
+        double x;
+        asm volatile("ld.shared.f64 %0, [%1];" : "=d"(x) : "r"(at) : "memory");
+        return x;
+    } else if constexpr (sizeof(T) == 4) {
+        float x;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+        return x;
+    } else {
+        unsigned short x;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at) : "memory");
+        return *reinterpret_cast<const T *>(&x);
+    }
+}
+
 // Passes a warp's 32 rows x 128 columns (lane = row) through shared memory, 128
 // bytes a row at a time, so that eight lanes hold a row's 128 bytes and a store
 // instruction covers four whole lines: lane by lane a store of 16 bytes would
@@ -73,6 +89,34 @@ __device__ __forceinline__ void by_rows(const float (&v)[128], unsigned staging,
         for (int i = 0; i < 8; i++) {
             const int row = i * 4 + (lane >> 3), j = lane & 7;
             put(row, c + j * kUnit, smem_load16(staging + row * 128 + ((j ^ (row & 7)) << 4)));
+        }
+        __syncwarp();
+    }
+}
+
+// The same where rows are not 16-byte aligned: a store instruction takes up to 32
+// neighbouring elements of one row. `put(row, column, element)`. (Each lane storing
+// its own row, 128 x 2 bytes in 32 lines at a time, took 40 us a tile.)
+template <class T, class Put>
+__device__ __forceinline__ void by_elements(const float (&v)[128], unsigned staging, int lane,
+                                            Put put) {
+    constexpr int kCols = 128 / (int)sizeof(T), kUnit = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int c = 0; c < 128; c += kCols) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            smem_store16(staging + lane * 128 + ((j ^ (lane & 7)) << 4),
+                         pack16<T>(v + c + j * kUnit));
+        __syncwarp();
+#pragma unroll 4
+        for (int r = 0; r < 32; r++) {
+#pragma unroll
+            for (int j0 = 0; j0 < kCols; j0 += 32) {
+                const int j = j0 + lane, byte = j * (int)sizeof(T);
+                if (j < kCols)
+                    put(r, c + j,
+                        smem_load<T>(staging + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15)));
+            }
         }
         __syncwarp();
     }
@@ -115,11 +159,13 @@ template <class T> struct StoreEpi {
                         if (j + u < left) to[u] = x[u];
                 }
             });
-        } else if (row0 + lane < rows) {
-            T *p = c + (row0 + lane) * stride + col;
-#pragma unroll
-            for (int j = 0; j < 128; j++)
-                if (col + j < cols) p[j] = T(v[j]);
+        } else {
+            T *p = c + row0 * stride + col;
+            const int rows_left = (int)min((int64_t)32, rows - row0);
+            const int left = (int)min((int64_t)128, cols - col);
+            by_elements<T>(v, staging, lane, [&](int r, int j, T x) {
+                if (r < rows_left && j < left) p[r * stride + j] = x;
+            });
         }
     }
 };

@@ -36,15 +36,16 @@ __global__ void __launch_bounds__(256) fill_bias_kernel(T *C, int64_t stride, in
         C[i / cols * stride + i % cols] = T(bias ? bias[i % cols] : 0.0f);
 }
 
-// Estimated tenths of a microsecond, from products of 129x2048x2048 to
-// 2048x4096x4096 measured both ways (within a fifth of either): a wave of pair
-// tiles takes 6.6 a stage and 35, a wave of thin CTAs 5 a stage and 65.
+// Estimated hundredths of a microsecond, from products of 129 x 2048 x 2048 to 2048
+// x 4096 x 4096 measured both ways (within a tenth of the pairs' times, a fifth of the
+// thin ones'): a wave of pair tiles takes 0.41 us a stage and 2.2, a wave of thin CTAs
+// 0.5 a stage and 2.2, or 5 where one CTA has a whole contraction and writes alone.
 static int64_t pair_cost(int64_t m, int64_t n, int64_t stages, int sms) {
     const int64_t tiles = (m + tc::kTile - 1) / tc::kTile * ((n + tc::kTile - 1) / tc::kTile);
-    return (tiles + sms / 2 - 1) / (sms / 2) * (66 * stages + 350);
+    return (tiles + sms / 2 - 1) / (sms / 2) * (41 * stages + 220);
 }
 static int64_t thin_cost(int64_t tiles, int64_t stages, int split, int slots) {
-    return (tiles * split + slots - 1) / slots * (50 * ((stages + split - 1) / split) + 650);
+    return (tiles * split + slots - 1) / slots * (50 * ((stages + split - 1) / split) + (split > 1 ? 220 : 500));
 }
 // How many CTAs share a thin tile's contraction: up to four, or a portable
 // cluster's eight where tiles are few. (Sixteen clusters of eight did not all fit

@@ -18,7 +18,7 @@
 namespace drift {
 namespace thin {
 
-constexpr int kThreads = 192;  // warps 0-3 epilogue, 4 TMA, 5 MMA
+constexpr int kThreads = 224;  // warps 0-3 epilogue, 4 TMA, 5 MMA, 6 scales
 constexpr int kTmemCols = 256;
 constexpr int kScaleCol = 128;
 
@@ -87,7 +87,7 @@ template <int NT, class T>
 __global__ void __launch_bounds__(kThreads, Shape<NT>::per_sm) thin_kernel(const __grid_constant__ Args args) {
     using S = Shape<NT>;
     extern __shared__ unsigned char raw[];
-    __shared__ uint64_t full[S::stages], empty[S::stages], acc_full;
+    __shared__ uint64_t full[S::stages], empty[S::stages], sf_full[S::stages], acc_full;
     __shared__ unsigned tmem_base;
     const unsigned base = (smem_addr(raw) + 1023) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -100,7 +100,8 @@ __global__ void __launch_bounds__(kThreads, Shape<NT>::per_sm) thin_kernel(const
     const int k1 = (int)((int64_t)args.k_stages * (rank + 1) / ranks);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int s = 0; s < S::stages; s++)
+            mbar_init(&full[s], 1), mbar_init(&empty[s], 1), mbar_init(&sf_full[s], 1);
         mbar_init(&acc_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -150,12 +151,14 @@ __global__ void __launch_bounds__(kThreads, Shape<NT>::per_sm) thin_kernel(const
                                    1u << 23;
             const uint64_t da = tc::smem_desc(base, 16, 1024, 2);
             const uint64_t db = tc::smem_desc(base + 16384, 16, 1024, 2);
-            const uint64_t sc = tc::smem_desc(base + 16384 + NT * 128, 0, 128, 0);
             int s = 0;
             unsigned ph = 0;
-            const auto mma = [&](int hs, bool first) {
-                const unsigned fa = tmem + kScaleCol + hs * 16, fb = fa + 8;
-                const unsigned off = hs * (S::stage >> 4);
+            for (int k = k0; k < k1; k++) {
+                ok = tc::wait(&sf_full[s], ph);  // completes after the operands' barrier
+                if (!ok) break;
+                tc::fence_after();
+                const unsigned fa = tmem + kScaleCol + s * 16, fb = fa + 8;
+                const unsigned off = s * (S::stage >> 4);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const unsigned id = (j & 1) * 2;
@@ -165,31 +168,35 @@ __global__ void __launch_bounds__(kThreads, Shape<NT>::per_sm) thin_kernel(const
                         " [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(tmem),
                         "l"(da + off + j * 2), "l"(db + off + j * 2),
                         "r"(idesc | id << 4 | id << 29), "r"(fa + (j >> 1) * 4),
-                        "r"(fb + (j >> 1) * 4), "r"((unsigned)(j > 0 || !first))
+                        "r"(fb + (j >> 1) * 4), "r"((unsigned)(j > 0 || k > k0))
                         : "memory");
                 }
-                commit(&empty[hs]);
-            };
-            int held = -1;
+                commit(&empty[s]);
+                if (++s == S::stages) s = 0, ph ^= 1;
+            }
+            if (ok) commit(&acc_full);
+        }
+        __syncwarp();
+    } else if (warp == 6) {
+        // A thread of their own issues the scale copies: in the MMAs' thread they would
+        // run between them, not beside them.
+        if (lane == 0) {
+            int s = 0;
+            unsigned ph = 0;
             for (int k = k0; k < k1; k++) {
                 ok = tc::wait(&full[s], ph);
                 if (!ok) break;
                 tc::fence_after();
                 const unsigned at = tmem + kScaleCol + s * 16;
-                const uint64_t from = sc + s * (S::stage >> 4);
+                const uint64_t from =
+                    tc::smem_desc(base + s * S::stage + 16384 + NT * 128, 0, 128, 0);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     copy_scales(at + h * 4, from + h * 32);
                     copy_scales(at + 8 + h * 4, from + 64 + h * 32);
                 }
-                // The scales go ahead of the stage before's MMAs, not between the two.
-                if (held >= 0) mma(held, k - 1 == k0);
-                held = s;
+                commit(&sf_full[s]);
                 if (++s == S::stages) s = 0, ph ^= 1;
-            }
-            if (ok) {
-                mma(held, k1 - k0 == 1);
-                commit(&acc_full);
             }
         }
         __syncwarp();

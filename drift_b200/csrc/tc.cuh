@@ -14,7 +14,8 @@
 //
 // Warps: 0-7 epilogue (two per quadrant of TMEM lanes, 128 columns each), 8
 // fetches with TMA, 9 allocates TMEM and, in the pair's first CTA, issues the
-// MMAs, 10 and 11 complete the control warpgroup. A stage's barrier `full` sits
+// MMAs, 10 issues KIND_MX4's copies of scales to TMEM, in a thread of its own so
+// that they run beside the MMAs, and 11 completes the group. A stage's barrier `full` sits
 // in the first CTA and counts both CTAs' bytes; a commit of the stage's MMAs frees
 // it in both CTAs. The accumulator passes to the epilogue by `acc_full` (a commit
 // to both) and back by `acc_empty` (first CTA, one arrival an epilogue warp of
@@ -24,19 +25,12 @@
 // scales a stage.
 //
 // Measured on one B200: KIND_16 1.49 PFLOP/s (92 % of a library product's rate) over
-// 4096 x 131072 x 4096 in a burst, 1.2 under the power cap. KIND_MX4 3.8 PFLOP/s at
-// 8192^3, 3.4 at 8192 x 8192 x 4096; a timing copy without the six scale copies a
-// stage ran 5.3, without B's loads no faster than with them: the tensor cores' queue
-// bounds it, and in it each scale copy costs 60 cycles beside an MMA's 230. Copying
-// the scales with tcgen05.st from registers instead, by warps of their own, ran 2.7.
-//
-// The tensor cores truncate each sum to fp32, so a long contraction drifts toward
-// zero by half a unit an MMA: 2^-17 of a logit over 4096 elements. KIND_16
-// therefore sums `run` stages (of 64 elements) in TMEM and adds those sums in
-// the epilogue's registers, rounded to nearest; the two accumulators hide it.
-// Under the power cap the reads still cost: 8 % of a long product at 8 stages a
-// run, 1 % at 32. KIND_MX4's products are small multiples of a power of two,
-// whose sums are mostly exact, and it has no room for a second accumulator.
+// 4096 x 131072 x 4096 in a burst, 1.2 under the power cap. KIND_MX4 5.07 PFLOP/s at
+// 8192^3, 4.5 at 8192 x 8192 x 4096 (issued from the MMAs' thread, the scale copies
+// queued between them, 60 cycles each: 3.8 and 3.4; copied with tcgen05.st by warps
+// of their own, 2.7 and 2.5). What bounds both now is shared memory: a stage is
+// written once and read by both CTAs' MMAs, 64 KiB of its 128 bytes a cycle in the
+// 512 cycles of the MMAs.
 //
 // Every wait is bounded; one that gives up flags DEV_ERR_TIMEOUT and the
 // kernel drains and returns.
