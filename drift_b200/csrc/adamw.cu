@@ -1,16 +1,16 @@
 // adamw.cu — one AdamW step over a list of tensors in one launch, moments in
 // 32 bits or in 8 bits with one scale per 256 elements.
 //
-// Every element does, in 32 bits, with fma(a, b, c) one rounding and every other
-// operation its own (this is the definition, so the same operations elsewhere
-// give m's and v's bits):
+// Every element does, in 32 bits, the moments' operations each rounded on its own
+// (this is their definition, so the same operations elsewhere give the bits of m, v
+// and m's codes; a unit's difference now and then would move a code by a whole step,
+// and m, which forgets in ten steps, by more in the next):
 //
-//   m' = fma(b1, m, (1-b1) g)     v' = fma(b2, v, ((1-b2) g) g)   r = sqrt(v')
+//   m' = b1 m + (1-b1) g          v' = b2 v + ((1-b2) g) g        r = sqrt(v')
 //   p' = fma(1 - lr wd, p, -(lr/(1-b1^t) m') / fma(r, 1/sqrt(1-b2^t), eps))
 //
-// The quotient is a product with a reciprocal, within two units in the last
-// place, and the root within one: the IEEE forms of both were a third of the
-// instructions, and instructions, not bytes, bounded the 8-bit kernel.
+// The quotient is a product with a reciprocal, within two units in the last place,
+// and the root within one: with the IEEE root the 8-bit kernel took 890 us for 690.
 //
 // In 8 bits the first moment is held as e4m3 codes of m * (448 / amax) and
 // the second as e4m3 codes of its root r, which spans half the binades that v
@@ -60,7 +60,7 @@ struct AdamArgs {
     AdamTensor t[kAdamTensors];
     uint32_t first[kAdamTensors + 1];  // first chunk of each tensor
     int count;
-    float b1, b2, c1, c2, eps;
+    float b1, b2, c1, c2, eps, one;  // one: 1, for f2_add
     const float *scal;        // lr/(1-b1^t), 1/sqrt(1-b2^t), 1 - lr wd
     const uint64_t *rng;      // Rng state of this step's draws
     const float *grad_scale;  // may be null
@@ -302,7 +302,7 @@ __device__ __forceinline__ void load_block(const AdamTensor &t, int64_t block, i
 }
 
 struct Scalars {
-    f2 b1, b2, c1, c2, eps, neg_a1, rc2, keep, gs;
+    f2 b1, b2, c1, c2, eps, neg_a1, rc2, keep, gs, one;
     uint64_t state;
     bool scaled;
 };
@@ -328,8 +328,8 @@ __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block,
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const f2 gj = k.scaled ? f2_mul(g[j], k.gs) : g[j];
-        m[j] = f2_fma(k.b1, m[j], f2_mul(k.c1, gj));
-        v[j] = f2_fma(k.b2, v[j], f2_mul(f2_mul(k.c2, gj), gj));
+        m[j] = f2_add(f2_mul(k.b1, m[j]), f2_mul(k.c1, gj), k.one);
+        v[j] = f2_add(f2_mul(k.b2, v[j]), f2_mul(f2_mul(k.c2, gj), gj), k.one);
         float a, b;
         f2_split(v[j], a, b);
         r[j] = f2_pack(sqrt_fast(a), sqrt_fast(b));
@@ -361,7 +361,7 @@ __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block,
             inv = s = __uint_as_float(0x7fffffffu);
         } else if (amax >= 0x1p-100f) {
             inv = 448.0f / amax;
-            s = amax * (1.0f / 448.0f);
+            s = amax / 448.0f;
         }
         if (lane == 0) t.ms[block] = s;
         if (lane == 16) t.vs[block] = s;
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kAdamThreads, EIGHT && !SR ? 4 : 2) adamw_kern
     int whole = t.vec ? count(t.n / kAdamBlock) : 0;
     Scalars k;
     k.b1 = f2_both(a.b1), k.b2 = f2_both(a.b2), k.c1 = f2_both(a.c1), k.c2 = f2_both(a.c2);
-    k.eps = f2_both(a.eps);
+    k.eps = f2_both(a.eps), k.one = f2_both(a.one);
     k.neg_a1 = f2_both(-a.scal[0]), k.rc2 = f2_both(a.scal[1]), k.keep = f2_both(a.scal[2]);
     k.scaled = a.grad_scale != nullptr;
     k.gs = f2_both(k.scaled ? *a.grad_scale : 1.0f);
@@ -467,6 +467,7 @@ int launch_adamw(const drift_adamw *h, const drift_adamw_tensor *tensors, int64_
     a.c1 = (float)(1.0 - h->beta1);
     a.c2 = (float)(1.0 - h->beta2);
     a.eps = (float)h->eps;
+    a.one = 1.0f;
     a.scal = d_scalars;
     a.rng = rng_used;
     a.grad_scale = d_grad_scale;

@@ -1,8 +1,5 @@
 // pairs.cuh — two fp32 operations an instruction (mul.rn.f32x2, fma.rn.f32x2):
-// each half is rounded as the scalar operation would. There is no f2_add: the
-// assembler contracts a product and an add.rn.f32x2 into one fused operation,
-// against -fmad=false, so sums of products are written as the fused operations
-// that they become.
+// each half is rounded as the scalar operation would.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -29,5 +26,10 @@ __device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
+
+// a + b, rounded: `one` is 1 in both halves, as a value that the compiler does not
+// know. The assembler contracts a product and an add.rn.f32x2 into one fused
+// operation, against -fmad=false; this sum it cannot.
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b, f2 one) { return f2_fma(a, one, b); }
 
 }  // namespace drift

@@ -632,14 +632,14 @@ DRIFT_API int drift_linear_xent_mean_dev(drift_ctx *ctx, const drift_xent *op, f
 /*
  * One AdamW step over `count` tensors (decoupled weight decay; drift_adam_dev's
  * update with weight_decay 0, in 32 bits). Per element, each operation rounded
- * to fp32, fma(a, b, c) once:
- *   m' = fma(b1, m, (1-b1) g);  v' = fma(b2, v, ((1-b2) g) g);  r = sqrt(v')
- *   p' = fma(1 - lr wd, p, -(lr / (1 - b1^t) m') / fma(r, 1 / sqrt(1 - b2^t), eps))
- * the quotient within two units in the last place, the root within one; eps is 0
- * or in [1e-30, 1e30].
+ * to fp32:
+ *   m' = b1 m + (1-b1) g;  v' = b2 v + ((1-b2) g) g;  r = sqrt(v')
+ *   p' = (1 - lr wd) p - (lr / (1 - b1^t) m') / (r / sqrt(1 - b2^t) + eps)
+ * where p' fuses its products with its sums, the quotient is within two units in
+ * the last place and the root within one; eps is 0 or in [1e-30, 1e30].
  * state_bits 32: m and v are floats. state_bits 8: m and r are held as e4m3
  * codes with one float scale per 256 consecutive elements, code =
- * e4m3(x * (448 / amax)), value = code * (amax * (1/448)), rounded to nearest or, with
+ * e4m3(x * (448 / amax)), value = code * (amax / 448), rounded to nearest or, with
  * `rounding` stochastic, by one draw an element in tensor order.
  */
 typedef struct drift_adamw {

@@ -25,7 +25,7 @@ def to8(x):
         inv = np.where(tiny, F(0), F(448) / amax)
     y = np.clip(b * inv, F(-448), F(448))
     code = torch.from_numpy(y.reshape(-1)[:n].copy()).to(torch.float8_e4m3fn)
-    return code, np.where(tiny, F(1), amax * (F(1) / F(448)))[:, 0].astype(F)
+    return code, np.where(tiny, F(1), amax / F(448))[:, 0].astype(F)
 
 
 def from8(code, scale):
@@ -44,8 +44,8 @@ def update(p, g, m, v, step):
     """One step of one tensor: each operation rounded to fp32."""
     b1, b2 = HYP["betas"]
     a1, rc2 = F(HYP["lr"] / (1 - b1 ** step)), F(1 / np.sqrt(1 - b2 ** step))
-    m = fma(F(b1), m, F(1 - b1) * g)
-    v = fma(F(b2), v, (F(1 - b2) * g) * g)
+    m = F(b1) * m + F(1 - b1) * g
+    v = F(b2) * v + (F(1 - b2) * g) * g
     r = np.sqrt(v)
     u = (a1 * m) / fma(rc2, r, F(HYP["eps"]))
     return fma(F(1 - HYP["lr"] * HYP["weight_decay"]), p, -u), m, v, r, u
