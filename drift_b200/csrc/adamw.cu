@@ -9,10 +9,11 @@
 //   m' = b1 m + (1-b1) g          v' = b2 v + ((1-b2) g) g        r = sqrt(v')
 //   p' = fma(1 - lr wd, p, -(lr/(1-b1^t) m') / fma(r, 1/sqrt(1-b2^t), eps))
 //
-// The quotient is a product with a reciprocal, within two units in the last place,
-// and the root within one: with the IEEE root the 8-bit kernel took 890 us for 690.
+// The quotient is a product with a reciprocal, within two units in the last place.
+// The root is within one; 8-bit moments, whose state it is, take Newton's step to
+// the nearest float (no code of 16M differed from the IEEE root's).
 //
-// In 8 bits the first moment is held as e4m3 codes of m * (448 / amax) and
+// In 8 bits the first moment is held as e4m3 codes of m * (1 / amax * 448) and
 // the second as e4m3 codes of its root r, which spans half the binades that v
 // does. p' uses the moments before they are rounded to codes.
 //
@@ -22,12 +23,12 @@
 // a handful of instructions and every access is one or two 16-byte loads or
 // stores a lane.
 //
-// Measured on one B200: 400M bf16 parameters with 8-bit moments in 690 us (5.86
-// TB/s, 91 % of the copy rate), 8.6M fp32 ones with 32-bit moments in 41 us (5.9
-// TB/s). Each CTA on a stretch of its own took 1143 us for the first: the CTAs in
-// flight then touch as many stretches of seven arrays, where side by side they
-// sweep one of each. 68 instructions an element (scalar operations, IEEE root and
-// quotient) took 1083 us.
+// Measured on one B200: 400M bf16 parameters with 8-bit moments in 720 us (5.6 TB/s,
+// 87 % of the copy rate; 752 with IEEE roots), 8.6M fp32 ones with 32-bit moments in
+// 41 us (5.9 TB/s). Each CTA on a stretch of its own took 60 % longer for the first:
+// the CTAs in flight then touch as many stretches of seven arrays, where side by side
+// they sweep one of each. Scalar operations, IEEE roots and quotients, 68
+// instructions an element, took 1083 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -94,6 +95,43 @@ __device__ __forceinline__ float sqrt_fast(float x) {  // within one unit
     float r;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+__device__ __forceinline__ float rsqrt_fast(float x) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Roots of four pairs, rounded to nearest but for a few in a million that fall a unit
+// short: s = v / sqrt(v) from the hardware's reciprocal root, then Newton's step
+// s - (s^2 - v) / (2 sqrt(v)) with a fused residual (Markstein 1990). That wants v well
+// inside the normal range; a warp with another v anywhere takes IEEE roots.
+__device__ __forceinline__ void roots(const f2 (&v)[4], f2 (&r)[4]) {
+    unsigned out = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float a, b;
+        f2_split(v[j], a, b);
+        // Between 2^-100 and 2^100, read as integers.
+        out = max(out, max(__float_as_uint(a) - 0x0d800000u, __float_as_uint(b) - 0x0d800000u));
+    }
+    if (__any_sync(0xffffffffu, out >= 0x64000000u)) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float a, b;
+            f2_split(v[j], a, b);
+            r[j] = f2_pack(__fsqrt_rn(a), __fsqrt_rn(b));
+        }
+        return;
+    }
+    const f2 minus_one = f2_both(-1.0f), minus_half = f2_both(-0.5f);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float a, b;
+        f2_split(v[j], a, b);
+        const f2 y = f2_pack(rsqrt_fast(a), rsqrt_fast(b));
+        const f2 s = f2_mul(v[j], y);
+        r[j] = f2_fma(f2_fma(s, s, f2_mul(v[j], minus_one)), f2_mul(y, minus_half), s);
+    }
 }
 // The largest magnitude of three; NaN wins.
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {
@@ -330,9 +368,20 @@ __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block,
         const f2 gj = k.scaled ? f2_mul(g[j], k.gs) : g[j];
         m[j] = f2_add(f2_mul(k.b1, m[j]), f2_mul(k.c1, gj), k.one);
         v[j] = f2_add(f2_mul(k.b2, v[j]), f2_mul(f2_mul(k.c2, gj), gj), k.one);
+    }
+    if constexpr (EIGHT) {
+        roots(v, r);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float a, b;
+            f2_split(v[j], a, b);
+            r[j] = f2_pack(sqrt_fast(a), sqrt_fast(b));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
         float a, b;
-        f2_split(v[j], a, b);
-        r[j] = f2_pack(sqrt_fast(a), sqrt_fast(b));
         f2_split(f2_fma(r[j], k.rc2, k.eps), a, b);
         const f2 step = f2_mul(f2_mul(k.neg_a1, m[j]), f2_pack(rcp_fast(a), rcp_fast(b)));
         p[j] = f2_fma(k.keep, p[j], step);
@@ -351,17 +400,17 @@ __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block,
         }
         // Elements past the end hold zeros throughout, so they leave an amax as
         // it is. A block whose values are all below 2^-100 is held as zeros
-        // (448 / amax would overflow); one with an Inf or NaN reads back as NaN, so
-        // that it is not mistaken for a state. Half of the warp divides for m,
-        // half for r.
+        // (the inverse would overflow); one with an Inf or NaN reads back as NaN, so
+        // that it is not mistaken for a state. Half of the warp inverts m's amax,
+        // half r's.
         const float am = warp_amax(m), ar = warp_amax(r);
         const float amax = lane < 16 ? am : ar;
         float inv = 0.0f, s = 1.0f;
         if (!(amax <= 3.402823466e38f)) {
             inv = s = __uint_as_float(0x7fffffffu);
         } else if (amax >= 0x1p-100f) {
-            inv = 448.0f / amax;
-            s = amax / 448.0f;
+            inv = __frcp_rn(amax) * 448.0f;
+            s = amax * (1.0f / 448.0f);
         }
         if (lane == 0) t.ms[block] = s;
         if (lane == 16) t.vs[block] = s;

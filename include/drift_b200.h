@@ -639,7 +639,7 @@ DRIFT_API int drift_linear_xent_mean_dev(drift_ctx *ctx, const drift_xent *op, f
  * the last place and the root within one; eps is 0 or in [1e-30, 1e30].
  * state_bits 32: m and v are floats. state_bits 8: m and r are held as e4m3
  * codes with one float scale per 256 consecutive elements, code =
- * e4m3(x * (448 / amax)), value = code * (amax / 448), rounded to nearest or, with
+ * e4m3(x * (1 / amax * 448)), value = code * (amax * (1 / 448)), rounded to nearest or, with
  * `rounding` stochastic, by one draw an element in tensor order.
  */
 typedef struct drift_adamw {

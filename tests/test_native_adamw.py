@@ -22,10 +22,10 @@ def to8(x):
     amax = np.abs(b).max(1, keepdims=True)
     tiny = amax < F(2.0 ** -100)
     with np.errstate(divide="ignore", over="ignore"):
-        inv = np.where(tiny, F(0), F(448) / amax)
+        inv = np.where(tiny, F(0), (F(1) / amax) * F(448))
     y = np.clip(b * inv, F(-448), F(448))
     code = torch.from_numpy(y.reshape(-1)[:n].copy()).to(torch.float8_e4m3fn)
-    return code, np.where(tiny, F(1), amax / F(448))[:, 0].astype(F)
+    return code, np.where(tiny, F(1), amax * (F(1) / F(448)))[:, 0].astype(F)
 
 
 def from8(code, scale):
