@@ -35,7 +35,8 @@ namespace drift {
 // ------------------------------------------------------------------ one block's arithmetic
 
 // A source type. `key` of an element orders like its magnitude, its NaNs above
-// its Inf (kInf) and Inf above the rest, and holds its exponent.
+// its Inf (kInf) and Inf above the rest, and holds its exponent (of a subnormal of
+// the wider types: one below the normal ones', where the scale is at its limit).
 template <int TYPE> struct MxSrc;
 template <> struct MxSrc<DRIFT_T_F64> {
     using T = double;
@@ -54,10 +55,7 @@ template <> struct MxSrc<DRIFT_T_F32> {
     static constexpr unsigned kInf = 0x7f800000u;
     __device__ static V get(T x) { return x; }
     __device__ static unsigned key(T x) { return __float_as_uint(x) & 0x7fffffffu; }
-    // A subnormal has its own exponent, as its double has.
-    __device__ static int exponent(unsigned key) {
-        return key >> 23 ? (int)(key >> 23) - 127 : -118 - __clz(key);
-    }
+    __device__ static int exponent(unsigned key) { return (int)(key >> 23) - 127; }
 };
 template <> struct MxSrc<DRIFT_T_BF16> {
     using T = __nv_bfloat16;
@@ -74,18 +72,15 @@ template <> struct MxSrc<DRIFT_T_BF16> {
             : "r"(a), "r"(b));
         return m;
     }
-    // Both halves times powers of two, in fp32: exact, but for results far below the
-    // smallest code. A product and a -0 fused keep the sign of a zero.
+    // Both halves times powers of two, exact but for results far below the smallest
+    // code: two products an instruction, then widened.
     __device__ static void scaled2(unsigned w, float lo, float hi, float &a, float &b) {
-        asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n fma.rn.f32.bf16 %0, l, %3, %5;\n"
-            " fma.rn.f32.bf16 %1, h, %4, %5;\n}"
-            : "=f"(a), "=f"(b)
-            : "r"(w), "h"((unsigned short)(__float_as_uint(lo) >> 16)),
-              "h"((unsigned short)(__float_as_uint(hi) >> 16)), "f"(-0.0f));
+        const unsigned k = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(w) : "r"(k));
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
     }
-    __device__ static int exponent(unsigned key) {
-        return MxSrc<DRIFT_T_F32>::exponent(key << 16);
-    }
+    __device__ static int exponent(unsigned key) { return (int)(key >> 7) - 127; }
 };
 template <> struct MxSrc<DRIFT_T_FP16> {
     using T = __half;
@@ -254,22 +249,25 @@ template <int TYPE> struct MxRaw8 {
     }
 };
 
-// The scale of a block from its key, and the factor 2^-shared. Key 0 is a block
-// of zeros, which callers hold as +0 whatever the signs.
+// The scale of a block from its key, and the factor 2^-shared, for a headroom of 1
+// at most: then shared is below 127 (but of large doubles), the factor a normal
+// number, and subnormals' scales are at the lower limit whatever their exponent.
+// Key 0 is a block of zeros, which callers hold as +0 whatever the signs.
 template <class V> struct MxFactor {
     int shared;
     V down;
 };
-__device__ __forceinline__ float mx_down(int shared, float) {
-    return shared < 127 ? __uint_as_float((unsigned)(127 - shared) << 23) : 0x1p-127f;
-}
-__device__ __forceinline__ double mx_down(int shared, double) { return pow2(-shared); }
 template <int TYPE>
 __device__ __forceinline__ MxFactor<typename MxSrc<TYPE>::V> mx_factor(unsigned key, int headroom) {
     MxFactor<typename MxSrc<TYPE>::V> f;
-    const int e = MxSrc<TYPE>::exponent(key) - 2 + headroom;
-    f.shared = key ? max(-127, min(127, e)) : 0;
-    f.down = mx_down(f.shared, f.down);
+    int e = max(MxSrc<TYPE>::exponent(key) + (headroom - 2), -127);
+    if constexpr (TYPE == DRIFT_T_F64) {
+        e = min(e, 127);
+        f.down = __longlong_as_double((long long)(1023 - e) << 52);
+    } else {
+        f.down = __uint_as_float((unsigned)(127 - e) << 23);
+    }
+    f.shared = key ? e : 0;
     return f;
 }
 
@@ -312,6 +310,7 @@ struct MxCast {
     const void *src;
     int64_t rows, cols, row_stride;
     int headroom, rm;
+    bool quick;                        // to nearest, headroom 1 at most
     bool vec, wide;                    // rows start 16-byte, 32-byte aligned
     uint8_t *codes, *scales;           // blocks along rows
     uint8_t *codes_t, *scales_t;       // blocks down columns: the transpose, packed
@@ -391,7 +390,7 @@ __device__ __forceinline__ unsigned mx_cast8(const MxCast &a, const MxRaw8<TYPE>
     key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
     key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
     V x[8];
-    if (__all_sync(0xffffffffu, key < S::kInf) && a.rm == DRIFT_NEAREST_EVEN) {
+    if (__all_sync(0xffffffffu, key < S::kInf) && a.quick) {
         const MxFactor<V> f = mx_factor<TYPE>(key, a.headroom);
         shared = f.shared;
         if (a.clamped) {
@@ -612,7 +611,7 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
             m = S::max2(m, u[j]);
         }
         const unsigned key[2] = {m & 0x7fffu, m >> 16 & 0x7fffu};
-        if (max(key[0], key[1]) < S::kInf && a.rm == DRIFT_NEAREST_EVEN) {
+        if (max(key[0], key[1]) < S::kInf && a.quick) {
             const MxFactor<V> f0 = mx_factor<TYPE>(key[0], a.headroom);
             const MxFactor<V> f1 = mx_factor<TYPE>(key[1], a.headroom);
             shared[0] = f0.shared, shared[1] = f1.shared;
@@ -650,7 +649,7 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
                                                 word * sizeof(T));
             key = max(key, S::key(x[j]));
         }
-        if (key < S::kInf && a.rm == DRIFT_NEAREST_EVEN) {
+        if (key < S::kInf && a.quick) {
             const MxFactor<V> f = mx_factor<TYPE>(key, a.headroom);
             shared[0] = f.shared;
             unsigned *wp = reinterpret_cast<unsigned *>(&codes[0]);
@@ -746,6 +745,7 @@ int launch_mx4_quantize(int headroom, int rm, int type, const void *src, int64_t
     a.src = src;
     a.rows = rows, a.cols = cols, a.row_stride = row_stride;
     a.headroom = headroom, a.rm = rm;
+    a.quick = rm == DRIFT_NEAREST_EVEN && headroom <= 1;
     const uintptr_t at = reinterpret_cast<uintptr_t>(src) | (uintptr_t)(row_stride * size[type]);
     a.vec = at % 16 == 0, a.wide = at % 32 == 0;
     a.codes = codes, a.scales = scales, a.codes_t = codes_t, a.scales_t = scales_t;

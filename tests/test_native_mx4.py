@@ -31,6 +31,22 @@ def oracle_rows(x, p):
     return out, clamps
 
 
+@pytest.mark.parametrize("headroom", [-4, 2, 5])
+@pytest.mark.parametrize("dt", list(DT))
+def test_cast_with_other_headrooms(headroom, dt):
+    p = P["nearest"].to_builder("h").mx_headroom(headroom).build()
+    x = source(70, 200, dt, 21)
+    x[0, :32] = torch.tensor([2.0 ** -130, 2.0 ** -132] + [0.0] * 30).to(DT[dt])
+    x[1, :32] = 3e38 if dt != "f16" else 6e4
+    host = x.double().cpu().numpy()
+    for axis, h in ((1, host), (0, np.ascontiguousarray(host.T))):
+        want, clamps = oracle_rows(h, p)
+        c = torch.zeros(1, dtype=torch.int64, device="cuda")
+        q = d.mx4_quantize_dev(p, x, axis=axis, **{"d_clamped" if axis else "d_clamped_t": c})
+        v = d.mx4_dequantize_dev(q).cpu().numpy()
+        assert (v.view(np.int64) == want.view(np.int64)).all() and int(c) == clamps
+
+
 def source(rows, cols, dt, seed, edges=True):
     rs = np.random.default_rng(seed)
     x = heavy_tailed(rs, rows * cols, 2.0).reshape(rows, cols)
