@@ -14,10 +14,11 @@
 // of 128 x 128 (64 of the wider types) in shared memory; where both directions are
 // wanted they read the same tile, so the source is read once.
 //
-// Measured on one B200: rows of 4096 x 4096 fp32 in 12.4 us (6.15 TB/s, 95 % of the
-// copy rate), of 8192 x 8192 bf16 in 35 us (4.8 TB/s), both axes in 75 us (2.7 TB/s).
-// 16-bit sources are bound by instructions, 12 an element and axis: a conversion
-// instruction makes two codes, and each element is widened and scaled on the way.
+// Measured on one B200: rows of 8192 x 8192 bf16 in 33 us (5.2 TB/s, 80 % of the copy
+// rate), columns in 39 us, both in 70 us (2.9 TB/s); rows of 4096 x 4096 fp32 in 10.3
+// us (partly from L2), both axes in 23 us. 16-bit sources are bound by instructions,
+// some 11 an element and axis: a conversion instruction makes two codes, and each
+// element is widened and scaled on the way.
 #include <algorithm>
 #include <type_traits>
 
@@ -544,20 +545,28 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
     constexpr int kGroups = G::kCols / 8;  // groups of eight in a row of the tile
     const bool whole = a.vec && r0 + kMxTr <= a.rows && c0 + G::kCols <= a.cols;
     MxRaw8<TYPE> raw[G::kLoads];
+    constexpr int kStep = 256 / kGroups;  // rows from one load to the next
+    const int row_t = tid / kGroups, col_t = tid % kGroups * 8;
+    {
+        const T *p = static_cast<const T *>(a.src) + (r0 + row_t) * a.row_stride + c0 + col_t;
+        const int64_t down = kStep * a.row_stride;
+        if (whole) {
 #pragma unroll
-    for (int i = 0; i < G::kLoads; i++) {
-        const int at = i * 256 + tid, r = at / kGroups, c = at % kGroups * 8;
-        const int valid = r0 + r < a.rows
-                              ? (int)max((int64_t)0, min((int64_t)8, a.cols - c0 - c)) : 0;
-        const T *p = static_cast<const T *>(a.src) + (r0 + r) * a.row_stride + c0 + c;
-        raw[i] = whole ? mx_load_whole<TYPE>(p, a.wide) : mx_load8<TYPE>(a.vec, p, valid);
+            for (int i = 0; i < G::kLoads; i++, p += down) raw[i] = mx_load_whole<TYPE>(p, a.wide);
+        } else {
+            const int valid = (int)max((int64_t)0, min((int64_t)8, a.cols - c0 - col_t));
+#pragma unroll
+            for (int i = 0; i < G::kLoads; i++, p += down)
+                raw[i] = mx_load8<TYPE>(a.vec, p, r0 + row_t + i * kStep < a.rows ? valid : 0);
+        }
     }
+    {
+        unsigned char *to = mx_smem + row_t * G::kLdBytes + col_t * sizeof(T);
 #pragma unroll
-    for (int i = 0; i < G::kLoads; i++) {
-        const int at = i * 256 + tid, r = at / kGroups, c = at % kGroups * 8;
-        uint4 *to = reinterpret_cast<uint4 *>(mx_smem + r * G::kLdBytes + c * sizeof(T));
+        for (int i = 0; i < G::kLoads; i++)
 #pragma unroll
-        for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++) to[j] = raw[i].w[j];
+            for (int j = 0; j < MxRaw8<TYPE>::kVecs; j++)
+                reinterpret_cast<uint4 *>(to + i * kStep * G::kLdBytes)[j] = raw[i].w[j];
     }
 
     if (a.codes) {
@@ -565,7 +574,7 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
         int err = 0;
         const int blocks = (int)mx4_blocks(a.cols), k_tiles = (int)mx4_k_tiles(a.cols);
         const int64_t row_bytes = (int64_t)blocks * 16;
-        const int r = tid / kGroups, block = (int)(c0 >> 5) + tid % kGroups / 4;
+        const int r = row_t, block = (int)(c0 >> 5) + tid % kGroups / 4;
         const bool in_cols = block < blocks;
         uint8_t *codes = a.codes + (r0 + r) * row_bytes + c0 / 2 + tid % kGroups * 4;
         uint8_t *scales = a.scales + ((int64_t)tile_r * k_tiles + block / 4) * kMxTileBytes +
@@ -573,7 +582,6 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
         uint64_t draw = (uint64_t)(r0 + r) * a.cols + c0 + tid % kGroups * 8;
 #pragma unroll
         for (int i = 0; i < G::kLoads; i++) {
-            constexpr int kStep = 256 / kGroups;  // rows from one load to the next
             const int at = r + i * kStep;
             int shared;
             const unsigned w = mx_cast8<TYPE>(a, raw[i], 8, state, draw, shared, clamps, err);
@@ -686,12 +694,16 @@ __global__ void __launch_bounds__(256, sizeof(typename MxSrc<TYPE>::T) == 8 ? 2 
     }
     mx_finish(clamps, err, a.clamped_t, a.err);
     __syncthreads();
+    {
+        const int c = tid >> 2, q = tid & 3;
+        uint8_t *to = a.codes_t + (c0 + c) * blocks * 16 + (r0 / 32 + q) * 16;
+        const bool in = r0 + q * 32 < a.rows;
 #pragma unroll
-    for (int i = 0; i < G::kCols * 4 / 256; i++) {
-        const int at = i * 256 + tid, c = at >> 2, q = at & 3;
-        if (c0 + c < a.cols && r0 + q * 32 < a.rows)
-            *reinterpret_cast<uint4 *>(a.codes_t + (c0 + c) * blocks * 16 + (r0 / 32 + q) * 16) =
-                *reinterpret_cast<const uint4 *>(mx_smem + c * 80 + q * 16);
+        for (int i = 0; i < G::kCols / 64; i++) {
+            if (in && c0 + c + i * 64 < a.cols)
+                *reinterpret_cast<uint4 *>(to + i * 64 * blocks * 16) =
+                    *reinterpret_cast<const uint4 *>(mx_smem + (c + i * 64) * 80 + q * 16);
+        }
     }
 }
 
