@@ -3,8 +3,8 @@
 // itself. Every kernel launched with launch_pdl calls pdl_wait() in every thread
 // before its first access to global memory (so that a chain of them is ordered:
 // the wait returns once the kernel before has ended, which had waited in turn)
-// and pdl_trigger() to let the next one be set up. A chain of five small kernels
-// is 1 to 1.5 us a kernel shorter for it.
+// and pdl_trigger() to let the next one be set up. Cast and
+// product of 64 x 2048 x 2048 take 6.4 us in a row for it, 7.9 without.
 #pragma once
 
 #include <cuda_runtime.h>

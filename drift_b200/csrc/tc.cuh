@@ -15,22 +15,23 @@
 // Warps: 0-7 epilogue (two per quadrant of TMEM lanes, 128 columns each), 8
 // fetches with TMA, 9 allocates TMEM and, in the pair's first CTA, issues the
 // MMAs, 10 issues KIND_MX4's copies of scales to TMEM, in a thread of its own so
-// that they run beside the MMAs, and 11 completes the group. A stage's barrier `full` sits
-// in the first CTA and counts both CTAs' bytes; a commit of the stage's MMAs frees
-// it in both CTAs. The accumulator passes to the epilogue by `acc_full` (a commit
-// to both) and back by `acc_empty` (first CTA, one arrival an epilogue warp of
-// either). The epilogue moves its 128 columns to registers first and then hands
-// TMEM back, so the next tile's MMAs overlap its arithmetic and stores. KIND_16
-// has two accumulators (2 x 256 columns); KIND_MX4 has one, and 24 columns of
-// scales a stage.
+// that they run beside the MMAs, and 11 completes the group. A stage's barrier
+// `full` sits in the first CTA and counts both CTAs' bytes; a commit of the stage's
+// MMAs frees it in both CTAs. The accumulator passes to the epilogue by `acc_full`
+// (a commit to both) and back by `acc_empty` (first CTA, one arrival an epilogue
+// warp of either). The epilogue moves its 128 columns to registers first and then
+// hands TMEM back, so the next tile's MMAs overlap its arithmetic and stores.
+// KIND_16 has two accumulators (2 x 256 columns); KIND_MX4 has one, and 24 columns
+// of scales a stage.
 //
 // Measured on one B200: KIND_16 1.49 PFLOP/s (92 % of a library product's rate) over
 // 4096 x 131072 x 4096 in a burst, 1.2 under the power cap. KIND_MX4 5.07 PFLOP/s at
 // 8192^3, 4.5 at 8192 x 8192 x 4096 (issued from the MMAs' thread, the scale copies
 // queued between them, 60 cycles each: 3.8 and 3.4; copied with tcgen05.st by warps
-// of their own, 2.7 and 2.5). What bounds both now is shared memory: a stage is
-// written once and read by both CTAs' MMAs, 64 KiB of its 128 bytes a cycle in the
-// 512 cycles of the MMAs.
+// of their own, 2.7 and 2.5). The tensor pipe is busy 63 to 68 % of KIND_16's time at
+// 2048 x 32768 x 4096 under the counters' cold caches, DRAM 9 to 16 %. By count shared
+// memory is the next bound: a stage is written once and read by both CTAs' MMAs,
+// 64 KiB in their 512 cycles, at 128 bytes a cycle all there is.
 //
 // Every wait is bounded; one that gives up flags DEV_ERR_TIMEOUT and the
 // kernel drains and returns.
@@ -190,6 +191,11 @@ struct Args {
     int k_stages;                // stages of the whole contraction
     int splits;                  // the contraction is cut into this many parts
     int run = 1 << 30;           // KIND_16: stages summed in TMEM before registers take over
+    // Whether the next kernel is set up while the last tiles run. Good before another
+    // product or a join of a few small CTAs (2048^3 products in a row: 11.6 -> 10.95
+    // us), bad before a kernel of many CTAs, which wait where the tiles work (the
+    // gradients of 64 x 2048 x 96: 41.1 -> 45.6 us).
+    bool early = true;
     int *err;
 };
 
@@ -446,7 +452,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     // Not before: a small kernel set up early would crowd on the first SMs to fall
     // free (a join of 32 CTAs then takes twice its time).
-    pdl_trigger();
+    if (args.early) pdl_trigger();
     if (!ok) {
         atomicOr(args.err, DEV_ERR_TIMEOUT);
         // Give copies and MMAs in flight time to land before TMEM and shared

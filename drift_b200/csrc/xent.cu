@@ -642,6 +642,7 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
         tc::Args a;
         if (!logit_args(a, op, v0, n, BF16, err)) return DRIFT_ECUDA;
         const float *bias = op->bias ? op->bias + v0 : nullptr;
+        a.early = !db;
         int rc;
         if (db) {
             const GradEpi<T, true> epi{d,   p.ld,  bias,  n_t,   n,   v0, rows,
@@ -665,6 +666,7 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
             a.m_tiles = tiles(n_t), a.n_tiles = tiles(dep), a.k_stages = stages(n);
             a.run = kGradRun;
             a.splits = std::min(p.splits, a.k_stages);
+            a.early = p.direct;
             if (p.direct) {
                 const StoreEpi<T> epi{dx, dx_stride, n_t, dep, nullptr, undo, beta,
                                       rows_aligned(dx, dx_stride)};
@@ -681,7 +683,7 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
                 !tc::encode_16(&a.b, BF16, x, dep, n_t, p.x_ld, false))
                 return DRIFT_ECUDA;
             a.m_tiles = tiles(n), a.n_tiles = tiles(dep), a.k_stages = stages(n_t);
-            a.splits = 1, a.run = kGradRun;
+            a.splits = 1, a.run = kGradRun, a.early = p.direct;
             T *to = dw + v0 * dw_stride;
             const StoreEpi<T> epi{to,      dw_stride, n,    dep,
                                   nullptr, undo,      beta, rows_aligned(to, dw_stride)};
@@ -709,7 +711,7 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
     const float scale = BF16 ? 1.0f : 32768.0f, beta = 1.0f / scale;
     tc::Args a;
     if (!logit_args(a, op, 0, n, BF16, err)) return DRIFT_ECUDA;
-    a.splits = std::min(p.splits, a.k_stages);
+    a.splits = std::min(p.splits, a.k_stages), a.early = false;
     int rc = tc::launch<tc::KIND_16, BF16, false, false>(
         a, PartEpi{logits, p.part, p.ld, n_t, n, false}, sm_count(), st);
     if (rc) return rc;
@@ -732,6 +734,7 @@ static int mean_kept(const drift_xent *op, const KeptPlan &p, float *mean, T *dx
             return DRIFT_ECUDA;
         a.m_tiles = tiles(n_t), a.n_tiles = tiles(dep), a.k_stages = stages(n);
         a.splits = std::min(p.dx_splits, a.k_stages), a.run = kGradRun;
+        a.early = a.splits == 1;
         if (a.splits == 1) {
             const StoreEpi<T> epi{dx,      dx_stride, n_t,  dep,
                                   nullptr, inv,       beta, rows_aligned(dx, dx_stride)};
