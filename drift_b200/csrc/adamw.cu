@@ -159,8 +159,8 @@ __device__ __forceinline__ Raw8 load_raw(const void *p, int type, int64_t i, int
     if (type == DRIFT_T_F32) {
         const float *f = static_cast<const float *>(p) + i;
         if (whole) {
-            r.w[0] = __ldg(reinterpret_cast<const uint4 *>(f));
-            r.w[1] = __ldg(reinterpret_cast<const uint4 *>(f) + 1);
+            r.w[0] = *reinterpret_cast<const uint4 *>(f);
+            r.w[1] = reinterpret_cast<const uint4 *>(f)[1];
         } else {
             unsigned *u = reinterpret_cast<unsigned *>(r.w);
 #pragma unroll
@@ -169,7 +169,7 @@ __device__ __forceinline__ Raw8 load_raw(const void *p, int type, int64_t i, int
     } else {
         const uint16_t *h = static_cast<const uint16_t *>(p) + i;
         if (whole) {
-            r.w[0] = __ldg(reinterpret_cast<const uint4 *>(h));
+            r.w[0] = *reinterpret_cast<const uint4 *>(h);
         } else {
             unsigned *u = reinterpret_cast<unsigned *>(r.w);
 #pragma unroll
@@ -241,7 +241,7 @@ __device__ __forceinline__ void store8(void *p, int type, int64_t i, int valid, 
 
 __device__ __forceinline__ uint64_t load_codes(const void *p, int64_t i, int valid, bool whole) {
     const uint8_t *c = static_cast<const uint8_t *>(p) + i;
-    if (whole) return __ldg(reinterpret_cast<const unsigned long long *>(c));
+    if (whole) return *reinterpret_cast<const uint64_t *>(c);
     uint64_t w = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++)

@@ -141,7 +141,7 @@ template <class T> struct StoreEpi {
         if (bias) {
 #pragma unroll
             for (int j = 0; j < 128; j++)
-                if (col + j < cols) v[j] += __ldg(bias + col + j);
+                if (col + j < cols) v[j] += bias[col + j];
         }
         if (vec) {
             T *p = c + row0 * stride + col;

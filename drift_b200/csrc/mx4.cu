@@ -15,8 +15,8 @@
 // wanted they read the same tile, so the source is read once.
 //
 // Measured on one B200: rows of 8192 x 8192 bf16 in 33 us (5.2 TB/s, 80 % of the copy
-// rate), columns in 39 us, both in 70 us (2.9 TB/s); rows of 4096 x 4096 fp32 in 10.3
-// us (partly from L2), both axes in 23 us. 16-bit sources are bound by instructions,
+// rate), columns in 39 us, both in 70 us (2.9 TB/s); rows of 4096 x 4096 fp32 in 12.3
+// us (6.2 TB/s), both axes in 23 us. 16-bit sources are bound by instructions,
 // some 11 an element and axis: a conversion instruction makes two codes, and each
 // element is widened and scaled on the way.
 #include <algorithm>
@@ -330,13 +330,13 @@ __device__ __forceinline__ MxRaw8<TYPE> mx_load_whole(const typename MxSrc<TYPE>
     if (kVecs > 1 && wide) {
 #pragma unroll
         for (int j = 0; j + 1 < kVecs; j += 2)
-            asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                 : "=r"(r.w[j].x), "=r"(r.w[j].y), "=r"(r.w[j].z), "=r"(r.w[j].w),
                   "=r"(r.w[j + 1].x), "=r"(r.w[j + 1].y), "=r"(r.w[j + 1].z), "=r"(r.w[j + 1].w)
                 : "l"(reinterpret_cast<const uint4 *>(p) + j));
     } else {
 #pragma unroll
-        for (int j = 0; j < kVecs; j++) r.w[j] = __ldg(reinterpret_cast<const uint4 *>(p) + j);
+        for (int j = 0; j < kVecs; j++) r.w[j] = reinterpret_cast<const uint4 *>(p)[j];
     }
     return r;
 }
@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(256) mx4_values_kernel(const uint8_t *codes,
         for (uint32_t g = blockIdx.x * 256 + threadIdx.x; g < groups; g += gridDim.x * 256) {
             const int64_t col = (int64_t)g * 8;
             const unsigned w =
-                __ldg(reinterpret_cast<const unsigned *>(codes + row * row_bytes + col / 2));
+                *reinterpret_cast<const unsigned *>(codes + row * row_bytes + col / 2);
             const int shared = (int)scales[mx4_scale_offset(row, col >> 5, k_tiles)] - 127;
             __align__(16) T v[8];
 #pragma unroll

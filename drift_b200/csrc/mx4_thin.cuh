@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NT>::per_sm) thin_kernel(const
                         tc::wait(&acc_full, 0, (long long)(k1 - k0) * tc::kRoundsPerStage));
         tc::fence_after();
         const int64_t r = (int64_t)tw * 128 + warp * 32 + lane;
-        const float b = args.bias && r < args.rows ? __ldg(args.bias + r) : 0.0f;
+        const float b = args.bias && r < args.rows ? args.bias[r] : 0.0f;
         T *c = static_cast<T *>(args.c) + r;
 #pragma unroll
         for (int j0 = 0; j0 < NT; j0 += 16) {
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NT>::per_sm) thin_kernel(const
         float b[4];
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            b[i] = args.bias && r + i < args.rows ? __ldg(args.bias + r + i) : 0.0f;
+            b[i] = args.bias && r + i < args.rows ? args.bias[r + i] : 0.0f;
         const int t1 = min((int)(NT * (rank + 1) / ranks),
                            (int)min(args.tokens - (int64_t)tt * NT, (int64_t)NT));
         unsigned from[8];

@@ -3,8 +3,10 @@
 // itself. Every kernel launched with launch_pdl calls pdl_wait() in every thread
 // before its first access to global memory (so that a chain of them is ordered:
 // the wait returns once the kernel before has ended, which had waited in turn)
-// and pdl_trigger() to let the next one be set up. Cast and
-// product of 64 x 2048 x 2048 take 6.4 us in a row for it, 7.9 without.
+// and pdl_trigger() to let the next one be set up. They read global
+// memory with plain loads: one marked as read-only for the kernel's life may be
+// moved before the wait. Cast and product of 64 x 2048 x 2048 take 6.4 us in a row
+// for it, 7.9 without.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -95,7 +95,7 @@ __device__ __forceinline__ void finish_logits(float (&v)[128], int64_t col, int6
     if (bias) {
 #pragma unroll
         for (int j = 0; j < 128; j++)
-            if (col + j < cols) v[j] += __ldg(bias + col + j);
+            if (col + j < cols) v[j] += bias[col + j];
     }
     if (col + 128 > cols) {
 #pragma unroll
@@ -329,7 +329,7 @@ struct CopyRows {
         const uint4 *f = from + row * from_ld;
         uint4 *t = to + row * to_ld;
         for (int64_t i = threadIdx.x; i < units; i += blockDim.x)
-            t[i] = on ? __ldg(f + i) : make_uint4(0, 0, 0, 0);
+            t[i] = on ? f[i] : make_uint4(0, 0, 0, 0);
     }
 };
 __global__ void __launch_bounds__(128) xent_copy_kernel(CopyRows xs, XentRows x) {
@@ -514,6 +514,7 @@ static KeptPlan kept_plan(const drift_xent *op) {
     p.ld = up(op->vocab, 8);
     p.use = op->tokens > 0 && op->vocab <= 32768 && t * p.ld <= (16LL << 20);
     p.part = t * p.ld;
+    if (!p.use) return p;
     // Few tiles: the contractions are cut, down to two stages a part here, where a
     // part is a pass over the logits in L2, and 16 for dx.
     const int lt = tiles(t) * tiles(op->vocab), dt = tiles(t) * tiles(op->depth);
