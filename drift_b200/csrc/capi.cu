@@ -1185,6 +1185,10 @@ static bool misaligned(const void *p, unsigned to) {
     return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0;
 }
 
+static unsigned type_bytes(int type) {  // DRIFT_T_*
+    return type == DRIFT_T_F64 ? 8 : type == DRIFT_T_F32 ? 4 : 2;
+}
+
 // Rows and columns that the packed form's 32-bit indices reach.
 static bool mx4_shape_ok(int64_t rows, int64_t cols) {
     return rows >= 0 && cols >= 0 && rows < (1LL << 31) && cols < (1LL << 31) &&
@@ -1217,6 +1221,7 @@ int drift_mx4_quantize_dev(drift_ctx *ctx, const drift_policy *p, int rounding, 
     if (rows == 0 || cols == 0) return DRIFT_OK;
     if (!d_src || !d_codes != !d_scales || !d_codes_t != !d_scales_t || (!d_codes && !d_codes_t))
         return fail(DRIFT_EINVAL, "null pointer");
+    if (misaligned(d_src, type_bytes(type))) return fail(DRIFT_EINVAL, "misaligned source");
     if (misaligned(d_codes, 16) || misaligned(d_scales, 16) || misaligned(d_codes_t, 16) ||
         misaligned(d_scales_t, 16))
         return fail(DRIFT_EINVAL, "codes and scales must be 16-byte aligned");
@@ -1246,6 +1251,7 @@ int drift_mx4_dequantize_dev(drift_ctx *ctx, const drift_mx4 *q, int type, void 
         return fail(DRIFT_EINVAL, "bad arguments");
     if (q->rows == 0 || q->cols == 0) return DRIFT_OK;
     if (!d_dst) return fail(DRIFT_EINVAL, "null pointer");
+    if (misaligned(d_dst, type_bytes(type))) return fail(DRIFT_EINVAL, "misaligned output");
     rc = launch_mx4_dequantize(q, type, d_dst, q->rows > 1 ? row_stride : q->cols,
                                pick(ctx, stream));
     return rc ? fail(rc, "mx4 dequantize launch") : DRIFT_OK;
@@ -1263,15 +1269,23 @@ int drift_mx4_gemm_dev(drift_ctx *ctx, const drift_mx4 *A, const drift_mx4 *B,
         return fail(DRIFT_EINVAL, "bad arguments");
     if (A->rows == 0 || B->rows == 0) return DRIFT_OK;
     if (!d_C) return fail(DRIFT_EINVAL, "null pointer");
+    if (misaligned(d_C, type_bytes(type)) || misaligned(d_bias, 4))
+        return fail(DRIFT_EINVAL, "misaligned output or bias");
     rc = launch_mx4_gemm(A, B, d_bias, type, d_C, A->rows > 1 ? c_stride : B->rows, ctx->d_err(),
                          pick(ctx, stream));
     return rc ? fail(rc, "mx4 gemm launch") : DRIFT_OK;
 }
 
+// Sizes whose tiles and bytes the plans can count: x and W below 2^40 elements.
+static bool xent_shape_ok(const drift_xent *op) {
+    constexpr int64_t most = 1LL << 31;
+    return op && op->tokens >= 0 && op->depth >= 1 && op->vocab >= 1 && op->tokens < most &&
+           op->depth < most && op->vocab < most && op->tokens * op->depth <= (1LL << 40) &&
+           op->vocab * op->depth <= (1LL << 40);
+}
+
 static int check_xent(const drift_xent *op) {
-    if (!op || op->tokens < 0 || op->depth < 1 || op->vocab < 1 || op->tokens >= (1LL << 31) ||
-        op->depth >= (1LL << 31) || op->vocab >= (1LL << 31))
-        return fail(DRIFT_EINVAL, "bad shape");
+    if (!xent_shape_ok(op)) return fail(DRIFT_EINVAL, "bad shape");
     if ((op->type != DRIFT_T_BF16 && op->type != DRIFT_T_FP16) ||
         (op->target_bits != 32 && op->target_bits != 64))
         return fail(DRIFT_EINVAL, "bad type");
@@ -1280,11 +1294,13 @@ static int check_xent(const drift_xent *op) {
         misaligned(op->x, 16) || misaligned(op->w, 16))
         return fail(DRIFT_EINVAL, "rows of x and w must be 16-byte aligned");
     if (op->tokens && (!op->x || !op->w || !op->targets)) return fail(DRIFT_EINVAL, "null pointer");
+    if (misaligned(op->targets, op->target_bits / 8) || misaligned(op->bias, 4))
+        return fail(DRIFT_EINVAL, "misaligned targets or bias");
     return DRIFT_OK;
 }
 
 int drift_linear_xent_workspace(const drift_xent *op, int mode, int64_t *bytes) {
-    if (!op || !bytes || mode < 0 || mode > 2 || op->tokens < 0 || op->depth < 1 || op->vocab < 1)
+    if (!bytes || mode < 0 || mode > 2 || !xent_shape_ok(op))
         return fail(DRIFT_EINVAL, "bad shape");
     *bytes = xent_workspace(op, mode);
     return DRIFT_OK;
@@ -1315,6 +1331,8 @@ int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, const float
         return fail(DRIFT_EINVAL, "bad arguments");
     if ((d_dx && dx_stride < op->depth) || (d_dw && dw_stride < op->depth))
         return fail(DRIFT_EINVAL, "bad stride");
+    if (misaligned(d_dx, 2) || misaligned(d_dw, 2) || misaligned(d_db, 4))
+        return fail(DRIFT_EINVAL, "misaligned gradient");
     if (!d_ws || ws_bytes < xent_workspace(op, 1) || misaligned(d_ws, 256))
         return fail(DRIFT_EINVAL, "workspace too small or misaligned");
     rc = launch_xent_grad(op, d_lse, d_dloss, dloss_stride, d_dx, dx_stride, d_dw, dw_stride,
@@ -1331,6 +1349,8 @@ int drift_linear_xent_mean_dev(drift_ctx *ctx, const drift_xent *op, float *d_me
     if (rc) return rc;
     if (!d_mean || (d_dx && dx_stride < op->depth) || (d_dw && dw_stride < op->depth))
         return fail(DRIFT_EINVAL, "bad arguments");
+    if (misaligned(d_dx, 2) || misaligned(d_dw, 2) || misaligned(d_db, 4))
+        return fail(DRIFT_EINVAL, "misaligned gradient");
     if (!d_ws || ws_bytes < xent_workspace(op, 2) || misaligned(d_ws, 256))
         return fail(DRIFT_EINVAL, "workspace too small or misaligned");
     rc = launch_xent_mean(op, d_mean, d_dx, dx_stride, d_dw, dw_stride, d_db, d_ws, ctx->d_err(),

@@ -37,6 +37,28 @@ def test_cross_entropy_workspace_of_any_shape(mode, tokens, depth, vocab):
     assert LIB.drift_linear_xent_workspace(ctypes.byref(op), 3, ctypes.byref(out)) == _lib.EINVAL
 
 
+@pytest.mark.parametrize("tokens,depth,vocab", [
+    (-1, 8, 8), (4, 0, 8), (4, 8, 0), (1 << 31, 8, 8), (4, 1 << 31, 8), (4, 8, 1 << 31),
+    (1 << 24, 1 << 24, 8), (4, 1 << 24, 1 << 24), ((1 << 31) - 1, (1 << 31) - 1, 8)])
+def test_cross_entropy_workspace_refuses_what_no_memory_holds(tokens, depth, vocab):
+    op = _lib.DriftXent(tokens=tokens, depth=depth, vocab=vocab)
+    out = ctypes.c_int64()
+    for mode in range(3):
+        assert LIB.drift_linear_xent_workspace(ctypes.byref(op), mode,
+                                               ctypes.byref(out)) == _lib.EINVAL
+
+
+@pytest.mark.parametrize("tokens,depth,vocab", [(1 << 24, 1, 1 << 24), (1 << 24, 1 << 16, 256),
+                                                ((1 << 31) - 1, 512, (1 << 31) - 1)])
+def test_cross_entropy_workspace_of_the_longest_sides(tokens, depth, vocab):
+    """Their tiles, 65536 a side, are past 32 bits in number."""
+    op = _lib.DriftXent(tokens=tokens, depth=depth, vocab=vocab)
+    out = ctypes.c_int64()
+    for mode in range(3):
+        _lib.check(LIB.drift_linear_xent_workspace(ctypes.byref(op), mode, ctypes.byref(out)))
+        assert out.value >= 16 * tokens
+
+
 def test_a_null_context_is_refused():
     q, x, h = _lib.DriftMx4(), _lib.DriftXent(), _lib.DriftAdamW()
     p = d.policies.by_name("mxfp4").to_c()
