@@ -103,7 +103,7 @@ def _streamed(fn):
             _start()
         if stream is None:
             return fn(*args, **kw)
-        ctx = kw.get("ctx") or getattr(args[0], "ctx", None) or _lib.Context.current()
+        ctx = kw.get("ctx") or getattr(args[0] if args else None, "ctx", None) or _lib.Context.current()
         if stream.device.index != ctx.device:
             raise ValueError(f"stream on {stream.device}, context on device {ctx.device}")
         with torch.cuda.stream(stream):
@@ -434,7 +434,8 @@ class AdamW:
     r_scale], each a list like `params`. The step count lives on the device
     (d_step, int64), so a captured step replays as the next one. `copies`
     (a list with None where there is none) receive the new parameters in their
-    own type, for low-precision copies of float32 masters."""
+    own type, for low-precision copies of float32 masters. All of them keep the
+    memory they have here: new values are copied into it."""
 
     def __init__(self, params: Sequence, *, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.01, state_bits: int = 32,
@@ -508,10 +509,14 @@ class AdamW:
             if c is not None:
                 t.copy = call.ptr(c, f"copies[{i}]", numel=n[i])
                 t.copy_type = _type_of(c.dtype, f"copies[{i}]", low)
-        # Everything a step writes, in order of address: no two may share memory.
+        # Everything a step writes, in order of address: no two may share memory. It is held
+        # here too, so that the table's addresses stay good whatever becomes of the lists.
+        self._held = [x.detach() for part in (self.params, *self.state, self.copies,
+                                              [self.d_step, d_rng_state])
+                      for x in part if x is not None]
+        self._at = [p.data_ptr() for p in self.params]
         written = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size())
-                         for part in (self.params, *self.state, self.copies) for x in part
-                         if x is not None and x.numel())
+                         for x in self._held if x.numel())
         if any(a[1] > b[0] for a, b in zip(written, written[1:])):
             raise ValueError("parameters, moments and copies must not share memory")
 
@@ -527,6 +532,8 @@ class AdamW:
         if lr is not None:
             self.hyper.lr = float(lr)
         call = _Call(self.params[0], self.ctx)
+        if list(map(torch.Tensor.data_ptr, self.params)) != self._at:
+            raise ValueError("a parameter's memory was replaced: it belongs to the optimizer")
         sizes = self._sizes
         want = run = sizes
         try:

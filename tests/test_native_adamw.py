@@ -248,6 +248,21 @@ def test_zero_and_non_finite_blocks():
     assert (p[:256] == 1).all() and torch.isfinite(p[512:]).all()
 
 
+def test_memory_taken_at_construction_is_kept_and_replacing_it_is_refused():
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt, ref = d.AdamW([p.clone()]), d.AdamW([p])
+    opt.state[0][0] = torch.zeros(300, device="cuda")  # the list's, not the optimizer's
+    junk = [torch.full((300,), float("nan"), device="cuda") for _ in range(8)]
+    for _ in range(2):
+        opt.step([g])
+        ref.step([g])
+    assert torch.equal(opt.params[0], ref.params[0])
+    assert all(torch.isnan(j).all() for j in junk)
+    opt.params[0].data = torch.ones(300, device="cuda")
+    with pytest.raises(ValueError):
+        opt.step([g])
+
+
 def test_refusals():
     p = torch.zeros(8, device="cuda")
     opt = d.AdamW([p])

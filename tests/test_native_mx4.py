@@ -373,6 +373,9 @@ def test_a_stream_of_its_own():
     got = d.mx4_gemm_dev(q, W, stream=s)
     s.synchronize()
     assert torch.equal(got, want)
+    got = d.mx4_gemm_dev(a=q, b=W, stream=s)
+    s.synchronize()
+    assert torch.equal(got, want)
 
 
 def test_types_are_the_header_s():
