@@ -122,6 +122,31 @@ __device__ __forceinline__ void by_elements(const float (&v)[128], unsigned stag
     }
 }
 
+// Adds bias[col ...] to a thread's columns below `cols` (the others get 0 added). All
+// lanes want the same 128 numbers: each loads four of them, and the warp reads them
+// back from shared memory. (128 loads a thread from global memory, in the few
+// registers left beside v, took longer than the products of a tile up to 1024 deep:
+// cross entropy of 1024 x 50176 x 512 in 88 us with a bias, 57 without.)
+__device__ __forceinline__ void add_bias(float (&v)[128], const float *bias, int64_t col,
+                                         int64_t cols, unsigned staging, int lane) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int i = j * 32 + lane;
+        const float b = col + i < cols ? bias[col + i] : 0.0f;
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(staging + i * 4), "f"(b) : "memory");
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 128; j += 4) {
+        const uint4 b = smem_load16(staging + j * 4);
+        v[j] += __uint_as_float(b.x), v[j + 1] += __uint_as_float(b.y);
+        v[j + 2] += __uint_as_float(b.z), v[j + 3] += __uint_as_float(b.w);
+        // Here and not where the sums are used, lest both terms wait in registers.
+        asm volatile("" : "+f"(v[j]), "+f"(v[j + 1]), "+f"(v[j + 2]), "+f"(v[j + 3]));
+    }
+    __syncwarp();
+}
+
 // C = D * alpha (+ bias), rounded once.
 template <class T> struct StoreEpi {
     T *c;
@@ -138,11 +163,7 @@ template <class T> struct StoreEpi {
 #pragma unroll
             for (int j = 0; j < 128; j++) v[j] *= f;
         }
-        if (bias) {
-#pragma unroll
-            for (int j = 0; j < 128; j++)
-                if (col + j < cols) v[j] += bias[col + j];
-        }
+        if (bias) add_bias(v, bias, col, cols, staging, lane);
         if (vec) {
             T *p = c + row0 * stride + col;
             const int64_t left = cols - col;

@@ -91,12 +91,8 @@ __device__ __forceinline__ Stat join(Stat a, Stat b) {
 
 // Adds the bias; columns past the piece become -inf.
 __device__ __forceinline__ void finish_logits(float (&v)[128], int64_t col, int64_t cols,
-                                              const float *bias) {
-    if (bias) {
-#pragma unroll
-        for (int j = 0; j < 128; j++)
-            if (col + j < cols) v[j] += bias[col + j];
-    }
+                                              const float *bias, unsigned staging, int lane) {
+    add_bias(v, bias, col, bias ? cols : 0, staging, lane);
     if (col + 128 > cols) {
 #pragma unroll
         for (int j = 0; j < 128; j++)
@@ -112,10 +108,10 @@ struct StatsEpi {
     int64_t rows, cols, v0;
     XentRows x;
     __device__ __forceinline__ void run(float (&v)[128], int64_t row0, int64_t col, const tc::Work &,
-                                        int lane, unsigned) const {
+                                        int lane, unsigned staging) const {
         if (col >= cols) return;
         const int64_t row = row0 + lane;
-        finish_logits(v, col, cols, bias);
+        finish_logits(v, col, cols, bias, staging, lane);
         float m[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
         for (int j = 4; j < 128; j++) m[j & 3] = max_nan(m[j & 3], v[j]);
@@ -156,7 +152,7 @@ template <class T, bool DB> struct GradEpi {
                                         int lane, unsigned staging) const {
         if (col >= cols) return;
         const int64_t row = row0 + lane;
-        finish_logits(v, col, cols, bias);
+        finish_logits(v, col, cols, bias, staging, lane);
         bool bad = false;
         const int64_t t = row < rows ? x.at(row, bad) : -1;
         const float gi = t >= 0 ? (g ? g[row] : 1.0f) : 0.0f;
