@@ -417,6 +417,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int64_t row0 = (int64_t)w.m * kTile + (int)rank * kRows + quad * 32;
             const int64_t col = (int64_t)w.n * kTile + half * 128;
             const bool live = row0 < epi.rows && col < epi.cols;  // else nothing to do
+            // What the epilogue loads ahead of its accumulator.
+            const auto before = epi.before(row0 + lane, col, lane);
             float v[128];
             const int run = KIND == KIND_16 ? min(args.run, w.k1 - w.k0) : w.k1 - w.k0;
             for (int k = w.k0; k < w.k1; k += run, n_acc++) {
@@ -446,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (lane == 0) arrive_cluster(map_cta(smem_addr(&acc_empty[acc]), 0));
             }
             if (!ok) break;
-            if (live) epi.run(v, row0, col, w, lane, staging);
+            if (live) epi.run(v, before, row0, col, w, lane, staging);
         }
     }
 
