@@ -23,12 +23,14 @@
 // a handful of instructions and every access is one or two 16-byte loads or
 // stores a lane.
 //
-// Measured on one B200: 400M bf16 parameters with 8-bit moments in 720 us (5.6 TB/s,
-// 87 % of the copy rate; 752 with IEEE roots), 8.6M fp32 ones with 32-bit moments in
-// 41 us (5.9 TB/s). Each CTA on a stretch of its own took 60 % longer for the first:
-// the CTAs in flight then touch as many stretches of seven arrays, where side by side
-// they sweep one of each. Scalar operations, IEEE roots and quotients, 68
-// instructions an element, took 1083 us.
+// Measured on one B200: 200M bf16 parameters with 8-bit moments in 346 us (5.8 TB/s, 90 %
+// of the copy rate; 366 with a reciprocal that keeps subnormals), 8.6M fp32 ones with
+// 32-bit moments in 37 us (6.0 TB/s). With 8-bit moments it is near its instructions
+// too (46 an element, 75 % of the issue slots), and slows with the clocks: 400M take
+// 690 to 760 us. Each CTA on a stretch of its own took 60 % longer for the first: the
+// CTAs in flight then touch as many stretches of seven arrays, where side by side they
+// sweep one of each. Scalar operations, IEEE roots and quotients, 68 instructions an
+// element, took 1083 us for 400M.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -86,9 +88,12 @@ __global__ void adamw_prepare_kernel(int64_t *step, double b1, double b2, double
     }
 }
 
-__device__ __forceinline__ float rcp_fast(float x) {  // within one unit
+// Within one unit. The denominators are 0, Inf, NaN or well inside the normal range (a
+// root is above 2^-75, and eps is 0 or above 1e-30; a root is below 2^64, its factor
+// below 2^27), where flushing subnormals changes nothing.
+__device__ __forceinline__ float rcp_fast(float x) {
     float r;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ float sqrt_fast(float x) {  // within one unit
@@ -342,7 +347,6 @@ __device__ __forceinline__ void load_block(const AdamTensor &t, int64_t block, i
 struct Scalars {
     f2 b1, b2, c1, c2, eps, neg_a1, rc2, keep, gs, one;
     uint64_t state;
-    bool scaled;
 };
 
 template <bool EIGHT, bool SR, int PT, int GT, bool WHOLE>
@@ -365,7 +369,7 @@ __device__ __forceinline__ void update_block(const AdamTensor &t, int64_t block,
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const f2 gj = k.scaled ? f2_mul(g[j], k.gs) : g[j];
+        const f2 gj = f2_mul(g[j], k.gs);  // by 1 without a scale
         m[j] = f2_add(f2_mul(k.b1, m[j]), f2_mul(k.c1, gj), k.one);
         v[j] = f2_add(f2_mul(k.b2, v[j]), f2_mul(f2_mul(k.c2, gj), gj), k.one);
     }
@@ -468,8 +472,7 @@ __global__ void __launch_bounds__(kAdamThreads, EIGHT && !SR ? 4 : 2) adamw_kern
     k.b1 = f2_both(a.b1), k.b2 = f2_both(a.b2), k.c1 = f2_both(a.c1), k.c2 = f2_both(a.c2);
     k.eps = f2_both(a.eps), k.one = f2_both(a.one);
     k.neg_a1 = f2_both(-a.scal[0]), k.rc2 = f2_both(a.scal[1]), k.keep = f2_both(a.scal[2]);
-    k.scaled = a.grad_scale != nullptr;
-    k.gs = f2_both(k.scaled ? *a.grad_scale : 1.0f);
+    k.gs = f2_both(a.grad_scale ? *a.grad_scale : 1.0f);
     k.state = SR ? *a.rng : 0;
     // The usual types have code of their own; fp16, unaligned tensors and the last,
     // partial block of one take the general form.
