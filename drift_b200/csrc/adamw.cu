@@ -26,11 +26,11 @@
 // Measured on one B200: 200M bf16 parameters with 8-bit moments in 346 us (5.8 TB/s, 90 %
 // of the copy rate; 366 with a reciprocal that keeps subnormals), 8.6M fp32 ones with
 // 32-bit moments in 37 us (6.0 TB/s). With 8-bit moments it is near its instructions
-// too (46 an element, 75 % of the issue slots), and is slower on a hot card: 400M
-// take 762 us in turn with other work. Each CTA on a stretch of its own took 60 % longer for the first: the
-// CTAs in flight then touch as many stretches of seven arrays, where side by side they
-// sweep one of each. Scalar operations, IEEE roots and quotients, 68 instructions an
-// element, took 1083 us for 400M.
+// too (46 an element, 75 % of the issue slots), and is slower on a hot card: 400M take
+// 762 us in turn with other work. Each CTA on a stretch of its own took 60 % longer for
+// the first: the CTAs in flight then touch as many stretches of seven arrays, where
+// side by side they sweep one of each. Scalar operations, IEEE roots and quotients,
+// 68 instructions an element, took 1083 us for 400M.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
