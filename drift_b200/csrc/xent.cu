@@ -497,7 +497,9 @@ static GradPlan grad_plan(const drift_xent *op) {
     p.part = t * p.acc_ld;
     p.d = 0;
     p.sums = up(t * p.ld * 2, 256);
-    p.acc = p.sums + (op->bias ? up(up(t, 256) / 32 * p.ld * 4, 256) : 0);
+    // Whether db is wanted is not known here, and a bias does not say. A sixteenth of d for
+    // many tokens.
+    p.acc = p.sums + up(up(t, 256) / 32 * p.ld * 4, 256);
     p.scale = p.acc + (p.direct ? 0 : up(p.splits * p.part * 4, 256));
     p.x_ld = up(op->depth, 8);
     p.x = p.scale + 256;

@@ -604,7 +604,8 @@ typedef struct drift_xent {
     int32_t type;
 } drift_xent;
 /* Workspace bytes of drift_linear_xent_dev (mode 0), drift_linear_xent_grad_dev
- * (1) and drift_linear_xent_mean_dev (2). */
+ * (1) and drift_linear_xent_mean_dev (2), whichever outputs are wanted: a
+ * function of tokens, depth and vocab alone. */
 DRIFT_API int drift_linear_xent_workspace(const drift_xent *op, int mode, int64_t *bytes);
 /* Per row: d_loss (may be NULL) and d_lse, the log of the sum of exponentials.
  * d_mean (may be NULL): two floats, the mean loss of the rows that are not
@@ -614,8 +615,9 @@ DRIFT_API int drift_linear_xent_dev(drift_ctx *ctx, const drift_xent *op, float 
                           void *stream);
 /* Gradients, from d_lse of the forward call and the gradient of each row's
  * loss, d_dloss[i * dloss_stride] (stride 0: one value for all rows): d_dx
- * (tokens x depth) and d_dw (vocab x depth) of `type`, d_db (vocab floats); each
- * may be NULL. Overwritten, not added to. The logits are computed again. */
+ * (tokens x depth) and d_dw (vocab x depth) of `type`, d_db (vocab floats, with a
+ * bias or without); each may be NULL. Overwritten, not added to. The logits are
+ * computed again. */
 DRIFT_API int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, const float *d_lse,
                                const float *d_dloss, int64_t dloss_stride, void *d_dx,
                                int64_t dx_stride, void *d_dw, int64_t dw_stride, float *d_db,

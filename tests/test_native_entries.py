@@ -1,0 +1,106 @@
+"""The native operators' C entries, called as a C program calls them: parts that the
+Python layer ties together on their own, strides, buffers of the caller's that hold
+anything, and vocabularies of several pieces."""
+import ctypes
+
+import pytest
+
+import drift_b200 as d
+from drift_b200 import _lib, native
+from tests.test_native_xent import DT, IG, inputs
+
+torch = pytest.importorskip("torch")
+gpu = pytest.mark.gpu
+
+LIB = _lib.load()
+GUARD = 64 << 20  # bytes behind a workspace
+
+
+def xent_op(x, w, tg, b=None, ignore=IG):
+    return _lib.DriftXent(x.shape[0], x.shape[1], w.shape[0], x.stride(0), w.stride(0),
+                          x.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(),
+                          tg.data_ptr(), ignore, 64 if tg.dtype == torch.int64 else 32,
+                          native._BF16 if x.dtype == torch.bfloat16 else native._FP16)
+
+
+def workspace_bytes(op, mode):
+    n = ctypes.c_int64()
+    _lib.check(LIB.drift_linear_xent_workspace(op, mode, n))
+    return n.value
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class Entry:
+    """Outputs, and a workspace of exactly the bytes asked for with a guard behind it."""
+
+    def __init__(self, x, w, tg, b=None):
+        self.op = xent_op(x, w, tg, b)
+        self.keep = (x, w, tg, b)
+        self.dx, self.dw = torch.empty(x.shape, dtype=x.dtype, device="cuda"), torch.empty(
+            w.shape, dtype=w.dtype, device="cuda")
+        self.db = torch.empty(w.shape[0], device="cuda")
+
+    def workspace(self, mode, fill=0xA5):
+        n = workspace_bytes(self.op, mode)
+        self.buf = torch.full((n + GUARD,), fill, dtype=torch.uint8, device="cuda")
+        return self.buf.data_ptr(), n
+
+    def check_guard(self):
+        d.check_dev()
+        n = self.buf.numel() - GUARD
+        assert (self.buf[n:] == 0xA5).all()
+
+    def gradients(self, lse, g, stride, need_db=True):
+        at, n = self.workspace(1)
+        dep = self.op.depth
+        _lib.check(LIB.drift_linear_xent_grad_dev(
+            d.Context.current().handle, self.op, lse.data_ptr(), g.data_ptr(), stride, ptr(self.dx),
+            dep, ptr(self.dw), dep, ptr(self.db) if need_db else None, at, n,
+            torch.cuda.current_stream().cuda_stream))
+        self.check_guard()
+        return self.dx, self.dw, self.db
+
+    def mean(self):
+        at, n = self.workspace(2)
+        dep, loss = self.op.depth, torch.empty((), device="cuda")
+        _lib.check(LIB.drift_linear_xent_mean_dev(
+            d.Context.current().handle, self.op, loss.data_ptr(), ptr(self.dx), dep, ptr(self.dw),
+            dep, ptr(self.db), at, n, torch.cuda.current_stream().cuda_stream))
+        self.check_guard()
+        return loss, self.dx, self.dw, self.db
+
+
+# ------------------------------------------------------------------ db without a bias
+
+@pytest.mark.parametrize("mode", [1, 2])
+@pytest.mark.parametrize("tokens,depth,vocab", [(1, 8, 1), (600, 72, 33000), (4096, 64, 32769),
+                                                (1 << 20, 24, 2600)])
+def test_the_workspace_holds_column_sums_without_a_bias(tokens, depth, vocab, mode):
+    """db may be wanted without one: a float for 32 tokens and a column of a piece."""
+    op = _lib.DriftXent(tokens=tokens, depth=depth, vocab=vocab)
+    without = workspace_bytes(op, mode)
+    op.bias = 256
+    assert workspace_bytes(op, mode) == without
+    if mode == 1:
+        piece = min(-(-vocab // 8) * 8, max(256, (128 << 20) // tokens // 256 * 256))
+        assert without >= 2 * tokens * piece + -(-tokens // 32) * 4 * min(piece, vocab)
+
+
+@gpu
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("t,dep,v", [(33, 40, 257), (600, 72, 33000)])
+def test_bias_gradients_without_a_bias(t, dep, v, dt):
+    """Bit for bit those of a bias of zeros, and nothing behind the workspace is written."""
+    x, w, tg, _ = inputs(t, dep, v, dt, bias=False)
+    zero = torch.zeros(v, device="cuda")
+    _, lse = d.linear_xent_dev(x, w, tg)
+    g = torch.randn(t, device="cuda")
+    want = d.linear_xent_grad_dev(x, w, tg, lse, g, bias=zero)
+    for a, c in zip(Entry(x, w, tg).gradients(lse, g, 1), want):
+        assert torch.equal(a, c)
+    want = d.linear_xent_mean_dev(x, w, tg, bias=zero)
+    for a, c in zip(Entry(x, w, tg).mean(), want):
+        assert torch.equal(a, c)
