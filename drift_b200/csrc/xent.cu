@@ -154,6 +154,7 @@ template <class T, bool DB> struct GradEpi {
     int64_t rows, cols, v0;
     XentRows x;
     const float *lse, *g;  // g: null for 1 throughout
+    int64_t g_stride;
     const float *scale;    // the power of two that d is held times: device, or null
     float fixed;           // and the host's
     float *sums;           // DB: [row / 32][column], not scaled
@@ -165,7 +166,7 @@ template <class T, bool DB> struct GradEpi {
         finish_logits(v, col, cols, Bias4(bias, col, cols, lane), staging, lane);
         bool bad = false;
         const int64_t t = row < rows ? x.at(row, bad) : -1;
-        const float gi = t >= 0 ? (g ? g[row] : 1.0f) : 0.0f;
+        const float gi = t >= 0 ? (g ? g[row * g_stride] : 1.0f) : 0.0f;
         const float z = t >= 0 ? lse[row] : 0.0f;
         const int64_t at = t - v0 - col;
 #pragma unroll
@@ -254,13 +255,14 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const Stat *parts, int 
 
 // fp16: the power of two that brings the largest |g| into (2^14, 2^15], and its
 // inverse; 1 where no finite one would help.
-__global__ void __launch_bounds__(1024) xent_scale_kernel(const float *g, int64_t n, float *scale) {
+__global__ void __launch_bounds__(1024) xent_scale_kernel(const float *g, int64_t g_stride,
+                                                          int64_t n, float *scale) {
     pdl_trigger();
     pdl_wait();
     __shared__ unsigned sm[32];
     unsigned m = 0;
     for (int64_t i = threadIdx.x; i < n; i += 1024)
-        m = max(m, __float_as_uint(g[i]) & 0x7fffffffu);
+        m = max(m, __float_as_uint(g[i * g_stride]) & 0x7fffffffu);
     m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
     __syncthreads();
@@ -633,7 +635,8 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
     const bool one = g_stride == 0;
     float *scale = BF16 || one ? nullptr : reinterpret_cast<float *>(ws + p.scale);
     if (scale) {
-        const int rc = launch_pdl(xent_scale_kernel, dim3(1), 1024, 0, st, 0, g, n_t, scale);
+        const int rc = launch_pdl(xent_scale_kernel, dim3(1), 1024, 0, st, 0, g, g_stride, n_t,
+                                  scale);
         if (rc) return rc;
     }
     const float fixed = !BF16 && one ? 32768.0f : 1.0f;
@@ -654,15 +657,15 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
         a.early = !db;
         int rc;
         if (db) {
-            const GradEpi<T, true> epi{d,   p.ld,  bias,  n_t,   n,   v0, rows,
-                                       lse, row_g, scale, fixed, sums};
+            const GradEpi<T, true> epi{d,   p.ld,  bias,     n_t,   n,     v0,  rows,
+                                       lse, row_g, g_stride, scale, fixed, sums};
             rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
             if (!rc)
                 rc = launch_pdl(xent_colsum_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, st, 0,
                                 sums, (n_t + 31) / 32, n, n, sum_undo, db + v0);
         } else {
-            const GradEpi<T, false> epi{d,   p.ld,  bias,  n_t,   n,      v0, rows,
-                                        lse, row_g, scale, fixed, nullptr};
+            const GradEpi<T, false> epi{d,   p.ld,  bias,     n_t,   n,     v0,     rows,
+                                        lse, row_g, g_stride, scale, fixed, nullptr};
             rc = tc::launch<tc::KIND_16, BF16, false, false>(a, epi, sm_count(), st);
         }
         if (rc) return rc;

@@ -7,7 +7,7 @@ import pytest
 
 import drift_b200 as d
 from drift_b200 import _lib, native
-from tests.test_native_xent import DT, IG, inputs
+from tests.test_native_xent import DT, IG, check_grads, inputs
 
 torch = pytest.importorskip("torch")
 gpu = pytest.mark.gpu
@@ -103,4 +103,26 @@ def test_bias_gradients_without_a_bias(t, dep, v, dt):
         assert torch.equal(a, c)
     want = d.linear_xent_mean_dev(x, w, tg, bias=zero)
     for a, c in zip(Entry(x, w, tg).mean(), want):
+        assert torch.equal(a, c)
+
+
+# ------------------------------------------------------------------ weights by row
+
+@gpu
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("stride", [1, 2, 7])
+@pytest.mark.parametrize("t,dep,v", [(1, 64, 96), (65, 40, 257), (300, 72, 1000)])
+def test_strided_weights(t, dep, v, dt, stride):
+    """Row i's weight is d_dloss[i * dloss_stride]; what lies between is not read."""
+    x, w, tg, b = inputs(t, dep, v, dt, seed=1)
+    _, lse = d.linear_xent_dev(x, w, tg, bias=b)
+    g = torch.randn(t, device="cuda")
+    apart = torch.full((t * stride,), float("nan"), device="cuda")
+    apart[::stride] = g
+    # One row's weight by the C entry is a weight by row, through Python one for all rows.
+    if t == 1:
+        return check_grads(x, w, tg, b, g, Entry(x, w, tg, b).gradients(lse, apart, stride))
+    want = d.linear_xent_grad_dev(x, w, tg, lse, g, bias=b)
+    check_grads(x, w, tg, b, g, want)
+    for a, c in zip(Entry(x, w, tg, b).gradients(lse, apart, stride), want):
         assert torch.equal(a, c)
