@@ -20,8 +20,9 @@
 //             dW = d^T x from it, reading d and W where they lie (MN-major).
 //
 // fp16 holds d times a power of two (2^15, or with weights by row one that brings
-// the largest |g| near 2^15), so that small probabilities keep their bits; the
-// products undo it exactly. bf16 has fp32's range and needs none.
+// the largest finite |g| of the rows that count near 2^15), so that small
+// probabilities keep their bits; the products undo it exactly. bf16 has fp32's range
+// and needs none.
 //
 // Bound: the tensor cores for many tokens (8 T D V operations with the
 // gradient's second computation of the logits, against 6 T D V if they were
@@ -253,23 +254,27 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const Stat *parts, int 
     loss[row] = t >= 0 ? z - target[row] : 0.0f;  // may be target itself
 }
 
-// fp16: the power of two that brings the largest |g| into (2^14, 2^15], and its
-// inverse; 1 where no finite one would help.
+// fp16: the power of two that brings the largest finite |g| of a row with a gradient
+// into [2^14, 2^15), and its inverse; 1 where all are below 2^-96. An Inf or NaN spoils
+// its own row of dx, not the others' scale.
 __global__ void __launch_bounds__(1024) xent_scale_kernel(const float *g, int64_t g_stride,
-                                                          int64_t n, float *scale) {
+                                                          XentRows x, int64_t n, float *scale) {
     pdl_trigger();
     pdl_wait();
     __shared__ unsigned sm[32];
     unsigned m = 0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024)
-        m = max(m, __float_as_uint(g[i * g_stride]) & 0x7fffffffu);
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        bool bad = false;
+        const unsigned w = __float_as_uint(g[i * g_stride]) & 0x7fffffffu;
+        m = max(m, w < 0x7f800000u && x.at(i, bad) >= 0 ? w : 0u);
+    }
     m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
     __syncthreads();
     if (threadIdx.x < 32) {
         m = __reduce_max_sync(0xffffffffu, sm[threadIdx.x]);
         const int e = (int)(m >> 23);  // biased exponent
-        const bool use = e > 30 && e < 255;
+        const bool use = e > 30;
         const int k = use ? 14 - (e - 127) : 0;
         if (threadIdx.x == 0) {
             scale[0] = exp2f((float)k);
@@ -635,8 +640,8 @@ static int backward(const drift_xent *op, const float *lse, const float *g, int6
     const bool one = g_stride == 0;
     float *scale = BF16 || one ? nullptr : reinterpret_cast<float *>(ws + p.scale);
     if (scale) {
-        const int rc = launch_pdl(xent_scale_kernel, dim3(1), 1024, 0, st, 0, g, g_stride, n_t,
-                                  scale);
+        const int rc = launch_pdl(xent_scale_kernel, dim3(1), 1024, 0, st, 0, g, g_stride, rows,
+                                  n_t, scale);
         if (rc) return rc;
     }
     const float fixed = !BF16 && one ? 32768.0f : 1.0f;

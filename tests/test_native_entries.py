@@ -126,3 +126,55 @@ def test_strided_weights(t, dep, v, dt, stride):
     check_grads(x, w, tg, b, g, want)
     for a, c in zip(Entry(x, w, tg, b).gradients(lse, apart, stride), want):
         assert torch.equal(a, c)
+
+
+@gpu
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("weight", [1e30, 3e38, float("inf"), float("nan")])
+@pytest.mark.parametrize("t,dep,v", [(65, 40, 257), (300, 72, 1000)])
+def test_weights_of_ignored_rows_change_nothing(t, dep, v, dt, weight):
+    """Nor those of rows whose target is outside the vocabulary. (float16 holds the
+    logits' gradient times a power of two that the weights choose.)"""
+    x, w, tg, b = inputs(t, dep, v, dt, ignored=0.3, seed=2)
+    tg[5] = v + 3
+    off = (tg == IG) | (tg >= v)
+    _, lse = d.linear_xent_dev(x, w, tg, bias=b)
+    with pytest.raises(d.DriftError):
+        d.check_dev()
+    g = torch.randn(t, device="cuda")
+    clean, dirty = g.masked_fill(off, 0.0), g.masked_fill(off, weight)
+    want = d.linear_xent_grad_dev(x, w, tg, lse, clean, bias=b)
+    valid = torch.where(off, IG, tg)
+    check_grads(x, w, valid, b, clean, want)
+    for a, c in zip(d.linear_xent_grad_dev(x, w, tg, lse, dirty, bias=b), want):
+        assert torch.equal(a, c)
+
+
+@gpu
+@pytest.mark.parametrize("dt", list(DT))
+def test_weights_of_rows_that_are_all_ignored(dt):
+    x, w, _, b = inputs(40, 64, 300, dt)
+    tg = torch.full((40,), IG, device="cuda")
+    _, lse = d.linear_xent_dev(x, w, tg, bias=b)
+    for weight in (1.0, 1e30, float("inf"), float("nan")):
+        for a in d.linear_xent_grad_dev(x, w, tg, lse, torch.full((40,), weight, device="cuda"),
+                                        bias=b):
+            assert not a.any()
+
+
+@gpu
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("weight", [float("inf"), float("nan")])
+def test_a_weight_that_is_not_finite_spoils_its_own_row_of_dx(dt, weight):
+    """The others are as with 0 there, small weights as a mean's among them."""
+    x, w, tg, b = inputs(65, 40, 257, dt, ignored=0.0, seed=3)
+    _, lse = d.linear_xent_dev(x, w, tg, bias=b)
+    g = torch.rand(65, device="cuda") * 1e-6
+    g[7] = 0.0
+    want = d.linear_xent_grad_dev(x, w, tg, lse, g, bias=b)
+    check_grads(x, w, tg, b, g, want)
+    g[7] = weight
+    dx = d.linear_xent_grad_dev(x, w, tg, lse, g, bias=b)[0]
+    assert not torch.isfinite(dx[7]).any()
+    dx[7] = want[0][7]
+    assert torch.equal(dx, want[0])
