@@ -1225,6 +1225,8 @@ int drift_mx4_quantize_dev(drift_ctx *ctx, const drift_policy *p, int rounding, 
     if (misaligned(d_codes, 16) || misaligned(d_scales, 16) || misaligned(d_codes_t, 16) ||
         misaligned(d_scales_t, 16))
         return fail(DRIFT_EINVAL, "codes and scales must be 16-byte aligned");
+    if (misaligned(d_rng_state, 8) || misaligned(d_clamped, 8) || misaligned(d_clamped_t, 8))
+        return fail(DRIFT_EINVAL, "misaligned Rng state or counter");
     const int rc = launch_mx4_quantize(
         p->mx_headroom, rounding, type, d_src, rows, cols, rows > 1 ? row_stride : cols, d_codes,
         d_scales, d_codes_t, d_scales_t, d_rng_state, (unsigned long long *)d_clamped,
@@ -1313,6 +1315,8 @@ int drift_linear_xent_dev(drift_ctx *ctx, const drift_xent *op, float *d_loss, f
     int rc = check_xent(op);
     if (rc) return rc;
     if (op->tokens && !d_lse) return fail(DRIFT_EINVAL, "null pointer");
+    if (misaligned(d_loss, 4) || misaligned(d_lse, 4) || misaligned(d_mean, 4))
+        return fail(DRIFT_EINVAL, "misaligned output");
     if (!d_ws || ws_bytes < xent_workspace(op, 0) || misaligned(d_ws, 256))
         return fail(DRIFT_EINVAL, "workspace too small or misaligned");
     rc = launch_xent(op, d_loss, d_lse, d_mean, d_ws, ctx->d_err(), pick(ctx, stream));
@@ -1331,8 +1335,9 @@ int drift_linear_xent_grad_dev(drift_ctx *ctx, const drift_xent *op, const float
         return fail(DRIFT_EINVAL, "bad arguments");
     if ((d_dx && dx_stride < op->depth) || (d_dw && dw_stride < op->depth))
         return fail(DRIFT_EINVAL, "bad stride");
-    if (misaligned(d_dx, 2) || misaligned(d_dw, 2) || misaligned(d_db, 4))
-        return fail(DRIFT_EINVAL, "misaligned gradient");
+    if (misaligned(d_dx, 2) || misaligned(d_dw, 2) || misaligned(d_db, 4) ||
+        misaligned(d_lse, 4) || misaligned(d_dloss, 4))
+        return fail(DRIFT_EINVAL, "misaligned gradient or log sums");
     if (!d_ws || ws_bytes < xent_workspace(op, 1) || misaligned(d_ws, 256))
         return fail(DRIFT_EINVAL, "workspace too small or misaligned");
     rc = launch_xent_grad(op, d_lse, d_dloss, dloss_stride, d_dx, dx_stride, d_dw, dw_stride,
@@ -1349,8 +1354,8 @@ int drift_linear_xent_mean_dev(drift_ctx *ctx, const drift_xent *op, float *d_me
     if (rc) return rc;
     if (!d_mean || (d_dx && dx_stride < op->depth) || (d_dw && dw_stride < op->depth))
         return fail(DRIFT_EINVAL, "bad arguments");
-    if (misaligned(d_dx, 2) || misaligned(d_dw, 2) || misaligned(d_db, 4))
-        return fail(DRIFT_EINVAL, "misaligned gradient");
+    if (misaligned(d_dx, 2) || misaligned(d_dw, 2) || misaligned(d_db, 4) || misaligned(d_mean, 4))
+        return fail(DRIFT_EINVAL, "misaligned gradient or mean");
     if (!d_ws || ws_bytes < xent_workspace(op, 2) || misaligned(d_ws, 256))
         return fail(DRIFT_EINVAL, "workspace too small or misaligned");
     rc = launch_xent_mean(op, d_mean, d_dx, dx_stride, d_dw, dw_stride, d_db, d_ws, ctx->d_err(),
@@ -1364,7 +1369,8 @@ int drift_adamw_dev(drift_ctx *ctx, const drift_adamw *h, const drift_adamw_tens
     DeviceScope scope(ctx);
     if (scope.status) return scope.status;
     if (!h || count < 0 || (count && !tensors) || !d_step || !d_scalars ||
-        misaligned(d_scalars, 8))
+        misaligned(d_scalars, 8) || misaligned(d_step, 8) || misaligned(d_lr, 4) ||
+        misaligned(d_grad_scale, 4) || misaligned(d_rng_state, 8))
         return fail(DRIFT_EINVAL, "bad arguments");
     if ((h->state_bits != 32 && h->state_bits != 8) ||
         !(h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1 &&

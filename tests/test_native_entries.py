@@ -178,3 +178,41 @@ def test_a_weight_that_is_not_finite_spoils_its_own_row_of_dx(dt, weight):
     assert not torch.isfinite(dx[7]).any()
     dx[7] = want[0][7]
     assert torch.equal(dx, want[0])
+
+
+# ------------------------------------------------------------------ addresses
+
+@gpu
+def test_misaligned_addresses_are_refused():
+    """Before any launch: every output, counter and scalar at its type's alignment."""
+    ctx, st = d.Context.current().handle, torch.cuda.current_stream().cuda_stream
+    x, w, tg, b = inputs(5, 64, 96, ignored=0.0)
+    op, buf = xent_op(x, w, tg, b), torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    n = [workspace_bytes(op, m) for m in range(3)]
+    ws = torch.empty(max(n), dtype=torch.uint8, device="cuda").data_ptr()
+    at = lambda k: buf.data_ptr() + 4096 * k  # noqa: E731
+    p = d.policies.by_name("mxfp4").to_c()
+    h = _lib.DriftAdamW(1e-3, 0.9, 0.999, 1e-8, 0.01, 8, int(d.Rounding.STOCHASTIC))
+    table = (_lib.DriftAdamWTensor * 1)(_lib.DriftAdamWTensor(
+        at(8), at(9), at(10), at(11), at(12), at(13), None, 64, native._F32, native._F32))
+    entries = [
+        # entry, arguments, and the bytes by which each pointer among them may not be off
+        (LIB.drift_mx4_quantize_dev,
+         [ctx, p, 2, native._BF16, x.data_ptr(), 5, 64, 64, at(0), at(1), at(2), at(3), at(4), at(5),
+          at(6), st], {4: 1, 8: 8, 9: 8, 10: 8, 11: 8, 12: 4, 13: 4, 14: 4}),
+        (LIB.drift_linear_xent_dev, [ctx, op, at(0), at(1), at(2), ws, n[0], st],
+         {2: 2, 3: 2, 4: 2, 5: 128}),
+        (LIB.drift_linear_xent_grad_dev,
+         [ctx, op, at(0), at(1), 1, at(2), 64, at(4), 64, at(8), ws, n[1], st],
+         {2: 2, 3: 2, 5: 1, 7: 1, 9: 2, 10: 128}),
+        (LIB.drift_linear_xent_mean_dev, [ctx, op, at(0), at(1), 64, at(4), 64, at(8), ws, n[2], st],
+         {2: 2, 3: 1, 5: 1, 7: 2, 8: 128}),
+        (LIB.drift_adamw_dev, [ctx, h, table, 1, at(0), at(1), at(2), at(3), at(4), st],
+         {4: 4, 5: 4, 6: 2, 7: 2, 8: 4})]
+    for entry, args, off in entries:
+        for k, by in off.items():
+            bad = list(args)
+            bad[k] += by
+            assert entry(*bad) == _lib.EINVAL, (entry.__name__, k)
+        _lib.check(entry(*args))
+    d.check_dev()
