@@ -44,9 +44,10 @@ def _start():
     global torch, _LIB
     import torch as _torch
 
-    torch, _LIB = _torch, _lib.load()
-    _TYPES.update({torch.float64: _F64, torch.float32: _F32, torch.bfloat16: _BF16,
-                   torch.float16: _FP16})
+    _LIB = _lib.load()
+    _TYPES.update({_torch.float64: _F64, _torch.float32: _F32, _torch.bfloat16: _BF16,
+                   _torch.float16: _FP16})
+    torch = _torch  # last: whoever finds it set, on any thread, finds the rest
 
 
 def _types():

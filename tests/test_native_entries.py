@@ -216,3 +216,23 @@ def test_misaligned_addresses_are_refused():
             assert entry(*bad) == _lib.EINVAL, (entry.__name__, k)
         _lib.check(entry(*args))
     d.check_dev()
+
+
+# ------------------------------------------------------------------ first use
+
+
+def test_the_first_use_is_published_last(monkeypatch):
+    """Another thread takes a `torch` that is set for all of it being set."""
+    seen = []
+
+    class Table(dict):
+        def update(self, *a):
+            seen.append(native.torch)
+            super().update(*a)
+
+    monkeypatch.setattr(native, "torch", None)
+    monkeypatch.setattr(native, "_LIB", None)
+    monkeypatch.setattr(native, "_TYPES", Table())
+    native._start()
+    assert seen == [None] and native.torch is torch and native._LIB is not None
+    assert native._TYPES[torch.float16] == native._FP16
