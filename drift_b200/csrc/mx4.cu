@@ -24,6 +24,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <math_constants.h>
 
 #include "codec.cuh"
 #include "internal.h"
@@ -791,7 +792,8 @@ __device__ __forceinline__ float2 mx_pair(unsigned byte) {
 }
 
 // Eight values a thread. A double, float or bf16 holds every value exactly,
-// except that 2^127 times 2 or more overflows float and bf16; fp16 rounds.
+// except that 2^127 times 2 or more overflows float and bf16; fp16 rounds. The scale
+// byte 255 is E8M0's NaN here as in the tensor cores.
 template <class T>
 __global__ void __launch_bounds__(256) mx4_values_kernel(const uint8_t *codes,
                                                          const uint8_t *scales, int64_t rows,
@@ -811,11 +813,12 @@ __global__ void __launch_bounds__(256) mx4_values_kernel(const uint8_t *codes,
             for (int j = 0; j < 4; j++) {
                 const float2 f = mx_pair(w >> (8 * j) & 0xffu);
                 if constexpr (sizeof(T) == 8) {
-                    const double up = pow2(shared);
+                    const double up = shared < 128 ? pow2(shared) : CUDART_NAN;
                     v[2 * j] = f.x * up, v[2 * j + 1] = f.y * up;
                 } else {
-                    const float up = shared > -127 ? __uint_as_float((unsigned)(shared + 127) << 23)
-                                                   : 0x1p-127f;
+                    const float up = shared == 128   ? CUDART_NAN_F
+                                     : shared > -127 ? __uint_as_float((unsigned)(shared + 127) << 23)
+                                                     : 0x1p-127f;
                     v[2 * j] = T(f.x * up), v[2 * j + 1] = T(f.y * up);
                 }
             }

@@ -178,8 +178,8 @@ class Mx4:
     def from_parts(codes, scales, cols: Optional[int] = None) -> "Mx4":
         """From plain arrays, as a file holds them: `codes` uint8 (rows, ceil(cols/32)*16),
         the even element in the low nibble, and `scales`
-        uint8 (rows, ceil(cols/32)), exponent + 127, none of them 255. Both are
-        copied; codes past `cols` are read as 0."""
+        uint8 (rows, ceil(cols/32)), exponent + 127; 255 makes its block NaN. Both
+        are copied; codes past `cols` are read as 0."""
         if torch is None:
             _start()
         rows, blocks = scales.shape

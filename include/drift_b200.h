@@ -538,7 +538,8 @@ DRIFT_API int drift_adam_dev(drift_ctx *ctx, double *d_param, const double *d_gr
  * `scales`: exponent + 127, in tiles of 128 rows x 4 blocks of 512 bytes where
  * row r, block b is byte (r % 32) * 16 + (r / 32) * 4 + b; a row of tiles has
  * ceil(cols / 256) * 2 of them; padding bytes are 127; 16-byte aligned. The
- * scale byte 255 is not used.
+ * cast never writes the scale byte 255; E8M0's NaN, it makes its block NaN in
+ * products and in values read back.
  */
 typedef struct drift_mx4 {
     int64_t rows, cols;

@@ -236,3 +236,43 @@ def test_the_first_use_is_published_last(monkeypatch):
     native._start()
     assert seen == [None] and native.torch is torch and native._LIB is not None
     assert native._TYPES[torch.float16] == native._FP16
+
+
+# ------------------------------------------------------------------ the scale byte 255
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16, torch.float16])
+def test_the_scale_byte_255_reads_as_nan(dtype):
+    """E8M0's NaN: its block's values are NaN in every type, and no other block's."""
+    gen = torch.Generator().manual_seed(3)
+    codes = torch.randint(0, 256, (5, 3 * 16), dtype=torch.uint8, generator=gen).cuda()
+    scales = torch.full((5, 3), 127, dtype=torch.uint8, device="cuda")
+    plain = d.mx4_dequantize_dev(d.Mx4.from_parts(codes, scales, 90), dtype=dtype)
+    scales[2, 1] = 255
+    got = d.mx4_dequantize_dev(d.Mx4.from_parts(codes, scales, 90), dtype=dtype)
+    assert torch.isnan(got[2, 32:64]).all()
+    got[2, 32:64] = plain[2, 32:64]
+    assert torch.equal(got, plain)
+
+
+@gpu
+@pytest.mark.parametrize("m", [5, 40, 200, 5000])
+def test_products_of_the_scale_byte_255_are_nan(m):
+    """Whichever side holds it; its row (column) alone."""
+    gen = torch.Generator().manual_seed(4)
+    n, k = 600, 300
+    codes = [torch.randint(0, 256, (r, 160), dtype=torch.uint8, generator=gen).cuda() for r in (m, n)]
+    scales = [torch.full((r, 10), 127, dtype=torch.uint8, device="cuda") for r in (m, n)]
+    a, b = (d.Mx4.from_parts(c, s, k) for c, s in zip(codes, scales))
+    plain = d.mx4_gemm_dev(a, b)
+    assert torch.isfinite(plain).all()
+    scales[0][3, 2] = scales[1][577, 9] = 255
+    bad = [d.Mx4.from_parts(c, s, k) for c, s in zip(codes, scales)]
+    got = d.mx4_gemm_dev(bad[0], b)
+    assert torch.isnan(got[3]).all()
+    got[3] = plain[3]
+    assert torch.equal(got, plain)
+    got = d.mx4_gemm_dev(a, bad[1])
+    assert torch.isnan(got[:, 577]).all()
+    got[:, 577] = plain[:, 577]
+    assert torch.equal(got, plain)
