@@ -337,12 +337,24 @@ struct CopyRows {
     const uint4 *from;  // null: no copy
     uint4 *to;
     int64_t from_ld, to_ld, units;  // in units of 16 bytes
+    int last;                       // elements of x in a row's last unit
     __device__ __forceinline__ void copy_row(int64_t row, bool on) const {
         if (!from) return;
         const uint4 *f = from + row * from_ld;
         uint4 *t = to + row * to_ld;
-        for (int64_t i = threadIdx.x; i < units; i += blockDim.x)
-            t[i] = on ? f[i] : make_uint4(0, 0, 0, 0);
+        for (int64_t i = threadIdx.x; i < units; i += blockDim.x) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (on && (i + 1 < units || last == 8)) {
+                w = f[i];
+            } else if (on) {  // the row's memory may end with its last element
+                const uint16_t *h = reinterpret_cast<const uint16_t *>(f + i);
+                unsigned *u = reinterpret_cast<unsigned *>(&w);
+#pragma unroll
+                for (int j = 0; j < 7; j++)
+                    if (j < last) u[j / 2] |= (unsigned)h[j] << (j & 1) * 16;
+            }
+            t[i] = w;
+        }
     }
 };
 __global__ void __launch_bounds__(128) xent_copy_kernel(CopyRows xs, XentRows x) {
@@ -567,10 +579,10 @@ static int launch_mean(const float *row_loss, int64_t n, const XentRows &rows, f
                       mean, inv);
 }
 
-// x's rows are whole units of 16 bytes (its stride is), and so are the copy's.
+// x's rows start on 16-byte boundaries (its stride is whole units), and so do the copy's.
 static CopyRows copy_rows(const drift_xent *op, void *to, int64_t to_ld) {
     return CopyRows{static_cast<const uint4 *>(op->x), static_cast<uint4 *>(to), op->x_stride / 8,
-                    to_ld / 8, (op->depth + 7) / 8};
+                    to_ld / 8, (op->depth + 7) / 8, (int)((op->depth - 1) % 8) + 1};
 }
 
 static int done() { return cudaGetLastError() == cudaSuccess ? DRIFT_OK : DRIFT_ECUDA; }

@@ -276,3 +276,29 @@ def test_products_of_the_scale_byte_255_are_nan(m):
     assert torch.isnan(got[:, 577]).all()
     got[:, 577] = plain[:, 577]
     assert torch.equal(got, plain)
+
+
+# ------------------------------------------------------------------ strided views of x
+
+@gpu
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("t,v", [(65, 257), (70, 33000)])
+@pytest.mark.parametrize("dep", [1, 37, 44])
+def test_columns_past_the_depth_are_not_read(t, v, dep, dt):
+    """A row ends at its depth, the last one perhaps the buffer with it: what follows
+    shows up nowhere, nor in the copy of x that the gradients make."""
+    x, w, tg, b = inputs(t, dep, v, dt)
+    wide = torch.full((t, 48), 0x7b7b, dtype=torch.int16, device="cuda").view(DT[dt])
+    wide[:, :dep] = x
+    wp = torch.zeros(v, 48, dtype=DT[dt], device="cuda")
+    wp[:, :dep] = w
+    _, lse = d.linear_xent_dev(x, w, tg, bias=b)
+    g = torch.randn(t, device="cuda")
+    want = d.linear_xent_grad_dev(x, w, tg, lse, g, bias=b)
+    mean = d.linear_xent_mean_dev(x, w, tg, bias=b)
+    e = Entry(wide[:, :dep], wp[:, :dep], tg, b)
+    e.dx, e.dw = torch.empty_like(x), torch.empty_like(w)
+    for call, ref, mode in ((lambda: e.gradients(lse, g, 1), want, 1), (e.mean, mean, 2)):
+        assert all(torch.equal(a, c) for a, c in zip(call(), ref))
+        words = e.buf[:workspace_bytes(e.op, mode) // 2 * 2].view(torch.int16) == 0x7b7b
+        assert not (words[:-2] & words[1:-1] & words[2:]).any()
