@@ -7,7 +7,7 @@ import pytest
 
 import drift_b200 as d
 from drift_b200 import _lib, native
-from tests.test_native_xent import DT, IG, check_grads, inputs
+from tests.test_native_xent import DT, IG, check_grads, check_losses, exact, inputs, logit_error
 
 torch = pytest.importorskip("torch")
 gpu = pytest.mark.gpu
@@ -302,3 +302,96 @@ def test_columns_past_the_depth_are_not_read(t, v, dep, dt):
         assert all(torch.equal(a, c) for a, c in zip(call(), ref))
         words = e.buf[:workspace_bytes(e.op, mode) // 2 * 2].view(torch.int16) == 0x7b7b
         assert not (words[:-2] & words[1:-1] & words[2:]).any()
+
+
+# ------------------------------------------------------------------ padding
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(1, 1), (129, 257), (300, 1000), (257, 40), (1500, 1025)])
+@pytest.mark.parametrize("axis", [0, 1, None])
+@pytest.mark.parametrize("dt", [torch.float64, torch.float32, torch.bfloat16])
+def test_every_padding_byte_is_written(rows, cols, axis, dt):
+    """Into buffers of the caller's that hold 0xFF throughout: padding codes become 0
+    and padding scale bytes 127, and the bytes behind either array stay."""
+    gen = torch.Generator().manual_seed(rows + cols)
+    x = torch.randn(rows, cols, generator=gen, dtype=torch.float64).to(dt).cuda()
+    kinds = {torch.float64: native._F64, torch.float32: native._F32, torch.bfloat16: native._BF16}
+    held, call = [], []
+    for r, c, on in ((rows, cols, axis != 0), (cols, rows, axis != 1)):
+        sizes = (ctypes.c_int64(), ctypes.c_int64())
+        _lib.check(LIB.drift_mx4_sizes(r, c, *sizes))
+        bufs = [torch.full((s.value + 4096,), 255, dtype=torch.uint8, device="cuda") for s in sizes]
+        call += [b.data_ptr() if on else None for b in bufs]
+        if on:
+            held.append((r, c, *((b, s.value) for b, s in zip(bufs, sizes))))
+    _lib.check(LIB.drift_mx4_quantize_dev(
+        d.Context.current().handle, d.policies.by_name("mxfp4").to_c(), 0, kinds[dt], x.data_ptr(),
+        rows, cols, cols, *call, None, None, None, torch.cuda.current_stream().cuda_stream))
+    d.check_dev()
+    for r, c, (codes, nc), (scales, ns) in held:
+        assert (codes[nc:] == 255).all() and (scales[ns:] == 255).all()
+        nib = torch.stack((codes[:nc] & 15, codes[:nc] >> 4), -1).view(r, -1)
+        assert not nib[:, c:].any()
+        # Every byte, padding included, as from_parts lays the plain scales out.
+        q = d.Mx4(codes[:nc], scales[:ns].clone(), r, c)
+        again = d.Mx4.from_parts(*q.to_parts(), cols=c)
+        assert torch.equal(again.scales, scales[:ns])
+
+
+# ------------------------------------------------------------------ vocabularies of several pieces
+
+def check_pieces(x, w, tg, b, g, loss, lse, grads, rows=1 << 16):
+    """check_losses and check_grads, rows at a time: dw's and db's sums and bounds add up."""
+    half, tiny = torch.finfo(x.dtype).eps / 2, 2.0 ** -25 if x.dtype == torch.float16 else 0.0
+    W = w.double().abs()
+    t, dep = x.shape
+    ww, lw = torch.zeros_like(W), torch.zeros_like(W)
+    wb, lb = (torch.zeros(len(w), dtype=torch.float64, device="cuda") for _ in range(2))
+    floor = 2.0 ** -38 * float(g.abs().max()) if x.dtype == torch.float16 else 0.0
+    dx, dw, db = grads
+    for a in range(0, t, rows):
+        c = slice(a, a + rows)
+        X, T, G = x[c], tg[c], g[c]
+        check_losses(X, w, T, b, loss[c], lse[c])
+        _, z, p, dl, wx, dw1, db1 = exact(X, w, T, b, G)
+        e = logit_error(X, w, b)
+        e = e + e.amax(1, keepdim=True) + 2.0 ** -17 + 2.0 ** -22 * z.abs()[:, None]
+        on = (G.double().abs() * (T != IG))[:, None]
+        soft = p * torch.expm1(e.clamp(max=10.0)) * on + 2.0 ** -22 * dl.abs()
+        el = soft + half * (dl.abs() + soft) + floor * (on > 0)
+        lim = (el + (len(w) + 2) * 2.0 ** -23 * dl.abs()) @ W
+        assert ((dx[c].double() - wx).abs() <= lim + half * (wx.abs() + lim) + tiny).all()
+        assert not dx[c][T == IG].any()
+        ww += dw1
+        lw += (el + (t + 2) * 2.0 ** -23 * dl.abs()).T @ X.double().abs()
+        wb += db1
+        lb += (soft + (t + 2) * 2.0 ** -23 * dl.abs()).sum(0)
+    assert ((dw.double() - ww).abs() <= lw + half * (ww.abs() + lw) + tiny).all()
+    assert ((db.double() - wb).abs() <= lb).all()
+
+
+@gpu
+@pytest.mark.parametrize("t,dep,v,dt", [
+    (600, 72, 250_001, "bf16"), (600, 72, 250_001, "f16"),  # gradients: two pieces, dx in parts
+    ((1 << 20) + 3, 24, 2600, "bf16")])  # the loss: three pieces; gradients: eleven
+def test_vocabularies_of_several_pieces(t, dep, v, dt):
+    """Row statistics run on from piece to piece, the target lies in any of them, dx adds
+    up over them, and the last one is short."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB free")
+    x, w, tg, b = inputs(t, dep, v, dt, seed=12)
+    g = torch.randn(t, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    loss, lse = d.linear_xent_dev(x, w, tg, bias=b)
+    got = d.linear_xent_grad_dev(x, w, tg, lse, g, bias=b)
+    check_pieces(x, w, tg, b, g, loss, lse, got)
+    again = d.linear_xent_grad_dev(x, w, tg, lse, g, bias=b)
+    assert all(torch.equal(a, c) for a, c in zip(got, again))
+    mean, *got = d.linear_xent_mean_dev(x, w, tg, bias=b)
+    n = int((tg != IG).sum())
+    # Positive losses, t / 1024 additions a thread, then 5 in a warp and 32 over them.
+    want = float(loss.double().sum()) / n
+    assert abs(float(mean) - want) <= (t / 1024 + 40) * 2.0 ** -24 * want
+    inv = torch.tensor([1.0 / n], device="cuda")
+    for a, c in zip(got, d.linear_xent_grad_dev(x, w, tg, lse, inv, bias=b)):
+        assert torch.equal(a, c)
+    d.check_dev()
