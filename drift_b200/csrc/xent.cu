@@ -475,6 +475,11 @@ static int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 static int tiles(int64_t x) { return (int)((x + tc::kTile - 1) / tc::kTile); }
 static int stages(int64_t k) { return (int)((k + 63) / 64); }
 
+// Pairs of SMs that the plans cut contractions for: a B200's, and not the current
+// device's, which need not be the context's when a workspace's size is asked for. (The
+// launches then ask for the device's own.)
+constexpr int kPlanPairs = 74;
+
 // The forward pass holds 16 bytes a row and 256 columns; pieces keep that near
 // 64 MB.
 struct ForwardPlan {
@@ -510,7 +515,7 @@ static GradPlan grad_plan(const drift_xent *op) {
     // to 16 stages (1024 entries) a part.
     const int dx_tiles = tiles(t) * tiles(op->depth);
     const int most = std::max(1, stages(p.ld) / 16);
-    p.splits = std::max(1, std::min(most, 74 / dx_tiles));
+    p.splits = std::max(1, std::min(most, kPlanPairs / dx_tiles));
     p.direct = p.pieces == 1 && p.splits == 1;
     p.acc_ld = up(op->depth, 4);
     p.part = t * p.acc_ld;
@@ -545,8 +550,8 @@ static KeptPlan kept_plan(const drift_xent *op) {
     // Few tiles: the contractions are cut, down to two stages a part here, where a
     // part is a pass over the logits in L2, and 16 for dx.
     const int lt = tiles(t) * tiles(op->vocab), dt = tiles(t) * tiles(op->depth);
-    p.splits = std::max(1, std::min({stages(op->depth) / 2, 74 / lt, 16}));
-    p.dx_splits = std::max(1, std::min(stages(op->vocab) / 16, 74 / dt));
+    p.splits = std::max(1, std::min({stages(op->depth) / 2, kPlanPairs / lt, 16}));
+    p.dx_splits = std::max(1, std::min(stages(op->vocab) / 16, kPlanPairs / dt));
     p.logits = 0;
     p.d = up(p.splits * p.part * 4, 256);
     p.loss = p.d + up(p.part * 2, 256);
