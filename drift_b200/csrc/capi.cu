@@ -1189,10 +1189,11 @@ static unsigned type_bytes(int type) {  // DRIFT_T_*
     return type == DRIFT_T_F64 ? 8 : type == DRIFT_T_F32 ? 4 : 2;
 }
 
-// Rows and columns that the packed form's 32-bit indices reach.
+// Rows and columns that the packed form's 32-bit indices reach, the last step of a grid's
+// loop (2^17 at most) included.
 static bool mx4_shape_ok(int64_t rows, int64_t cols) {
     return rows >= 0 && cols >= 0 && rows < (1LL << 31) && cols < (1LL << 31) &&
-           ((rows + 127) / 128 * 128) * ((cols + 255) / 256) < (1LL << 32);
+           ((rows + 127) / 128 * 128) * ((cols + 255) / 256) <= (1LL << 32) - (1LL << 17);
 }
 
 int drift_mx4_sizes(int64_t rows, int64_t cols, int64_t *code_bytes, int64_t *scale_bytes) {

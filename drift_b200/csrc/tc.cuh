@@ -500,7 +500,7 @@ inline int launch(const Args &args, const Epi &epi, int sms, cudaStream_t st) {
     static unsigned long long done = 0;
     if (!allow_smem(kernel, smem_bytes<KIND>(), done)) return DRIFT_ECUDA;
     const int64_t total = (int64_t)args.m_tiles * args.n_tiles * args.splits;
-    if (total > 0x7fffffff) return DRIFT_EINVAL;
+    if (total > 0x7fffffff - sms) return DRIFT_EINVAL;  // the kernel steps past it once
     const int pairs = (int)(total < sms / 2 ? total : sms / 2);
     return launch_pdl(kernel, dim3(pairs * 2), kThreads, smem_bytes<KIND>(), st, 0, args, epi);
 }

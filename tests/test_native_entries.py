@@ -395,3 +395,13 @@ def test_vocabularies_of_several_pieces(t, dep, v, dt):
     for a, c in zip(got, d.linear_xent_grad_dev(x, w, tg, lse, inv, bias=b)):
         assert torch.equal(a, c)
     d.check_dev()
+
+
+# ------------------------------------------------------------------ the longest sides
+
+@pytest.mark.parametrize("rows,cols,fits", [
+    ((1 << 31) - (1 << 17), 257, True), ((1 << 31) - 128, 257, False),
+    (((1 << 32) - (1 << 17)) // 4, 1024, True), ((1 << 30) - 128, 1024, False)])
+def test_packed_sizes_leave_a_stride_below_32_bits(rows, cols, fits):
+    """The cast counts chunks of 256 elements in 32 bits, a grid's stride at a time."""
+    assert LIB.drift_mx4_sizes(rows, cols, None, None) == (0 if fits else _lib.EINVAL)
