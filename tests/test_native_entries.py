@@ -405,3 +405,43 @@ def test_vocabularies_of_several_pieces(t, dep, v, dt):
 def test_packed_sizes_leave_a_stride_below_32_bits(rows, cols, fits):
     """The cast counts chunks of 256 elements in 32 bits, a grid's stride at a time."""
     assert LIB.drift_mx4_sizes(rows, cols, None, None) == (0 if fits else _lib.EINVAL)
+
+
+# ------------------------------------------------------------------ several chunks a warp
+
+@gpu
+@pytest.mark.parametrize("kind", ["nearest", "truncate", "stochastic"])
+@pytest.mark.parametrize("dt", [torch.float64, torch.float32, torch.bfloat16, torch.float16])
+def test_long_casts_equal_their_rows(dt, kind):
+    """A matrix whose warps take several chunks of a row, with Inf, zeros and signed
+    zeros in it, against its rows cast one by one: codes, scales and clamps. Element (i, j)
+    uses draw i * cols + j."""
+    rows, cols, seed, golden = 900, 2090, 0x0123456789ABCDEF, 0x9E3779B97F4A7C15
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    x = torch.randn(rows, cols, device="cuda", generator=gen, dtype=torch.float64)
+    x *= torch.randn(rows, cols, device="cuda", generator=gen, dtype=torch.float64).exp()
+    x = x.to(dt)
+    x[::37, ::101] = float("inf")
+    x[5::41, 3::97] = float("-inf")
+    x[11] = 0.0
+    x[12, 64:128] = -0.0
+    p = d.policies.by_name("mxfp4")
+    rm = {"nearest": d.Rounding.NEAREST_EVEN, "truncate": d.Rounding.TRUNCATE,
+          "stochastic": d.Rounding.STOCHASTIC}[kind]
+
+    def signed(k):
+        k &= 2 ** 64 - 1
+        return k - (k >> 63 << 64)
+
+    st = torch.tensor([seed], dtype=torch.int64, device="cuda")
+    clamps, each = (torch.zeros(1, dtype=torch.int64, device="cuda") for _ in range(2))
+    q = d.mx4_quantize_dev(p, x, rm, d_rng_state=st, d_clamped=clamps)
+    assert int(st) == (signed(seed + rows * cols * golden) if kind == "stochastic" else seed)
+    starts = torch.tensor([signed(seed + i * cols * golden) for i in range(rows)], device="cuda")
+    got, scale = q.to_parts()
+    for i in range(rows):
+        one = d.mx4_quantize_dev(p, x[i:i + 1], rm, d_rng_state=starts[i:i + 1], d_clamped=each)
+        c, s = one.to_parts()
+        assert torch.equal(got[i], c[0]) and torch.equal(scale[i], s[0])
+    assert torch.equal(clamps, each)
+    d.check_dev()
