@@ -30,8 +30,9 @@
 // queued between them, 60 cycles each: 3.8 and 3.4; copied with tcgen05.st by warps
 // of their own, 2.7 and 2.5). The tensor pipe is busy 63 to 68 % of KIND_16's time at
 // 2048 x 32768 x 4096 under the counters' cold caches, DRAM 9 to 16 %. By count shared
-// memory is the next bound: a stage is written once and read by both CTAs' MMAs,
-// 64 KiB in their 512 cycles, at 128 bytes a cycle all there is.
+// memory is near its limit: a stage is written once and read by both CTAs' MMAs,
+// 64 KiB in their 512 cycles, at 128 bytes a cycle all there is. No counter has shown
+// that it is what holds KIND_MX4, whose pipe is busy 48 % of the time.
 //
 // Every wait is bounded; one that gives up flags DEV_ERR_TIMEOUT and the
 // kernel drains and returns.

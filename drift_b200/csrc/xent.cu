@@ -16,8 +16,10 @@
 //   gradient  a piece of the vocabulary at a time: the logits again, whose
 //             epilogue writes d in the inputs' type (one rounding, which halves
 //             its bytes and feeds the tensor cores; an element's error is half a
-//             unit of that type, as the results' own), then dx += d W and
-//             dW = d^T x from it, reading d and W where they lie (MN-major).
+//             unit of that type, as the results' own: theirs, relative, grows from
+//             1.65e-3 to 1.98e-3 at 64 x 2048 x 96 and stays at 1.7e-3 at 4096 x
+//             131072 x 4096), then dx += d W and dW = d^T x from it, reading d and W
+//             where they lie (MN-major).
 //
 // fp16 holds d times a power of two (2^15, or with weights by row one that brings
 // the largest finite |g| of the rows that count near 2^15), so that small
@@ -27,7 +29,7 @@
 // Bound: the tensor cores for many tokens (8 T D V operations with the
 // gradient's second computation of the logits, against 6 T D V if they were
 // kept); the bytes of W for few. Measured on one B200: 4096 tokens x 131072 entries
-// x 4096 with gradients in 14.2 to 15.2 ms (1.16 to 1.24 PFLOP/s under the power
+// x 4096 with gradients in 14.2 to 15.3 ms (1.15 to 1.24 PFLOP/s under the power
 // cap), the loss of 64 tokens x 131072 x 4096 in 224 us (4.8 TB/s).
 #include <algorithm>
 
@@ -39,7 +41,9 @@ namespace drift {
 
 // Stages of 64 summed in TMEM, whose sums truncate: 2^-18 of a logit's magnitude at
 // most over 16, which moves an fp32 loss by a few units; the gradients' products
-// round to 16 bits, so theirs may be longer.
+// round to 16 bits, so theirs may be longer. Measured on 1001 log sums, relative: 3.0e-7
+// at depths of 1024, 2048 and 4096 (with runs of 64 stages 3.0e-7, 6.6e-7 and 1.3e-6;
+// sums rounded to nearest at each step 3e-8).
 constexpr int kLogitRun = 16, kGradRun = 64;
 
 constexpr float kLog2e = 1.4426950408889634f;

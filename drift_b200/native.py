@@ -15,8 +15,11 @@ Every call runs on torch's current stream of the tensors' device unless
 `stream` is given, and on the calling thread's context (`Context.current()`)
 unless `ctx` is; the tensors must live on the context's device. Outputs and
 scratch come from torch's allocator under that stream, so calls may be
-captured into CUDA graphs. Errors that only the device sees (a NaN cast to
-e2m1, a target outside the vocabulary) are raised by `check_dev`.
+captured into CUDA graphs, after a first call on the thread (which opens its
+context). Errors that only the device sees (a NaN cast to e2m1, a target outside
+the vocabulary) are raised by `check_dev`; a graph reports its own to the context
+it was captured with, which has to stay open as long as it is replayed: a thread's
+own context closes with the thread.
 """
 from __future__ import annotations
 
@@ -431,8 +434,11 @@ class AdamW:
     moment itself and the root of the second. `rounding` then may be
     Rounding.STOCHASTIC, with d_rng_state (int64, one element).
 
-    The moments start at zero, or are `state`: [m, v] or [m, m_scale, r,
-    r_scale], each a list like `params`. The step count lives on the device
+    A gradient that is Inf or NaN leaves its moments so: in 8 bits its whole block of
+    256 reads as NaN from then on.
+
+    The moments start at zero (on the stream current at construction), or are `state`:
+    [m, v] or [m, m_scale, r, r_scale], each a list like `params`. The step count lives on the device
     (d_step, int64), so a captured step replays as the next one. `copies`
     (a list with None where there is none) receive the new parameters in their
     own type, for low-precision copies of float32 masters. All of them keep the

@@ -520,8 +520,9 @@ DRIFT_API int drift_adam_dev(drift_ctx *ctx, double *d_param, const double *d_gr
  * in the reference, except where a comment cites one. They allocate nothing
  * and keep nothing in the context but its error word: every scratch buffer is
  * the caller's, so calls on different streams, threads or captured graphs are
- * independent as long as they have different buffers. They leave the calling
- * thread's current device as it was. Pointers are device pointers of the
+ * independent as long as they have different buffers. A captured call reports to
+ * its context's error word whenever it is replayed: close the context after the
+ * graph. They leave the calling thread's current device as it was. Pointers are device pointers of the
  * context's device.
  */
 /* Element types of matrices that cross as void*. */
@@ -643,7 +644,9 @@ DRIFT_API int drift_linear_xent_mean_dev(drift_ctx *ctx, const drift_xent *op, f
  * state_bits 32: m and v are floats. state_bits 8: m and r are held as e4m3
  * codes with one float scale per 256 consecutive elements, code =
  * e4m3(x * (1 / amax * 448)), value = code * (amax * (1 / 448)), rounded to nearest or, with
- * `rounding` stochastic, by one draw an element in tensor order.
+ * `rounding` stochastic, by one draw an element in tensor order. A block whose
+ * magnitudes are all below 2^-100 is held as zeros with scale 1, one with an Inf or
+ * NaN as NaN.
  */
 typedef struct drift_adamw {
     double lr, beta1, beta2, eps, weight_decay;
