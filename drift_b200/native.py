@@ -219,7 +219,7 @@ def _mx4_policy(p: NumericPolicy):
     c = p.__dict__.get("_mx4")
     if c is None:
         if p.scaling != Scaling.MX_BLOCK or p.scale_block != 32 or \
-                Formats.E2M1 not in (p.input_format, p.grad_format):
+                Formats.E2M1.id not in (f.id for f in (p.input_format, p.grad_format) if f):
             raise ValueError("the packed cast needs a policy with e2m1 elements and MX blocks of "
                              "32")
         c = p.__dict__["_mx4"] = (p.to_c(), int(p.input_rounding))

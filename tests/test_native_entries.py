@@ -2,6 +2,7 @@
 Python layer ties together on their own, strides, buffers of the caller's that hold
 anything, and vocabularies of several pieces."""
 import ctypes
+import pickle
 
 import pytest
 
@@ -445,3 +446,14 @@ def test_long_casts_equal_their_rows(dt, kind):
         assert torch.equal(got[i], c[0]) and torch.equal(scale[i], s[0])
     assert torch.equal(clamps, each)
     d.check_dev()
+
+
+# ------------------------------------------------------------------ policies and views
+
+def test_a_policy_from_another_process_is_the_same_policy():
+    """Its formats are copies; what they are counts, not which."""
+    p = pickle.loads(pickle.dumps(d.policies.by_name("mxfp4-headroom").to_builder("p").build()))
+    c, rounding = native._mx4_policy(p)
+    assert c.mx_headroom == p.mx_headroom and rounding == int(p.input_rounding)
+    with pytest.raises(ValueError):
+        native._mx4_policy(pickle.loads(pickle.dumps(d.policies.by_name("fp8-mx"))))
