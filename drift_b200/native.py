@@ -245,6 +245,8 @@ def mx4_quantize_dev(p: NumericPolicy, src, rm: Optional[Rounding] = None, *,
         raise ValueError("src: expected a matrix")
     call = _Call(src, ctx)
     t = _type_of(src.dtype, "src")
+    if src.is_neg():
+        src = src.resolve_neg()
     rng = cl = cl_t = None
     if d_rng_state is not None:
         rng = call.ptr(d_rng_state, "d_rng_state", torch.int64, 1)
@@ -324,6 +326,8 @@ def _xent_rows(call: _Call, t, what: str):
     if t.dim() != 2:
         raise ValueError(f"{what}: expected a matrix")
     call.ptr(t, what, contiguous=False)
+    if t.is_neg():
+        t = t.resolve_neg()
     rows, d = t.shape
     s0, s1 = t.stride()
     if rows <= 1:

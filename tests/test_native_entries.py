@@ -457,3 +457,19 @@ def test_a_policy_from_another_process_is_the_same_policy():
     assert c.mx_headroom == p.mx_headroom and rounding == int(p.input_rounding)
     with pytest.raises(ValueError):
         native._mx4_policy(pickle.loads(pickle.dumps(d.policies.by_name("fp8-mx"))))
+
+
+@gpu
+@pytest.mark.parametrize("cols", [1, 40])
+def test_negated_views_are_cast_by_their_values(cols):
+    """The imaginary part of a conjugate is a view whose memory holds the opposite sign."""
+    z = torch.randn(50, cols, dtype=torch.complex64, device="cuda")
+    p = d.policies.by_name("mxfp4")
+    for x in (z.conj().imag, torch._neg_view(z.real.contiguous())):
+        for got, want in zip(d.mx4_quantize_dev(p, x, axis=None),
+                             d.mx4_quantize_dev(p, x.resolve_neg(), axis=None)):
+            assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    x, w, tg, b = inputs(50, cols, 96)
+    want = d.linear_xent_mean_dev(x, w, tg, bias=b)
+    got = d.linear_xent_mean_dev(torch._neg_view(-x), torch._neg_view(-w), tg, bias=b)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
